@@ -229,7 +229,7 @@ def _plain_logprobs(s):
     row = torch.float64 if x.dtype == torch.float64 else torch.float32
     zero = torch.zeros((), dtype=torch.float64, device="cuda")
     logp = torch.where(part, xa - torch.log(total), zero).to(row)
-    stats = torch.stack([m.to(row), torch.where(part, total, zero).to(row)], 1)
+    stats = torch.stack([m.to(row), (torch.where(part, total, zero) - 1).to(row)], 1)
     g = torch.where(part, s["grad_logp"], 0.0)
     h = torch.where(part, s["hess_logp"], 0.0) if s["hess"] else None
     grad, hess = _to_scores(e, total, at, part, g, h, torch.float32 if x.dtype == torch.float64 else x.dtype, s["hess"])
@@ -343,8 +343,8 @@ def _exact_rows(s, r0, r1):
     out = {"logp": x.new_zeros(n).index_put((rows,), lp.detach())}
     if s["op"] == "logprobs":
         top = torch.where(live, x.nan_to_num(nan=0.0, neginf=-math.inf).amax(1), 0.0)
-        total = torch.where(live, torch.exp(torch.logsumexp(x, 1) - top), 0.0)
-        out["stats"] = torch.stack([top, total], 1)
+        less_one = torch.where(live, torch.expm1(torch.logsumexp(x, 1) - top), -1.0)
+        out["stats"] = torch.stack([top, less_one], 1)
         d1 = take(s["grad_logp"]).double()[rows]
         d2 = take(s["hess_logp"]).double()[rows] if s["hess"] else None
         value, want = (lp * d1).sum(), True
