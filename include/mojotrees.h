@@ -326,6 +326,101 @@ int32_t mojotrees_b200_bin_csc(const int64_t *indptr, const int64_t *indices, co
  * No counterpart in the reference. */
 int32_t mojotrees_b200_check_quotients(int64_t n, uint64_t seed, int64_t *out_mismatches, MojoTreesError *error);
 
+/* ------------------------------------------------- losses from feedback
+ * Derivatives of losses whose training signal is feedback instead of labels:
+ * logged decisions with rewards, and pairs of which one was preferred.  The
+ * objectives of mojotrees_b200_train_*_policy and _preference, for callers
+ * that hold the scores on the device themselves.  No counterpart in the
+ * reference (its ranking objective needs query groups with graded labels).
+ *
+ * Every array is device memory that the caller owns, all of a call on one
+ * device; the work runs on `stream` (a cudaStream_t of that device; NULL =
+ * the legacy stream), whichever device is current.  The calls allocate
+ * nothing, wait for nothing, share no state and can be captured into a
+ * graph.  Outputs may not overlap inputs.
+ *
+ * scores[r * row_stride + k] is the raw score of class k in row r, of
+ * score_type; n_classes is at most 262144.  actions[r] is the class that row
+ * took (int32 or int64: action_bytes 4 or 8).  Per-row values ("row type")
+ * are double for float64 scores and float for the others; derivatives with
+ * respect to the scores are float for float64 and float32 scores and of the
+ * scores' type for 16-bit ones, at out[r * out_stride + k].  Classes with a
+ * score of -inf have probability 0.  A row whose action is negative, whose
+ * weight is 0 or whose scores are all -inf takes no part: its outputs are 0,
+ * whatever else the row holds.  An action of n_classes or more makes its
+ * row's outputs NaN. */
+#define MOJOTREES_B200_SCORE_F64 0
+#define MOJOTREES_B200_SCORE_F32 1
+#define MOJOTREES_B200_SCORE_F16 2
+#define MOJOTREES_B200_SCORE_BF16 3
+
+/* log softmax(scores)[action] per row (row type [n_rows]), and what its
+ * gradient needs (row type [n_rows][2]): the row's maximum, and the sum of
+ * exp(score - maximum) less 1 (0 and -1 for a row that takes no part). */
+int32_t mojotrees_b200_action_logprobs(const void* scores, int32_t score_type, int64_t n_rows, int64_t n_classes,
+                                       int64_t row_stride, const void* actions, int32_t action_bytes, void* out_logp,
+                                       void* out_stats, void* stream, MojoTreesError* error);
+
+/* Derivatives of a loss with respect to the scores from its first and second
+ * derivative g, h with respect to the log probabilities (float [n_rows]):
+ * with p = softmax(scores), grad = g ([k = action] - p_k) and
+ * hess = h ([k = action] - p_k)^2 + |g| p_k (1 - p_k), which is not negative
+ * for h >= 0.  hess_logp and out_hess may both be NULL. */
+int32_t mojotrees_b200_action_logprobs_grad(const void* scores, int32_t score_type, int64_t n_rows, int64_t n_classes,
+                                            int64_t row_stride, const void* actions, int32_t action_bytes,
+                                            const void* stats, const float* grad_logp, const float* hess_logp,
+                                            void* out_grad, void* out_hess, int64_t out_stride, void* stream,
+                                            MojoTreesError* error);
+
+/* Clipped policy loss of logged decisions, with l the log probability of the
+ * row's action, ratio = exp(l - old_logp) and t = ref_logp - l:
+ *   loss = weight * (-min(ratio * advantage,
+ *                         clip(ratio, 1 - clip_low, 1 + clip_high) * advantage)
+ *                    + kl_coef * (exp(t) - t - 1))
+ * per row (not averaged: divide the weights).  Per-row arrays have the row
+ * type; ref_logp may be NULL when kl_coef is 0, weights NULL for 1.  out_logp
+ * receives l and may be NULL.  out_grad and out_hess receive the derivatives
+ * with respect to the scores as mojotrees_b200_action_logprobs_grad makes
+ * them from dloss/dl and max(0, the ratio term's d2loss/dl2) + the KL term's;
+ * out_hess may be NULL, and both for the loss alone.  A row whose action's
+ * score is -inf has log probability -inf and otherwise takes no part. */
+int32_t mojotrees_b200_policy_loss(const void* scores, int32_t score_type, int64_t n_rows, int64_t n_classes,
+                                   int64_t row_stride, const void* actions, int32_t action_bytes,
+                                   const void* advantages, const void* old_logp, const void* ref_logp,
+                                   const void* weights, double clip_low, double clip_high, double kl_coef,
+                                   void* out_loss, void* out_logp, void* out_grad, void* out_hess, int64_t out_stride,
+                                   void* stream, MojoTreesError* error);
+
+/* The pairs of a preference loss, laid out on a device once for any number
+ * of calls: item winners[p] was preferred to losers[p] (both in
+ * [0, n_items), different), with weights[p] >= 0 (NULL: 1); host arrays,
+ * copied.  gpu_device_id -1: the current device.  The plan is not changed by
+ * calls that use it, which may overlap; free it when none is running and no
+ * graph holds one. */
+typedef struct MojoTreesPreferencePlan MojoTreesPreferencePlan;
+int32_t mojotrees_b200_preference_plan_create(const int64_t* winners, const int64_t* losers, const float* weights,
+                                              int64_t n_pairs, int64_t n_items, int32_t gpu_device_id,
+                                              MojoTreesPreferencePlan** out_plan, MojoTreesError* error);
+void mojotrees_b200_preference_plan_free(MojoTreesPreferencePlan* plan);
+
+/* Paired preference loss of the items' scores (raw scores or log
+ * probabilities of whole answers, double or float [n_items]) relative to a
+ * reference model's (same type; NULL: 0).  For a pair, with
+ * u = (score - reference of the winner) - (score - reference of the loser):
+ *   MOJOTREES_B200_PREFERENCE_LOGISTIC  -(1 - s) log sigmoid(beta u)
+ *                                       - s log sigmoid(-beta u), s = label_smoothing
+ *   MOJOTREES_B200_PREFERENCE_SQUARED   (u - 1 / (2 beta))^2
+ * times its weight.  out_loss (scores' type [n_pairs], may be NULL) receives
+ * each pair's; out_grad and out_hess (float [n_items], may both be NULL) the
+ * sums over an item's pairs of the first and second derivative with respect
+ * to its score, in a fixed order; 0 for an item without pairs. */
+#define MOJOTREES_B200_PREFERENCE_LOGISTIC 0
+#define MOJOTREES_B200_PREFERENCE_SQUARED 1
+int32_t mojotrees_b200_preference_loss(const MojoTreesPreferencePlan* plan, const void* scores, const void* reference,
+                                       int32_t score_type, double beta, double label_smoothing, int32_t loss_kind,
+                                       void* out_loss, float* out_grad, float* out_hess, void* stream,
+                                       MojoTreesError* error);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

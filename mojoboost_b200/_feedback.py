@@ -1,0 +1,186 @@
+"""Losses that learn from feedback instead of labels, on device scores.
+
+The losses behind the policy and preference fits, for callers whose scores
+are torch tensors on a CUDA device: the log probabilities of taken classes,
+the clipped policy loss of logged decisions and the paired preference loss,
+each with its first and second derivative (include/mojotrees.h has the
+formulas).  Calls run on torch's current stream of the scores' device, do not
+wait for the device and can be captured into a CUDA graph.
+
+A row takes no part, with outputs 0, when its action is negative, its weight
+is 0 or every score is -inf; an action of n_classes or more gives NaN there.
+torch is imported by the first call.
+"""
+import ctypes
+
+import numpy as np
+
+from . import _capi
+from ._capi import MojoTreesError, _Err, _ptr, lib
+
+PREFERENCE_LOSSES = {"logistic": 0, "squared": 1}
+
+_types = None
+
+
+def _torch_types():
+    """{score dtype: (C code, per-row dtype, derivatives' dtype)}, and torch."""
+    global _types
+    if _types is None:
+        import torch
+        _types = ({torch.float64: (0, torch.float64, torch.float32), torch.float32: (1, torch.float32, torch.float32),
+                   torch.float16: (2, torch.float32, torch.float16), torch.bfloat16: (3, torch.float32, torch.bfloat16)},
+                  torch)
+    return _types
+
+
+def _invalid(message):
+    return MojoTreesError(_capi.ERROR_INVALID_ARGUMENT, message)
+
+
+def _vector(name, t, n, dtype, device, shape=None):
+    """The address of a contiguous tensor of n values (shape: its shape instead)."""
+    if t is None:
+        return None
+    shape = (n,) if shape is None else shape
+    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        raise _invalid(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}, got "
+                       f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows(scores, actions):
+    """The arguments that describe scores and actions, and what follows from them."""
+    types, torch = _torch_types()
+    if scores.dtype not in types:
+        raise _invalid(f"scores must be float64, float32, float16 or bfloat16, got {scores.dtype}")
+    if scores.dim() != 2 or scores.device.type != "cuda":
+        raise _invalid(f"scores must be [n_rows, n_classes] on a CUDA device, got {tuple(scores.shape)} on {scores.device}")
+    n, k = scores.shape
+    stride = scores.stride(0) if n > 1 else k
+    if (k > 1 and scores.stride(1) != 1) or stride < k:
+        raise _invalid("scores must hold a row's classes next to each other and rows that do not overlap")
+    if actions.dtype not in (torch.int32, torch.int64):
+        raise _invalid(f"actions must be int32 or int64, got {actions.dtype}")
+    code, row, out = types[scores.dtype]
+    a = _vector("actions", actions, n, actions.dtype, scores.device)
+    head = (scores.data_ptr(), code, n, k, stride, a, 4 if actions.dtype == torch.int32 else 8)
+    return torch, head, row, out
+
+
+def _stream(torch, device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def action_logprobs(scores, actions):
+    """log softmax(scores)[actions] of [n_rows, n_classes] scores, and the row
+    statistics its gradient needs: (logp [n_rows], stats [n_rows, 2]), float64
+    for float64 scores and else float32."""
+    torch, head, row, _ = _rows(scores, actions)
+    n = head[2]
+    logp = torch.empty(n, dtype=row, device=scores.device)
+    stats = torch.empty((n, 2), dtype=row, device=scores.device)
+    e = _Err()
+    e.check(lib().mojotrees_b200_action_logprobs(*head, logp.data_ptr(), stats.data_ptr(),
+                                                 _stream(torch, scores.device), e.h))
+    return logp, stats
+
+
+def action_logprobs_grad(scores, actions, stats, grad_logp, hess_logp=None):
+    """Derivatives of a loss with respect to the scores from those with respect
+    to action_logprobs' log probabilities (float32 [n_rows]): (grad, hess), hess
+    None without hess_logp.  float32 for float64 and float32 scores, else the
+    scores' type."""
+    torch, head, row, out = _rows(scores, actions)
+    n, k, dev = head[2], head[3], scores.device
+    st = _vector("stats", stats, n, row, dev, (n, 2))
+    g = _vector("grad_logp", grad_logp, n, torch.float32, dev)
+    h = _vector("hess_logp", hess_logp, n, torch.float32, dev)
+    grad = torch.empty((n, k), dtype=out, device=dev)
+    hess = None if hess_logp is None else torch.empty((n, k), dtype=out, device=dev)
+    e = _Err()
+    e.check(lib().mojotrees_b200_action_logprobs_grad(*head, st, g, h, grad.data_ptr(),
+                                                      None if hess is None else hess.data_ptr(), k,
+                                                      _stream(torch, dev), e.h))
+    return grad, hess
+
+
+def policy_loss(scores, actions, advantages, old_logp, ref_logp=None, weights=None, clip_low=0.2, clip_high=0.2,
+                kl_coef=0.0, grad=True, hess=False):
+    """Clipped policy loss per row, with a KL term to a reference policy:
+    weight * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * (exp(t) - t - 1)),
+    r = exp(logp - old_logp), t = ref_logp - logp.  Per-row tensors are float64
+    for float64 scores and else float32.  Returns (loss, logp, grad, hess); the
+    derivatives with respect to the scores are None where not asked for."""
+    torch, head, row, out = _rows(scores, actions)
+    n, k, dev = head[2], head[3], scores.device
+    if hess and not grad:
+        raise _invalid("hess needs grad")
+    rows = [_vector(name, t, n, row, dev) for name, t in (("advantages", advantages), ("old_logp", old_logp),
+                                                          ("ref_logp", ref_logp), ("weights", weights))]
+    loss = torch.empty(n, dtype=row, device=dev)
+    logp = torch.empty(n, dtype=row, device=dev)
+    dg = torch.empty((n, k), dtype=out, device=dev) if grad else None
+    dh = torch.empty((n, k), dtype=out, device=dev) if hess else None
+    e = _Err()
+    e.check(lib().mojotrees_b200_policy_loss(*head, *rows, clip_low, clip_high, kl_coef, loss.data_ptr(),
+                                             logp.data_ptr(), None if dg is None else dg.data_ptr(),
+                                             None if dh is None else dh.data_ptr(), k, _stream(torch, dev), e.h))
+    return loss, logp, dg, dh
+
+
+def _index_array(name, v):
+    v = np.asarray(v)
+    if v.dtype.kind not in "iu" and v.size:
+        raise _invalid(f"{name} must be integers, got {v.dtype}")
+    return np.ascontiguousarray(v, dtype=np.int64)
+
+
+class PreferencePlan:
+    """The pairs of a preference loss on a device: item winners[p] was
+    preferred to losers[p], with weights[p] (default 1).  Made once from host
+    arrays; any number of preference_loss calls may use it, and it has to
+    outlive them and the CUDA graphs that hold one."""
+
+    def __init__(self, winners, losers, n_items, weights=None, device=None):
+        w, l = _index_array("winners", winners), _index_array("losers", losers)
+        ws = None if weights is None else np.ascontiguousarray(weights, dtype=np.float32)
+        if w.ndim != 1 or w.shape != l.shape or (ws is not None and ws.shape != w.shape):
+            raise _invalid("winners, losers and weights must be one-dimensional and of one length")
+        self.n_items, self.n_pairs = int(n_items), w.size
+        e = _Err()
+        h = ctypes.c_void_p()
+        e.check(lib().mojotrees_b200_preference_plan_create(_ptr(w), _ptr(l), _ptr(ws), w.size, self.n_items,
+                                                            -1 if device is None else int(device), ctypes.byref(h),
+                                                            e.h))
+        self.h = h.value
+
+    def __del__(self):
+        if getattr(self, "h", None) and _capi._lib is not None:
+            _capi._lib.mojotrees_b200_preference_plan_free(self.h)
+            self.h = None
+
+
+def preference_loss(plan, scores, reference=None, beta=1.0, label_smoothing=0.0, loss="logistic"):
+    """Paired preference loss of the items' scores (raw scores or log
+    probabilities of whole answers, float64 or float32 [n_items]) relative to
+    a reference model's.  loss "logistic": -log sigmoid(beta u), with label
+    smoothing; "squared": (u - 1 / (2 beta))^2, for a pair's difference u of
+    score - reference.  Returns (loss [n_pairs], grad [n_items], hess
+    [n_items]); the derivatives are float32."""
+    types, torch = _torch_types()
+    if scores.dtype not in (torch.float64, torch.float32) or scores.device.type != "cuda":
+        raise _invalid(f"scores must be float64 or float32 on a CUDA device, got {scores.dtype} on {scores.device}")
+    if loss not in PREFERENCE_LOSSES:
+        raise _invalid(f"loss must be one of {', '.join(PREFERENCE_LOSSES)}, got {loss!r}")
+    dev = scores.device
+    s = _vector("scores", scores, plan.n_items, scores.dtype, dev)
+    r = _vector("reference", reference, plan.n_items, scores.dtype, dev)
+    out = torch.empty(plan.n_pairs, dtype=scores.dtype, device=dev)
+    grad = torch.empty(plan.n_items, dtype=torch.float32, device=dev)
+    hess = torch.empty(plan.n_items, dtype=torch.float32, device=dev)
+    e = _Err()
+    e.check(lib().mojotrees_b200_preference_loss(plan.h, s, r, types[scores.dtype][0], beta, label_smoothing,
+                                                 PREFERENCE_LOSSES[loss], out.data_ptr(), grad.data_ptr(),
+                                                 hess.data_ptr(), _stream(torch, dev), e.h))
+    return out, grad, hess

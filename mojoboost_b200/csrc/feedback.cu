@@ -1,0 +1,737 @@
+// Losses that learn from feedback instead of labels, each with its gradient
+// and hessian: kernels, launchers and C entry points.
+//
+// With z a row's scores, a the class it took, p = softmax(z):
+//   log probability  l = z_a - m - log sum exp(z - m), m = max z
+//   back to scores   G_k = g ([k = a] - p_k)
+//                    H_k = h ([k = a] - p_k)^2 + |g| p_k (1 - p_k)
+// for g = dL/dl, h = d2L/dl2.  H is the diagonal of the Hessian with the
+// curvature of l, -p_k (1 - p_k), taken with weight |g| instead of -g, so it
+// is never negative; for cross entropy (g = -1, h = 0) it is p_k (1 - p_k).
+//
+// A row takes no part when its class is negative, its weight is 0 or every
+// score is -inf (all classes masked), and for the policy loss when the class
+// it took is masked: its outputs are 0, whatever else the row holds.  A class
+// of n_classes or more gives NaN in that row.
+#include "feedback.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include <algorithm>
+#include <memory>
+#include <stdexcept>
+#include <string>
+
+#include "../../include/mojotrees.h"
+#include "capi_util.h"
+#include "trainer.h"
+
+namespace mtb {
+namespace {
+
+#define MTB_CUDA_FB(call)                                                                    \
+  do {                                                                                       \
+    cudaError_t e_ = (call);                                                                 \
+    if (e_ != cudaSuccess)                                                                   \
+      throw std::runtime_error(std::string("CUDA error: ") + cudaGetErrorString(e_) + " at " \
+                               + #call);                                                     \
+  } while (0)
+
+// Per score type: C computes a row's exponentials, Row holds per-row values,
+// Out the derivatives.  float64 scores are computed in float64 throughout and
+// narrowed to float32 derivatives, as the trainer's other objectives are;
+// 16-bit scores are widened to float32 and only the stored derivatives are
+// rounded back.
+template <typename T>
+struct Types {
+  using C = float;
+  using Row = float;
+  using Out = T;
+};
+template <>
+struct Types<double> {
+  using C = double;
+  using Row = double;
+  using Out = float;
+};
+
+__device__ __forceinline__ double widen(double v) { return v; }
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void narrow(float v, float& o) { o = v; }
+__device__ __forceinline__ void narrow(double v, float& o) { o = (float)v; }
+__device__ __forceinline__ void narrow(float v, __half& o) { o = __float2half_rn(v); }
+__device__ __forceinline__ void narrow(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ double exp_c(double d) { return exp(d); }
+__device__ __forceinline__ float exp_c(float d) { return __expf(d); }
+
+// The larger of two values, NaN when either is.
+template <typename C>
+__device__ __forceinline__ C max_nan(C a, C b) {
+  return (b > a || b != b) ? b : a;
+}
+
+// A row's softmax sum as sum exp(z - m) = 1 + rest: `rest` leaves out one
+// class at the maximum, so it keeps its relative accuracy when one class has
+// nearly all of the probability, and with it 1 - p of that class.
+template <typename C>
+struct RowSum {
+  C m;
+  double rest;
+};
+
+template <typename T>
+struct RowPointers {
+  const T* scores;
+  const int* actions32;
+  const long long* actions64;
+  long long n, stride;
+  int K;
+  __device__ __forceinline__ long long action(long long r) const {
+    return actions64 ? actions64[r] : (long long)actions32[r];
+  }
+};
+
+template <typename T>
+struct OutPointers {
+  typename Types<T>::Out* grad;
+  typename Types<T>::Out* hess;
+  long long row_stride, class_stride;
+};
+
+template <typename T>
+struct PolicyPointers {
+  using Row = typename Types<T>::Row;
+  const Row *advantages, *old_logp, *ref_logp, *weights;
+  double log_low, log_high;    // log of the clip range's ends
+  double clip_low, clip_high;  // the ends
+  double kl;
+  Row *loss, *logp;
+};
+
+// The gradient on l jumps at the ends of the clip range, so there l has to be
+// right beyond the accuracy of a float32 sum: a row whose log ratio is this
+// near to an end sums its exponentials again in float64.  A thread adds at
+// most kMaxClasses / 256 = 1024 of them in float32, each within 2^-21 of its
+// value: below 1024 * 2^-24 + 2^-21 = 6.2e-5.
+constexpr double kBorderSlack = 7e-5;
+
+struct RowDerivative {
+  double g, h;
+};
+
+// Loss of a row with log probability l, and its derivatives in l.
+template <typename T>
+__device__ __forceinline__ RowDerivative policy_terms(const PolicyPointers<T>& t, double l, double adv, double old,
+                                                      double ref, double w, double* loss) {
+  const double d = l - old;
+  const double ra = exp(d) * adv;
+  const bool active = adv >= 0.0 ? d <= t.log_high : d >= t.log_low;
+  double v = active ? -ra : (adv >= 0.0 ? -t.clip_high * adv : -t.clip_low * adv);
+  double g = active ? -ra : 0.0;
+  if (ra != ra) v = g = ra;
+  double h = g > 0.0 ? g : 0.0;
+  if (t.ref_logp) {
+    const double e = expm1(ref - l);
+    v += t.kl * (e - (ref - l));
+    g -= t.kl * e;
+    h += t.kl * (e + 1.0);
+  }
+  *loss = w * v;
+  return {w * g, w * h};
+}
+
+// Whether the float32 sum leaves open on which side of an end of the clip
+// range the row lies.
+template <typename T>
+__device__ __forceinline__ bool near_border(const PolicyPointers<T>& t, double d, double adv) {
+  return fabs(d - (adv >= 0.0 ? t.log_high : t.log_low)) < kBorderSlack;
+}
+
+// p_k and [k = a] - p_k from z_k - m and the row's sum.
+template <typename C>
+__device__ __forceinline__ void derivative(C z, const C m, C inv_total, C rest_share, bool taken, C g, C h, bool want_h,
+                                           C* grad, C* hess) {
+  const C p = exp_c(z - m) * inv_total;
+  const C left = z == m ? rest_share : (C)1 - p;  // 1 - p
+  const C q = taken ? left : -p;
+  *grad = g * q;
+  if (want_h) *hess = h * q * q + fabs(g) * p * left;
+}
+
+enum RowOp : int { ROW_LOGPROBS = 0, ROW_BACK = 1, ROW_POLICY = 2 };
+
+template <typename T>
+struct RowArgs {
+  RowPointers<T> in;
+  OutPointers<T> out;
+  PolicyPointers<T> pol;
+  typename Types<T>::Row* logp;         // ROW_LOGPROBS
+  typename Types<T>::Row* stats;        // ROW_LOGPROBS (written), ROW_BACK (read)
+  const float *grad_logp, *hess_logp;   // ROW_BACK
+};
+
+constexpr int kRowThreads = 256;
+
+__device__ __forceinline__ double add_f64(double a, double b) { return a + b; }
+
+template <typename V, typename F>
+__device__ __forceinline__ V block_reduce(V v, V* sm, F f) {
+  for (int k = 16; k > 0; k >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, k));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = sm[0];
+  for (int i = 1; i < kRowThreads / 32; ++i) v = f(v, sm[i]);
+  return v;
+}
+
+// One block per row: the maximum, the sum, the derivatives, each a pass over
+// the row.
+template <typename T, int OP>
+__global__ void __launch_bounds__(kRowThreads) k_feedback_rows(const RowArgs<T> A) {
+  using C = typename Types<T>::C;
+  using Row = typename Types<T>::Row;
+  __shared__ C sm_c[kRowThreads / 32];
+  __shared__ double sm_d[kRowThreads / 32];
+  const int K = A.in.K;
+  for (long long r = blockIdx.x; r < A.in.n; r += gridDim.x) {
+    const T* z = A.in.scores + r * A.in.stride;
+    const long long a = A.in.action(r);
+    const bool bad = a >= K;
+    bool part = a >= 0;
+    if (OP == ROW_POLICY && A.pol.weights) part = part && A.pol.weights[r] != (Row)0;
+    C m = 0;
+    double rest = -1.0;
+    if (OP == ROW_BACK) {
+      m = A.stats[2 * r];
+      rest = (double)A.stats[2 * r + 1];
+      part = part && rest != -1.0;
+    } else if (part && !bad) {
+      C mx = -INFINITY;
+      for (int k = threadIdx.x; k < K; k += kRowThreads) mx = max_nan<C>(mx, widen(z[k]));
+      mx = block_reduce(mx, sm_c, max_nan<C>);
+      if (mx == (C)-INFINITY) {
+        part = false;
+      } else {
+        m = mx;
+        C s = 0;
+        int ties = 0;
+        for (int k = threadIdx.x; k < K; k += kRowThreads) {
+          const C d = (C)widen(z[k]) - m;
+          if (d != 0) s += exp_c(d);
+          else ++ties;
+        }
+        const double others = block_reduce((double)s, sm_d, add_f64);
+        rest = others + (block_reduce((double)ties, sm_d, add_f64) - 1.0);
+      }
+    }
+    RowDerivative row = {0.0, 0.0};
+    if (OP == ROW_LOGPROBS) {
+      if (threadIdx.x == 0) {
+        const double l = part ? (bad ? (double)NAN : (double)widen(z[a]) - (double)m - log1p(rest)) : 0.0;
+        A.logp[r] = (Row)l;
+        A.stats[2 * r] = part && bad ? (Row)NAN : (Row)m;
+        A.stats[2 * r + 1] = part ? (bad ? (Row)NAN : (Row)rest) : (Row)-1;
+      }
+      __syncthreads();
+      continue;
+    } else if (OP == ROW_BACK) {
+      row = {part ? (double)A.grad_logp[r] : 0.0, part && A.hess_logp ? (double)A.hess_logp[r] : 0.0};
+    } else {
+      double l = 0.0, loss = 0.0;
+      if (part && bad) {
+        l = loss = row.g = row.h = NAN;
+      } else if (part) {
+        const double za = (double)widen(z[a]);
+        l = za - (double)m - log1p(rest);
+        if (za == -INFINITY) {
+          part = false;
+        } else {
+          const double adv = (double)A.pol.advantages[r], old = (double)A.pol.old_logp[r];
+          if (sizeof(C) == 4 && near_border(A.pol, l - old, adv)) {
+            double s = 0.0;
+            for (int k = threadIdx.x; k < K; k += kRowThreads) s += exp((double)widen(z[k]) - (double)m);
+            l = za - (double)m - log(block_reduce(s, sm_d, add_f64));
+          }
+          row = policy_terms(A.pol, l, adv, old, A.pol.ref_logp ? (double)A.pol.ref_logp[r] : 0.0,
+                             A.pol.weights ? (double)A.pol.weights[r] : 1.0, &loss);
+        }
+      }
+      if (threadIdx.x == 0) {
+        if (A.pol.loss) A.pol.loss[r] = (Row)loss;
+        if (A.pol.logp) A.pol.logp[r] = (Row)l;
+      }
+    }
+    if (OP == ROW_POLICY && !A.out.grad) {
+      __syncthreads();
+      continue;
+    }
+    auto* gp = A.out.grad + r * A.out.row_stride;
+    auto* hp = A.out.hess ? A.out.hess + r * A.out.row_stride : nullptr;
+    const C g = (C)row.g, h = (C)row.h, inv = (C)(1.0 / (1.0 + rest)), left = (C)(rest / (1.0 + rest));
+    for (int k = threadIdx.x; k < K; k += kRowThreads) {
+      C dg = 0, dh = 0;
+      if (part && bad) dg = dh = (C)NAN;
+      else if (part) derivative<C>(widen(z[k]), m, inv, left, k == a, g, h, hp != nullptr, &dg, &dh);
+      narrow(dg, gp[k * A.out.class_stride]);
+      if (hp) narrow(dh, hp[k * A.out.class_stride]);
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int OP>
+void launch_rows_t(const RowArgs<T>& A, cudaStream_t st) {
+  if (A.in.n == 0) return;
+  const unsigned grid = (unsigned)std::min<long long>(A.in.n, 1 << 20);
+  k_feedback_rows<T, OP><<<grid, kRowThreads, 0, st>>>(A);
+  MTB_CUDA_FB(cudaGetLastError());
+}
+
+template <typename T>
+RowArgs<T> row_args(const ScoreRows& in) {
+  RowArgs<T> A = {};
+  A.in.scores = static_cast<const T*>(in.scores);
+  (in.actions64 ? (const void*&)A.in.actions64 : (const void*&)A.in.actions32) = in.actions;
+  A.in.n = in.n;
+  A.in.K = in.K;
+  A.in.stride = in.stride;
+  return A;
+}
+
+template <typename T>
+void set_out(RowArgs<T>& A, const ScoreDerivatives& out) {
+  using Out = typename Types<T>::Out;
+  A.out = {static_cast<Out*>(out.grad), static_cast<Out*>(out.hess), out.row_stride, out.class_stride};
+}
+
+template <typename F>
+void by_type(int type, F&& f) {
+  switch (type) {
+    case SCORE_F64: f((double*)nullptr); break;
+    case SCORE_F32: f((float*)nullptr); break;
+    case SCORE_F16: f((__half*)nullptr); break;
+    case SCORE_BF16: f((__nv_bfloat16*)nullptr); break;
+    default: throw std::invalid_argument("unknown score type");
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Paired preference loss
+// ---------------------------------------------------------------------------
+
+// With u = (s_w - s_l) - (ref_w - ref_l):
+//   logistic  L = (1 - e) softplus(-beta u) + e softplus(beta u)
+//             L' = beta (e sig(beta u) - (1 - e) sig(-beta u))
+//             L'' = beta^2 sig(beta u) sig(-beta u)
+//   squared   L = (u - 1 / (2 beta))^2
+// in float64 throughout: u is the difference of log probabilities of whole
+// answers, tens or hundreds each.
+struct PairMath {
+  double beta, smoothing, target;  // target: 1 / (2 beta)
+  int kind;
+  __device__ __forceinline__ double loss(double u) const {
+    if (kind == PREFERENCE_SQUARED) return (u - target) * (u - target);
+    const double x = beta * u, soft = log1p(exp(-fabs(x)));
+    if (x != x) return x;
+    const double won = (1.0 - smoothing) * (soft + fmax(-x, 0.0));
+    return smoothing > 0.0 ? won + smoothing * (soft + fmax(x, 0.0)) : won;  // an infinite x times 0 is no NaN
+  }
+  __device__ __forceinline__ RowDerivative derivative(double u) const {
+    if (kind == PREFERENCE_SQUARED) return {2.0 * (u - target), 2.0};
+    const double x = beta * u, e = exp(-fabs(x)), big = 1.0 / (1.0 + e), small = e * big;
+    const double up = x >= 0.0 ? big : small, down = x >= 0.0 ? small : big;
+    return {beta * (smoothing * up - (1.0 - smoothing) * down), beta * beta * big * small};
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ double lean(const T* s, const T* ref, int i) {
+  return ref ? (double)s[i] - (double)ref[i] : (double)s[i];
+}
+
+// u from each item's distance to its reference: what an infinite reference
+// or score leaves undefined is NaN.
+template <typename T>
+__global__ void __launch_bounds__(256) k_preference_items(const int* __restrict__ offsets,
+                                                          const int* __restrict__ partners,
+                                                          const float* __restrict__ entry_w, long long n,
+                                                          const T* __restrict__ s, const T* __restrict__ ref,
+                                                          PairMath pm, float* __restrict__ grad,
+                                                          float* __restrict__ hess) {
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+    const int e1 = offsets[i + 1];
+    double g = 0.0, h = 0.0;
+    for (int e = offsets[i]; e < e1; ++e) {
+      const int code = partners[e], j = code & 0x7fffffff;
+      const double sign = code < 0 ? -1.0 : 1.0;
+      const double u = sign * (lean(s, ref, (int)i) - lean(s, ref, j));
+      RowDerivative d = pm.derivative(u);
+      const double w = entry_w ? (double)entry_w[e] : 1.0;
+      g += w * sign * d.g;
+      h += w * d.h;
+    }
+    grad[i] = (float)g;
+    hess[i] = (float)h;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_preference_pairs(const int2* __restrict__ pairs,
+                                                          const float* __restrict__ pair_w, long long n,
+                                                          const T* __restrict__ s, const T* __restrict__ ref,
+                                                          PairMath pm, T* __restrict__ loss) {
+  for (long long p = (long long)blockIdx.x * blockDim.x + threadIdx.x; p < n; p += (long long)gridDim.x * blockDim.x) {
+    const int2 c = pairs[p];
+    const double w = pair_w ? (double)pair_w[p] : 1.0;
+    loss[p] = w == 0.0 ? (T)0 : (T)(w * pm.loss(lean(s, ref, c.x) - lean(s, ref, c.y)));
+  }
+}
+
+template <typename T>
+void launch_preference_t(const PreferencePlan& plan, const PreferenceTerms& t, cudaStream_t st) {
+  const PairMath pm = {t.beta, t.smoothing, 1.0 / (2.0 * t.beta), t.kind};
+  const T* s = static_cast<const T*>(t.scores);
+  const T* ref = static_cast<const T*>(t.reference);
+  auto blocks = [](long long n) { return (unsigned)std::min<long long>((n + 255) / 256, 1 << 20); };
+  if (plan.n_items > 0 && t.grad) {
+    k_preference_items<T><<<blocks(plan.n_items), 256, 0, st>>>(plan.offsets, plan.partners, plan.entry_w,
+                                                                plan.n_items, s, ref, pm, t.grad, t.hess);
+    MTB_CUDA_FB(cudaGetLastError());
+  }
+  if (plan.n_pairs > 0 && t.loss) {
+    k_preference_pairs<T><<<blocks(plan.n_pairs), 256, 0, st>>>(plan.pairs, plan.pair_w, plan.n_pairs, s, ref, pm,
+                                                                static_cast<T*>(t.loss));
+    MTB_CUDA_FB(cudaGetLastError());
+  }
+}
+
+}  // namespace
+
+void launch_logprobs(const ScoreRows& in, void* logp, void* stats, cudaStream_t st) {
+  by_type(in.type, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    RowArgs<T> A = row_args<T>(in);
+    A.logp = static_cast<typename Types<T>::Row*>(logp);
+    A.stats = static_cast<typename Types<T>::Row*>(stats);
+    launch_rows_t<T, ROW_LOGPROBS>(A, st);
+  });
+}
+
+void launch_logprobs_grad(const ScoreRows& in, const void* stats, const float* grad_logp, const float* hess_logp,
+                          const ScoreDerivatives& out, cudaStream_t st) {
+  by_type(in.type, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    RowArgs<T> A = row_args<T>(in);
+    A.stats = const_cast<typename Types<T>::Row*>(static_cast<const typename Types<T>::Row*>(stats));
+    A.grad_logp = grad_logp;
+    A.hess_logp = hess_logp;
+    set_out(A, out);
+    launch_rows_t<T, ROW_BACK>(A, st);
+  });
+}
+
+void launch_policy(const ScoreRows& in, const PolicyTerms& t, const ScoreDerivatives& out, cudaStream_t st) {
+  by_type(in.type, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    using Row = typename Types<T>::Row;
+    RowArgs<T> A = row_args<T>(in);
+    A.pol.advantages = static_cast<const Row*>(t.advantages);
+    A.pol.old_logp = static_cast<const Row*>(t.old_logp);
+    A.pol.ref_logp = static_cast<const Row*>(t.ref_logp);
+    A.pol.weights = static_cast<const Row*>(t.weights);
+    A.pol.log_low = log1p(-t.clip_low);
+    A.pol.log_high = log1p(t.clip_high);
+    A.pol.clip_low = 1.0 - t.clip_low;
+    A.pol.clip_high = 1.0 + t.clip_high;
+    A.pol.kl = t.kl_coef;
+    A.pol.loss = static_cast<Row*>(t.loss);
+    A.pol.logp = static_cast<Row*>(t.logp);
+    set_out(A, out);
+    launch_rows_t<T, ROW_POLICY>(A, st);
+  });
+}
+
+PreferencePlan::~PreferencePlan() {
+  cudaFree(offsets);
+  cudaFree(partners);
+  cudaFree(entry_w);
+  cudaFree(pairs);
+  cudaFree(pair_w);
+}
+
+namespace {
+
+template <typename T>
+T* to_device(const std::vector<T>& v) {
+  T* p = nullptr;
+  MTB_CUDA_FB(cudaMalloc(&p, sizeof(T) * std::max<size_t>(1, v.size())));
+  const cudaError_t e = v.empty() ? cudaSuccess : cudaMemcpy(p, v.data(), sizeof(T) * v.size(), cudaMemcpyHostToDevice);
+  if (e != cudaSuccess) {
+    cudaFree(p);
+    throw std::runtime_error(std::string("CUDA error: ") + cudaGetErrorString(e) + " (preference plan)");
+  }
+  return p;
+}
+
+}  // namespace
+
+void PreferencePlan::check(const int64_t* winners, const int64_t* losers, const float* weights, long long np,
+                           long long ni) {
+  for (long long p = 0; p < np; ++p) {
+    const int64_t a = winners[p], b = losers[p];
+    if (a < 0 || a >= ni || b < 0 || b >= ni) throw std::invalid_argument("pair item out of range");
+    if (a == b) throw std::invalid_argument("an item is paired with itself");
+    if (weights && !(weights[p] >= 0.0f && std::isfinite(weights[p])))
+      throw std::invalid_argument("pair weights must be finite and non-negative");
+  }
+}
+
+void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const float* weights, long long np,
+                           long long ni) {
+  std::vector<int> off((size_t)ni + 1, 0);
+  std::vector<int2> pr((size_t)np);
+  for (long long p = 0; p < np; ++p) {
+    const int64_t a = winners[p], b = losers[p];
+    pr[p] = make_int2((int)a, (int)b);
+    if (weights && weights[p] == 0.0f) continue;
+    ++off[a + 1];
+    ++off[b + 1];
+  }
+  for (long long i = 0; i < ni; ++i) off[i + 1] += off[i];
+  n_entries = off[ni];
+  std::vector<int> at(off.begin(), off.end() - 1), part((size_t)n_entries);
+  std::vector<float> ew(weights ? (size_t)n_entries : 0);
+  for (long long p = 0; p < np; ++p) {  // an item's entries stay in the pairs' order
+    if (weights && weights[p] == 0.0f) continue;
+    const int ea = at[pr[p].x]++, eb = at[pr[p].y]++;
+    part[ea] = pr[p].y;
+    part[eb] = pr[p].x | (int)0x80000000;
+    if (weights) ew[ea] = ew[eb] = weights[p];
+  }
+  MTB_CUDA_FB(cudaGetDevice(&device));
+  n_items = ni;
+  n_pairs = np;
+  weighted = weights != nullptr;
+  offsets = to_device(off);
+  partners = to_device(part);
+  pairs = to_device(pr);
+  if (weighted) {
+    entry_w = to_device(ew);
+    pair_w = to_device(std::vector<float>(weights, weights + np));
+  }
+}
+
+void launch_preference(const PreferencePlan& plan, const PreferenceTerms& t, cudaStream_t st) {
+  if (t.type == SCORE_F64) launch_preference_t<double>(plan, t, st);
+  else launch_preference_t<float>(plan, t, st);
+}
+
+}  // namespace mtb
+
+// ---------------------------------------------------------------------------
+// C entry points
+// ---------------------------------------------------------------------------
+
+struct MojoTreesPreferencePlan {
+  mtb::PreferencePlan plan;
+};
+
+namespace {
+
+using mtb::Unsupported;
+
+template <typename F>
+int32_t checked(MojoTreesError* error, F&& fn) {
+  mtb::capi_clear_error(error);
+  try {
+    fn();
+    return MOJOTREES_OK;
+  } catch (const std::invalid_argument& e) {
+    mtb::capi_set_error(error, e.what());
+    return MOJOTREES_ERROR_INVALID_ARGUMENT;
+  } catch (const Unsupported& e) {
+    mtb::capi_set_error(error, e.what());
+    return MOJOTREES_ERROR_UNSUPPORTED;
+  } catch (const std::exception& e) {
+    mtb::capi_set_error(error, e.what());
+    return MOJOTREES_ERROR_TRAINING;
+  }
+}
+
+void require(bool ok, const char* what) {
+  if (!ok) throw std::invalid_argument(what);
+}
+
+void require_cuda() {
+  if (mtb::cuda_device_count() < 1) throw Unsupported("no CUDA device is available");
+}
+
+// Makes a device current for a call, and the caller's again after it.
+struct DeviceScope {
+  int before = -1;
+  bool moved = false;
+  explicit DeviceScope(int dev) {
+    MTB_CUDA_FB(cudaGetDevice(&before));
+    if (dev >= 0 && dev != before) {
+      MTB_CUDA_FB(cudaSetDevice(dev));
+      moved = true;
+    }
+  }
+  ~DeviceScope() {
+    if (moved) cudaSetDevice(before);
+  }
+};
+
+// The device that holds `p`; every array of a call has to be there.
+int device_of(const void* p) {
+  cudaPointerAttributes a;
+  if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+    cudaGetLastError();
+    throw std::invalid_argument("array is not in device memory");
+  }
+  require(a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged, "array is not in device memory");
+  return a.device;
+}
+
+int common_device(std::initializer_list<const void*> arrays) {
+  int dev = -1;
+  for (const void* p : arrays) {
+    if (!p) continue;
+    const int d = device_of(p);
+    require(dev < 0 || d == dev, "arrays of one call are on different devices");
+    dev = d;
+  }
+  return dev;
+}
+
+mtb::ScoreRows score_rows(const void* scores, int32_t type, int64_t n_rows, int64_t n_classes, int64_t stride,
+                          const void* actions, int32_t action_bytes) {
+  require(type >= mtb::SCORE_F64 && type <= mtb::SCORE_BF16, "unknown score type");
+  require(n_rows >= 0, "n_rows must be non-negative");
+  require(n_classes >= 1 && n_classes <= mtb::kMaxClasses, "n_classes must be in [1, 262144]");
+  require(stride >= n_classes, "row_stride must be at least n_classes");
+  require(n_rows == 0 || stride <= (int64_t)1 << 46 && n_rows <= ((int64_t)1 << 46) / stride, "scores are too large");
+  require(action_bytes == 4 || action_bytes == 8, "actions must be 4 or 8 byte integers");
+  require(n_rows == 0 || (scores && actions), "null pointer argument");
+  return {scores, type, n_rows, (int)n_classes, stride, actions, action_bytes == 8};
+}
+
+mtb::ScoreDerivatives derivatives(void* grad, void* hess, int64_t n_rows, int64_t n_classes, int64_t stride) {
+  require(stride >= n_classes, "out_stride must be at least n_classes");
+  require(n_rows == 0 || stride <= (int64_t)1 << 46 && n_rows <= ((int64_t)1 << 46) / stride, "derivatives are too large");
+  return {grad, hess, stride, 1};
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t mojotrees_b200_action_logprobs(const void* scores, int32_t score_type, int64_t n_rows, int64_t n_classes,
+                                       int64_t row_stride, const void* actions, int32_t action_bytes, void* out_logp,
+                                       void* out_stats, void* stream, MojoTreesError* error) {
+  return checked(error, [&] {
+    const mtb::ScoreRows in = score_rows(scores, score_type, n_rows, n_classes, row_stride, actions, action_bytes);
+    require(n_rows == 0 || (out_logp && out_stats), "null pointer argument");
+    require_cuda();
+    if (n_rows == 0) return;
+    DeviceScope on(common_device({scores, actions, out_logp, out_stats}));
+    mtb::launch_logprobs(in, out_logp, out_stats, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int32_t mojotrees_b200_action_logprobs_grad(const void* scores, int32_t score_type, int64_t n_rows, int64_t n_classes,
+                                            int64_t row_stride, const void* actions, int32_t action_bytes,
+                                            const void* stats, const float* grad_logp, const float* hess_logp,
+                                            void* out_grad, void* out_hess, int64_t out_stride, void* stream,
+                                            MojoTreesError* error) {
+  return checked(error, [&] {
+    const mtb::ScoreRows in = score_rows(scores, score_type, n_rows, n_classes, row_stride, actions, action_bytes);
+    require(n_rows == 0 || (stats && grad_logp && out_grad), "null pointer argument");
+    require(!hess_logp == !out_hess, "hess_logp and out_hess go together");
+    const mtb::ScoreDerivatives out = derivatives(out_grad, out_hess, n_rows, n_classes, out_stride);
+    require_cuda();
+    if (n_rows == 0) return;
+    DeviceScope on(common_device({scores, actions, stats, grad_logp, hess_logp, out_grad, out_hess}));
+    mtb::launch_logprobs_grad(in, stats, grad_logp, hess_logp, out, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int32_t mojotrees_b200_policy_loss(const void* scores, int32_t score_type, int64_t n_rows, int64_t n_classes,
+                                   int64_t row_stride, const void* actions, int32_t action_bytes,
+                                   const void* advantages, const void* old_logp, const void* ref_logp,
+                                   const void* weights, double clip_low, double clip_high, double kl_coef,
+                                   void* out_loss, void* out_logp, void* out_grad, void* out_hess, int64_t out_stride,
+                                   void* stream, MojoTreesError* error) {
+  return checked(error, [&] {
+    const mtb::ScoreRows in = score_rows(scores, score_type, n_rows, n_classes, row_stride, actions, action_bytes);
+    require(n_rows == 0 || (advantages && old_logp && out_loss), "null pointer argument");
+    require(clip_low >= 0.0 && clip_low <= 1.0, "clip_low must be in [0, 1]");
+    require(clip_high >= 0.0, "clip_high must be non-negative");
+    require(kl_coef >= 0.0 && std::isfinite(kl_coef), "kl_coef must be finite and non-negative");
+    require(kl_coef == 0.0 || ref_logp || n_rows == 0, "kl_coef needs ref_logp");
+    require(out_grad || !out_hess, "out_hess needs out_grad");
+    const mtb::ScoreDerivatives out =
+        out_grad ? derivatives(out_grad, out_hess, n_rows, n_classes, out_stride) : mtb::ScoreDerivatives{};
+    require_cuda();
+    if (n_rows == 0) return;
+    DeviceScope on(common_device({scores, actions, advantages, old_logp, ref_logp, weights, out_loss, out_logp,
+                                  out_grad, out_hess}));
+    const mtb::PolicyTerms t = {advantages, old_logp, kl_coef > 0.0 ? ref_logp : nullptr, weights, clip_low,
+                                clip_high, kl_coef, out_loss, out_logp};
+    mtb::launch_policy(in, t, out, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int32_t mojotrees_b200_preference_plan_create(const int64_t* winners, const int64_t* losers, const float* weights,
+                                              int64_t n_pairs, int64_t n_items, int32_t gpu_device_id,
+                                              MojoTreesPreferencePlan** out_plan, MojoTreesError* error) {
+  return checked(error, [&] {
+    require(out_plan, "null pointer argument");
+    require(n_pairs >= 0 && n_items >= 0, "n_pairs and n_items must be non-negative");
+    require(n_items < (int64_t)1 << 31, "more than 2^31-1 items");
+    require(n_pairs < (int64_t)1 << 30, "more than 2^30-1 pairs");
+    require(n_pairs == 0 || (winners && losers), "null pointer argument");
+    mtb::PreferencePlan::check(winners, losers, weights, n_pairs, n_items);
+    require_cuda();
+    require(gpu_device_id < mtb::cuda_device_count(), "gpu_device_id out of range");
+    DeviceScope on(gpu_device_id);
+    std::unique_ptr<MojoTreesPreferencePlan> h(new MojoTreesPreferencePlan());
+    h->plan.build(winners, losers, weights, n_pairs, n_items);
+    *out_plan = h.release();
+  });
+}
+
+void mojotrees_b200_preference_plan_free(MojoTreesPreferencePlan* plan) { delete plan; }
+
+int32_t mojotrees_b200_preference_loss(const MojoTreesPreferencePlan* plan, const void* scores, const void* reference,
+                                       int32_t score_type, double beta, double label_smoothing, int32_t loss_kind,
+                                       void* out_loss, float* out_grad, float* out_hess, void* stream,
+                                       MojoTreesError* error) {
+  return checked(error, [&] {
+    require(plan, "null pointer argument");
+    require(score_type == mtb::SCORE_F64 || score_type == mtb::SCORE_F32, "preference scores are float64 or float32");
+    require(beta > 0.0 && std::isfinite(beta), "beta must be positive");
+    require(label_smoothing >= 0.0 && label_smoothing <= 0.5, "label_smoothing must be in [0, 0.5]");
+    require(loss_kind == mtb::PREFERENCE_LOGISTIC || loss_kind == mtb::PREFERENCE_SQUARED, "unknown preference loss");
+    require(loss_kind == mtb::PREFERENCE_LOGISTIC || label_smoothing == 0.0, "label_smoothing needs the logistic loss");
+    const mtb::PreferencePlan& p = plan->plan;
+    require(p.n_items == 0 || scores, "null pointer argument");
+    require(!out_grad == !out_hess, "out_grad and out_hess go together");
+    require_cuda();
+    if (p.n_items == 0) return;
+    const int dev = common_device({scores, reference, out_loss, out_grad, out_hess});
+    require(dev == p.device, "arrays are not on the plan's device");
+    DeviceScope on(dev);
+    const mtb::PreferenceTerms t = {scores, reference, score_type, beta, label_smoothing, loss_kind, out_loss,
+                                    out_grad, out_hess};
+    mtb::launch_preference(p, t, static_cast<cudaStream_t>(stream));
+  });
+}
+
+}  // extern "C"
