@@ -115,10 +115,14 @@ struct PolicyPointers {
 
 // The gradient on l jumps at the ends of the clip range, so there l has to be
 // right beyond the accuracy of a float32 sum: a row whose log ratio is this
-// near to an end sums its exponentials again in float64.  A thread adds at
-// most kMaxClasses / 256 = 1024 of them in float32, each within 2^-21 of its
-// value: below 1024 * 2^-24 + 2^-21 = 6.2e-5.
-constexpr double kBorderSlack = 7e-5;
+// near to an end sums its exponentials again in float64.  A float32 sum of
+// exponentials adds at most `adds` of them one after the other (2^-24 each),
+// and each is off by (2 + 1.173 |d|) 2^-23 for d = z - m (__expf's documented
+// bound), d itself by |d| 2^-24; weighted by the probabilities |d| averages
+// below log K <= 12.5.
+__host__ __device__ constexpr double border_slack(int adds, double log_k) {
+  return 1.1 * (adds * 0x1p-24 + (2.0 + 1.173 * log_k) * 0x1p-23 + log_k * 0x1p-24);
+}
 
 struct RowDerivative {
   double g, h;
@@ -148,16 +152,17 @@ __device__ __forceinline__ RowDerivative policy_terms(const PolicyPointers<T>& t
 // Whether the float32 sum leaves open on which side of an end of the clip
 // range the row lies.
 template <typename T>
-__device__ __forceinline__ bool near_border(const PolicyPointers<T>& t, double d, double adv) {
-  return fabs(d - (adv >= 0.0 ? t.log_high : t.log_low)) < kBorderSlack;
+__device__ __forceinline__ bool near_border(const PolicyPointers<T>& t, double d, double adv, double slack) {
+  return fabs(d - (adv >= 0.0 ? t.log_high : t.log_low)) < slack;
 }
 
-// p_k and [k = a] - p_k from z_k - m and the row's sum.
+// Derivatives at class k from e = exp(z_k - m) and the row's sum.  e is 1 for
+// a class at the maximum (or one so near to it that its term of the sum is 1).
 template <typename C>
-__device__ __forceinline__ void derivative(C z, const C m, C inv_total, C rest_share, bool taken, C g, C h, bool want_h,
-                                           C* grad, C* hess) {
-  const C p = exp_c(z - m) * inv_total;
-  const C left = z == m ? rest_share : (C)1 - p;  // 1 - p
+__device__ __forceinline__ void derivative(C e, C inv_total, C rest_share, bool taken, C g, C h, bool want_h, C* grad,
+                                           C* hess) {
+  const C p = e * inv_total;
+  const C left = e == (C)1 ? rest_share : (C)1 - p;  // 1 - p
   const C q = taken ? left : -p;
   *grad = g * q;
   if (want_h) *hess = h * q * q + fabs(g) * p * left;
@@ -222,8 +227,8 @@ __global__ void __launch_bounds__(kRowThreads) k_feedback_rows(const RowArgs<T> 
         C s = 0;
         int ties = 0;
         for (int k = threadIdx.x; k < K; k += kRowThreads) {
-          const C d = (C)widen(z[k]) - m;
-          if (d != 0) s += exp_c(d);
+          const C e = exp_c((C)widen(z[k]) - m);
+          if (e != (C)1) s += e;
           else ++ties;
         }
         const double others = block_reduce((double)s, sm_d, add_f64);
@@ -253,7 +258,7 @@ __global__ void __launch_bounds__(kRowThreads) k_feedback_rows(const RowArgs<T> 
           part = false;
         } else {
           const double adv = (double)A.pol.advantages[r], old = (double)A.pol.old_logp[r];
-          if (sizeof(C) == 4 && near_border(A.pol, l - old, adv)) {
+          if (sizeof(C) == 4 && near_border(A.pol, l - old, adv, border_slack(kMaxClasses / kRowThreads + 16, 12.5))) {
             double s = 0.0;
             for (int k = threadIdx.x; k < K; k += kRowThreads) s += exp((double)widen(z[k]) - (double)m);
             l = za - (double)m - log(block_reduce(s, sm_d, add_f64));
@@ -277,7 +282,7 @@ __global__ void __launch_bounds__(kRowThreads) k_feedback_rows(const RowArgs<T> 
     for (int k = threadIdx.x; k < K; k += kRowThreads) {
       C dg = 0, dh = 0;
       if (part && bad) dg = dh = (C)NAN;
-      else if (part) derivative<C>(widen(z[k]), m, inv, left, k == a, g, h, hp != nullptr, &dg, &dh);
+      else if (part) derivative<C>(exp_c((C)widen(z[k]) - m), inv, left, k == a, g, h, hp != nullptr, &dg, &dh);
       narrow(dg, gp[k * A.out.class_stride]);
       if (hp) narrow(dh, hp[k * A.out.class_stride]);
     }
@@ -285,9 +290,228 @@ __global__ void __launch_bounds__(kRowThreads) k_feedback_rows(const RowArgs<T> 
   }
 }
 
+// Up to 128 classes: a row lies in the registers of L lanes, four classes a
+// lane (class l + L e in lane l), so the scores are read once.  A warp takes
+// kBatch batches of 32 / L rows at a time and then computes the float64
+// scalars of those rows (a logarithm and two exponentials, as much work as
+// the row's own exponentials) with a lane per row instead of once per L lanes.
+// The derivatives go through shared memory, so that each array is stored as
+// one contiguous piece per warp.
+constexpr int kSmallThreads = 256;
+constexpr int kSmallPer = 4;    // classes a lane
+constexpr int kSmallBatch = 4;  // batches a warp
+constexpr int kSmallClasses = 32 * kSmallPer;
+
+template <typename T, int OP>
+struct SmallWarp {
+  using C = typename Types<T>::C;
+  using Out = typename Types<T>::Out;
+  struct Row {
+    C m, g, h, inv, left;
+    int taken, mode;  // mode 0: zeros, 1: derivatives, 2: NaN
+  };
+  Row row[32];
+  double rest[32];
+  Out stage[kSmallBatch * 32 * kSmallPer];
+};
+
+template <typename T, int OP, int L>
+__global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<T> A) {
+  using C = typename Types<T>::C;
+  using Row = typename Types<T>::Row;
+  using Out = typename Types<T>::Out;
+  constexpr int kRows = 32 / L;                                    // rows of a batch
+  constexpr int kBatches = kSmallBatch < L ? kSmallBatch : L;      // at most a row per lane
+  constexpr int kWarpRows = kRows * kBatches;
+  extern __shared__ __align__(16) unsigned char small_smem[];
+  const int lane = threadIdx.x & 31, l = lane % L;
+  SmallWarp<T, OP>& W = reinterpret_cast<SmallWarp<T, OP>*>(small_smem)[threadIdx.x >> 5];
+  const int K = A.in.K;
+  const long long base = ((long long)blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5)) * kWarpRows;
+  if (base >= A.in.n) return;
+  const int rows = (int)min((long long)kWarpRows, A.in.n - base);
+
+  C v[kBatches][kSmallPer];
+#pragma unroll
+  for (int b = 0; b < kBatches; ++b) {
+    const int i = b * kRows + lane / L;
+    const T* z = A.in.scores + (base + i) * A.in.stride;
+#pragma unroll
+    for (int e = 0; e < kSmallPer; ++e) v[b][e] = i < rows && l + L * e < K ? (C)widen(z[l + L * e]) : (C)-INFINITY;
+  }
+  // this lane's row
+  const long long r = base + lane;
+  const bool mine = lane < rows;
+  long long a = -1;
+  double adv = 0.0, old = 0.0, ref = 0.0, w = 1.0;
+  if (mine) {
+    a = A.in.action(r);
+    if (OP == ROW_POLICY) {
+      adv = (double)A.pol.advantages[r];
+      old = (double)A.pol.old_logp[r];
+      if (A.pol.ref_logp) ref = (double)A.pol.ref_logp[r];
+      if (A.pol.weights) w = (double)A.pol.weights[r];
+    }
+  }
+  bool part = a >= 0 && w != 0.0;
+  const bool bad = part && a >= K;
+  C m = 0;
+  double rest = -1.0;
+  if (OP == ROW_BACK) {
+    if (mine) {
+      m = A.stats[2 * r];
+      rest = (double)A.stats[2 * r + 1];
+      W.row[lane].m = m;
+    }
+    part = part && rest != -1.0;
+    __syncwarp();
+#pragma unroll
+    for (int b = 0; b < kBatches; ++b) {
+      const C mb = W.row[b * kRows + lane / L].m;
+#pragma unroll
+      for (int e = 0; e < kSmallPer; ++e) v[b][e] = exp_c(v[b][e] - mb);
+    }
+  } else {
+#pragma unroll
+    for (int b = 0; b < kBatches; ++b) {
+      C mb = v[b][0];
+#pragma unroll
+      for (int e = 1; e < kSmallPer; ++e) mb = max_nan(mb, v[b][e]);
+#pragma unroll
+      for (int k = L / 2; k > 0; k >>= 1) mb = max_nan(mb, __shfl_xor_sync(0xffffffffu, mb, k));
+      C sum = 0;
+      int ties = 0;
+#pragma unroll
+      for (int e = 0; e < kSmallPer; ++e) {
+        const C x = exp_c(v[b][e] - mb);
+        v[b][e] = x;
+        if (x != (C)1) sum += x;
+        else ++ties;
+      }
+#pragma unroll
+      for (int k = L / 2; k > 0; k >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        ties += __shfl_xor_sync(0xffffffffu, ties, k);
+      }
+      if (l == 0) {
+        W.row[b * kRows + lane / L].m = mb;
+        W.rest[b * kRows + lane / L] = (double)sum + (double)(ties - 1);
+      }
+    }
+    __syncwarp();
+    if (mine) {
+      m = W.row[lane].m;
+      rest = W.rest[lane];
+    }
+    if (m == (C)-INFINITY && !bad) part = false;
+    if (!part) m = 0;
+  }
+
+  // the rows' scalars, a lane each
+  RowDerivative row = {0.0, 0.0};
+  if (OP == ROW_LOGPROBS) {
+    if (mine) {
+      double lp = 0.0;
+      if (part && !bad) lp = (double)widen(A.in.scores[r * A.in.stride + a]) - (double)m - log1p(rest);
+      A.logp[r] = bad ? (Row)NAN : (Row)lp;
+      A.stats[2 * r] = bad ? (Row)NAN : (Row)m;
+      A.stats[2 * r + 1] = bad ? (Row)NAN : part ? (Row)rest : (Row)-1;
+    }
+    return;
+  } else if (OP == ROW_BACK) {
+    if (part) {
+      row.g = (double)A.grad_logp[r];
+      if (A.hess_logp) row.h = (double)A.hess_logp[r];
+    }
+  } else {
+    double lp = 0.0, loss = 0.0;
+    bool near = false;
+    double za = 0.0;
+    if (part && !bad) {
+      za = (double)widen(A.in.scores[r * A.in.stride + a]);
+      lp = za - (double)m - log1p(rest);
+      if (za == -INFINITY) part = false;
+      else near = sizeof(C) == 4 && near_border(A.pol, lp - old, adv, border_slack(kSmallPer + 5, 4.9));
+    }
+    if (sizeof(C) == 4) {
+      for (unsigned todo = __ballot_sync(0xffffffffu, near); todo; todo &= todo - 1) {
+        const int src = __ffs(todo) - 1;
+        const double top = (double)__shfl_sync(0xffffffffu, m, src);
+        const T* z = A.in.scores + (base + src) * A.in.stride;
+        double sum = 0.0;
+        for (int k = lane; k < K; k += 32) sum += exp((double)widen(z[k]) - top);
+        for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        if (lane == src) lp = za - top - log(sum);
+      }
+    }
+    if (bad) lp = loss = NAN;
+    else if (part) row = policy_terms(A.pol, lp, adv, old, ref, w, &loss);
+    if (mine) {
+      if (A.pol.loss) A.pol.loss[r] = (Row)loss;
+      if (A.pol.logp) A.pol.logp[r] = (Row)lp;
+    }
+    if (!A.out.grad) return;
+  }
+  W.row[lane].g = (C)row.g;
+  W.row[lane].h = (C)row.h;
+  W.row[lane].inv = (C)(1.0 / (1.0 + rest));
+  W.row[lane].left = (C)(rest / (1.0 + rest));
+  W.row[lane].taken = (int)a;
+  W.row[lane].mode = bad ? 2 : part ? 1 : 0;
+  __syncwarp();
+
+  // derivatives, staged row by row
+  const bool want_h = A.out.hess != nullptr;
+#pragma unroll 1
+  for (int pass = 0; pass < (want_h ? 2 : 1); ++pass) {
+#pragma unroll
+    for (int b = 0; b < kBatches; ++b) {
+      const int i = b * kRows + lane / L;
+      const typename SmallWarp<T, OP>::Row R = W.row[i];
+#pragma unroll
+      for (int e = 0; e < kSmallPer; ++e) {
+        const int k = l + L * e;
+        C dg, dh = 0;
+        derivative<C>(v[b][e], R.inv, R.left, k == R.taken, R.g, R.h, pass == 1, &dg, &dh);
+        const C d = pass == 1 ? dh : dg;
+        if (i < rows && k < K) narrow(R.mode == 1 ? d : R.mode == 0 ? (C)0 : (C)NAN, W.stage[i * K + k]);
+      }
+    }
+    __syncwarp();
+    Out* to = pass == 1 ? A.out.hess : A.out.grad;
+    if (A.out.class_stride == 1 && A.out.row_stride == K) {
+      for (int j = lane; j < rows * K; j += 32) to[base * K + j] = W.stage[j];
+    } else {
+      for (int j = lane; j < rows * K; j += 32) {
+        const int k = j / rows, i = j % rows;
+        to[(base + i) * A.out.row_stride + k * A.out.class_stride] = W.stage[i * K + k];
+      }
+    }
+    __syncwarp();
+  }
+}
+
+template <typename T, int OP, int L>
+void launch_small_t(const RowArgs<T>& A, cudaStream_t st) {
+  constexpr int per_block = (32 / L) * (kSmallBatch < L ? kSmallBatch : L) * (kSmallThreads / 32);
+  const size_t smem = sizeof(SmallWarp<T, OP>) * (kSmallThreads / 32);
+  k_feedback_small<T, OP, L><<<(unsigned)((A.in.n + per_block - 1) / per_block), kSmallThreads, smem, st>>>(A);
+}
+
 template <typename T, int OP>
 void launch_rows_t(const RowArgs<T>& A, cudaStream_t st) {
   if (A.in.n == 0) return;
+  if (A.in.K <= kSmallClasses) {
+    const int lanes = (A.in.K + kSmallPer - 1) / kSmallPer;
+    if (lanes <= 1) launch_small_t<T, OP, 1>(A, st);
+    else if (lanes <= 2) launch_small_t<T, OP, 2>(A, st);
+    else if (lanes <= 4) launch_small_t<T, OP, 4>(A, st);
+    else if (lanes <= 8) launch_small_t<T, OP, 8>(A, st);
+    else if (lanes <= 16) launch_small_t<T, OP, 16>(A, st);
+    else launch_small_t<T, OP, 32>(A, st);
+    MTB_CUDA_FB(cudaGetLastError());
+    return;
+  }
   const unsigned grid = (unsigned)std::min<long long>(A.in.n, 1 << 20);
   k_feedback_rows<T, OP><<<grid, kRowThreads, 0, st>>>(A);
   MTB_CUDA_FB(cudaGetLastError());
