@@ -290,225 +290,316 @@ __global__ void __launch_bounds__(kRowThreads) k_feedback_rows(const RowArgs<T> 
   }
 }
 
-// Up to 128 classes: a row lies in the registers of L lanes, four classes a
-// lane (class l + L e in lane l), so the scores are read once.  A warp takes
-// kBatch batches of 32 / L rows at a time and then computes the float64
-// scalars of those rows (a logarithm and two exponentials, as much work as
-// the row's own exponentials) with a lane per row instead of once per L lanes.
-// The derivatives go through shared memory, so that each array is stored as
-// one contiguous piece per warp.
-constexpr int kSmallThreads = 256;
-constexpr int kSmallPer = 4;    // classes a lane
-constexpr int kSmallBatch = 4;  // batches a warp
-constexpr int kSmallClasses = 32 * kSmallPer;
+// ---------------------------------------------------------------------------
+// Rows of up to 128 classes
+//
+// A warp copies 32 / L whole rows into shared memory, L lanes take a row each
+// (class l + L e in lane l, at most 16 a lane), and the derivatives go back
+// through the same memory, so every array crosses the memory system once and
+// in one piece per warp.  With L = 1 (up to 16 classes) no lane waits for
+// another.  A row's float64 scalars, a logarithm, two exponentials and a
+// quotient, cost as much as ten classes; every lane of a row computes them.
+// ---------------------------------------------------------------------------
 
-template <typename T, int OP>
-struct SmallWarp {
-  using C = typename Types<T>::C;
-  using Out = typename Types<T>::Out;
-  struct Row {
-    C m, g, h, inv, left;
-    int taken, mode;  // mode 0: zeros, 1: derivatives, 2: NaN
-  };
-  Row row[32];
-  double rest[32];
-  Out stage[kSmallBatch * 32 * kSmallPer];
+constexpr int kSmallThreads = 128;
+constexpr int kSmallPer = 16;  // classes a lane
+constexpr int kSmallClasses = 8 * kSmallPer;
+
+// exp(d) of d <= 0 in float64 by table and polynomial (P. T. P. Tang, "Table-
+// driven implementation of the exponential function in IEEE floating-point
+// arithmetic", ACM TOMS 15(2), 1989): d = (n / 32) ln 2 + r, exp(d) =
+// 2^(n / 32) (1 + r + ... + r^6 / 720), the truncation below 2^-57 for |r| <=
+// ln 2 / 64.  NaN stays; below -708 (3e-308) the value is 0.
+struct ExpTable {
+  const double* two;  // 2^(j / 32), shared memory
+  __device__ __forceinline__ double operator()(double d) const {
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+    const bool none = d < -708.0;
+    d = none ? 0.0 : d;
+    const double t = fma(d, 46.166241308446828, kRound);
+    const int n = __double2loint(t);
+    const double k = t - kRound;
+    double r = fma(k, -2.1660849392498290e-2, d);  // ln 2 / 32, and its rounding error
+    r = fma(k, -7.2470212932696861e-19, r);
+    double q = fma(r, 1.0 / 720.0, 1.0 / 120.0);
+    q = fma(q, r, 1.0 / 24.0);
+    q = fma(q, r, 1.0 / 6.0);
+    q = fma(q, r, 0.5);
+    q = fma(q, r * r, r);
+    const double two_n = two[n & 31];
+    const double scaled = __hiloint2double(__double2hiint(two_n) + (n >> 5 << 20), __double2loint(two_n));
+    return none ? 0.0 : fma(scaled, q, scaled);
+  }
+  __device__ __forceinline__ float operator()(float d) const { return __expf(d); }
+};
+
+// Rows in shared memory: a row of a multiple of 16 bytes starts at an odd
+// multiple of 16, so that lanes reading the same class of different rows meet
+// at most four to a bank; other rows follow each other directly.
+struct TileRows {
+  int bytes, stride;
+  __host__ __device__ explicit TileRows(int row_bytes)
+      : bytes(row_bytes), stride(row_bytes % 16 == 0 ? (row_bytes / 16 | 1) * 16 : row_bytes) {}
+};
+
+// A lane's walk over the elements lane, lane + 32, ... of rows of `width`.
+struct RowWalk {
+  int row, col, width, step_row, step_col;
+  __device__ __forceinline__ RowWalk(int lane, int w)
+      : row(lane / w), col(lane % w), width(w), step_row(32 / w), step_col(32 % w) {}
+  __device__ __forceinline__ void next() {
+    row += step_row;
+    col += step_col;
+    if (col >= width) {
+      col -= width;
+      ++row;
+    }
+  }
+};
+
+// Copies `rows` rows of K elements between global memory (row_stride and
+// class_stride elements apart) and shared memory; the whole warp calls it.
+// vec: the rows are one piece of global memory that starts on 16 bytes.
+template <bool TO_SHARED, typename E>
+__device__ __forceinline__ void copy_rows(E* global, unsigned char* tile, TileRows R, int rows, int K,
+                                          long long row_stride, long long class_stride, bool vec) {
+  const int lane = threadIdx.x & 31;
+  if (vec) {
+    const int total = rows * R.bytes;
+    if (R.bytes % 16 == 0) {
+      RowWalk at(lane, R.bytes / 16);
+      for (int c = lane * 16; c < total; c += 512, at.next()) {
+        uint4* sh = reinterpret_cast<uint4*>(tile + at.row * R.stride + at.col * 16);
+        uint4* gl = reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(global) + c);
+        if (TO_SHARED) *sh = *gl;
+        else *gl = *sh;
+      }
+    } else {
+      for (int c = lane * 16; c + 16 <= total; c += 512) {
+        uint4* sh = reinterpret_cast<uint4*>(tile + c);
+        uint4* gl = reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(global) + c);
+        if (TO_SHARED) *sh = *gl;
+        else *gl = *sh;
+      }
+      E* sh = reinterpret_cast<E*>(tile);
+      for (int j = total / 16 * 16 / (int)sizeof(E) + lane; j < total / (int)sizeof(E); j += 32) {
+        if (TO_SHARED) sh[j] = global[j];
+        else global[j] = sh[j];
+      }
+    }
+  } else if (class_stride == 1) {
+    RowWalk at(lane, K);
+    for (; at.row < rows; at.next()) {
+      E& sh = reinterpret_cast<E*>(tile + at.row * R.stride)[at.col];
+      E& gl = global[at.row * row_stride + at.col];
+      if (TO_SHARED) sh = gl;
+      else gl = sh;
+    }
+  } else {  // classes apart: rows next to each other
+    RowWalk at(lane, rows);
+    for (; at.row < K; at.next()) {
+      E& sh = reinterpret_cast<E*>(tile + at.col * R.stride)[at.row];
+      E& gl = global[at.col * row_stride + at.row * class_stride];
+      if (TO_SHARED) sh = gl;
+      else gl = sh;
+    }
+  }
+}
+
+struct SmallLayout {
+  int tile;              // bytes of a warp's tile
+  bool vec_in, vec_out;  // see copy_rows
 };
 
 template <typename T, int OP, int L>
-__global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<T> A) {
+__global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<T> A, const SmallLayout lay) {
   using C = typename Types<T>::C;
   using Row = typename Types<T>::Row;
   using Out = typename Types<T>::Out;
-  constexpr int kRows = 32 / L;                                    // rows of a batch
-  constexpr int kBatches = kSmallBatch < L ? kSmallBatch : L;      // at most a row per lane
-  constexpr int kWarpRows = kRows * kBatches;
+  constexpr int kRows = 32 / L;
   extern __shared__ __align__(16) unsigned char small_smem[];
+  __shared__ double two[32];
+  const ExpTable ex = {two};
+  if (sizeof(C) == 8) {
+    if (threadIdx.x < 32) two[threadIdx.x] = exp2(threadIdx.x / 32.0);
+    __syncthreads();
+  }
   const int lane = threadIdx.x & 31, l = lane % L;
-  SmallWarp<T, OP>& W = reinterpret_cast<SmallWarp<T, OP>*>(small_smem)[threadIdx.x >> 5];
   const int K = A.in.K;
-  const long long base = ((long long)blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5)) * kWarpRows;
-  if (base >= A.in.n) return;
-  const int rows = (int)min((long long)kWarpRows, A.in.n - base);
-
-  C v[kBatches][kSmallPer];
-#pragma unroll
-  for (int b = 0; b < kBatches; ++b) {
-    const int i = b * kRows + lane / L;
-    const T* z = A.in.scores + (base + i) * A.in.stride;
-#pragma unroll
-    for (int e = 0; e < kSmallPer; ++e) v[b][e] = i < rows && l + L * e < K ? (C)widen(z[l + L * e]) : (C)-INFINITY;
-  }
-  // this lane's row
-  const long long r = base + lane;
-  const bool mine = lane < rows;
-  long long a = -1;
-  double adv = 0.0, old = 0.0, ref = 0.0, w = 1.0;
-  if (mine) {
-    a = A.in.action(r);
-    if (OP == ROW_POLICY) {
-      adv = (double)A.pol.advantages[r];
-      old = (double)A.pol.old_logp[r];
-      if (A.pol.ref_logp) ref = (double)A.pol.ref_logp[r];
-      if (A.pol.weights) w = (double)A.pol.weights[r];
-    }
-  }
-  bool part = a >= 0 && w != 0.0;
-  const bool bad = part && a >= K;
-  C m = 0;
-  double rest = -1.0;
-  if (OP == ROW_BACK) {
+  unsigned char* tile = small_smem + (threadIdx.x >> 5) * lay.tile;
+  const TileRows in_rows(K * (int)sizeof(T)), out_rows(K * (int)sizeof(Out));
+  const long long step = (long long)gridDim.x * (kSmallThreads / 32) * kRows;
+  for (long long base = ((long long)blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5)) * kRows; base < A.in.n;
+       base += step) {
+    const int rows = (int)min((long long)kRows, A.in.n - base);
+    copy_rows<true>(const_cast<T*>(A.in.scores) + base * A.in.stride, tile, in_rows, rows, K, A.in.stride, 1, lay.vec_in);
+    const int i = lane / L;  // this lane's row
+    const bool mine = i < rows;
+    const long long r = base + i;
+    long long a = -1;
+    double adv = 0.0, old = 0.0, ref = 0.0, w = 1.0, rest = -1.0;
+    RowDerivative row = {0.0, 0.0};
+    C m = 0;
     if (mine) {
-      m = A.stats[2 * r];
-      rest = (double)A.stats[2 * r + 1];
-      W.row[lane].m = m;
+      a = A.in.action(r);
+      if (OP == ROW_POLICY) {
+        adv = (double)A.pol.advantages[r];
+        old = (double)A.pol.old_logp[r];
+        if (A.pol.ref_logp) ref = (double)A.pol.ref_logp[r];
+        if (A.pol.weights) w = (double)A.pol.weights[r];
+      }
+      if (OP == ROW_BACK) {
+        m = A.stats[2 * r];
+        rest = (double)A.stats[2 * r + 1];
+        row.g = (double)A.grad_logp[r];
+        if (A.hess_logp) row.h = (double)A.hess_logp[r];
+      }
     }
-    part = part && rest != -1.0;
+    bool part = a >= 0 && w != 0.0 && (OP != ROW_BACK || rest != -1.0);
+    const bool bad = part && a >= K;
     __syncwarp();
+    const T* z = reinterpret_cast<const T*>(tile + i * in_rows.stride);
+    const double za = (double)widen(part && !bad ? z[a] : z[0]);
+    C v[kSmallPer];
+    if (OP != ROW_BACK) {
+      C mx = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < kBatches; ++b) {
-      const C mb = W.row[b * kRows + lane / L].m;
+      for (int e = 0; e < kSmallPer; ++e) {
+        v[e] = -INFINITY;
+        if (e * L < K) {
+          if (l + e * L < K && mine) v[e] = widen(z[l + e * L]);
+          mx = max_nan(mx, v[e]);
+        }
+      }
 #pragma unroll
-      for (int e = 0; e < kSmallPer; ++e) v[b][e] = exp_c(v[b][e] - mb);
-    }
-  } else {
-#pragma unroll
-    for (int b = 0; b < kBatches; ++b) {
-      C mb = v[b][0];
-#pragma unroll
-      for (int e = 1; e < kSmallPer; ++e) mb = max_nan(mb, v[b][e]);
-#pragma unroll
-      for (int k = L / 2; k > 0; k >>= 1) mb = max_nan(mb, __shfl_xor_sync(0xffffffffu, mb, k));
+      for (int k = L / 2; k > 0; k >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, k));
       C sum = 0;
       int ties = 0;
 #pragma unroll
       for (int e = 0; e < kSmallPer; ++e) {
-        const C x = exp_c(v[b][e] - mb);
-        v[b][e] = x;
-        if (x != (C)1) sum += x;
-        else ++ties;
+        if (e * L < K) {
+          v[e] = ex(v[e] - mx);
+          if (v[e] != (C)1) sum += v[e];
+          else ++ties;
+        }
       }
 #pragma unroll
       for (int k = L / 2; k > 0; k >>= 1) {
         sum += __shfl_xor_sync(0xffffffffu, sum, k);
         ties += __shfl_xor_sync(0xffffffffu, ties, k);
       }
-      if (l == 0) {
-        W.row[b * kRows + lane / L].m = mb;
-        W.rest[b * kRows + lane / L] = (double)sum + (double)(ties - 1);
+      if (mx == (C)-INFINITY && !bad) part = false;
+      if (part) {
+        m = mx;
+        rest = (double)sum + (double)(ties - 1);
       }
-    }
-    __syncwarp();
-    if (mine) {
-      m = W.row[lane].m;
-      rest = W.rest[lane];
-    }
-    if (m == (C)-INFINITY && !bad) part = false;
-    if (!part) m = 0;
-  }
-
-  // the rows' scalars, a lane each
-  RowDerivative row = {0.0, 0.0};
-  if (OP == ROW_LOGPROBS) {
-    if (mine) {
-      double lp = 0.0;
-      if (part && !bad) lp = (double)widen(A.in.scores[r * A.in.stride + a]) - (double)m - log1p(rest);
-      A.logp[r] = bad ? (Row)NAN : (Row)lp;
-      A.stats[2 * r] = bad ? (Row)NAN : (Row)m;
-      A.stats[2 * r + 1] = bad ? (Row)NAN : part ? (Row)rest : (Row)-1;
-    }
-    return;
-  } else if (OP == ROW_BACK) {
-    if (part) {
-      row.g = (double)A.grad_logp[r];
-      if (A.hess_logp) row.h = (double)A.hess_logp[r];
-    }
-  } else {
-    double lp = 0.0, loss = 0.0;
-    bool near = false;
-    double za = 0.0;
-    if (part && !bad) {
-      za = (double)widen(A.in.scores[r * A.in.stride + a]);
-      lp = za - (double)m - log1p(rest);
-      if (za == -INFINITY) part = false;
-      else near = sizeof(C) == 4 && near_border(A.pol, lp - old, adv, border_slack(kSmallPer + 5, 4.9));
-    }
-    if (sizeof(C) == 4) {
-      for (unsigned todo = __ballot_sync(0xffffffffu, near); todo; todo &= todo - 1) {
-        const int src = __ffs(todo) - 1;
-        const double top = (double)__shfl_sync(0xffffffffu, m, src);
-        const T* z = A.in.scores + (base + src) * A.in.stride;
-        double sum = 0.0;
-        for (int k = lane; k < K; k += 32) sum += exp((double)widen(z[k]) - top);
-        for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-        if (lane == src) lp = za - top - log(sum);
-      }
-    }
-    if (bad) lp = loss = NAN;
-    else if (part) row = policy_terms(A.pol, lp, adv, old, ref, w, &loss);
-    if (mine) {
-      if (A.pol.loss) A.pol.loss[r] = (Row)loss;
-      if (A.pol.logp) A.pol.logp[r] = (Row)lp;
-    }
-    if (!A.out.grad) return;
-  }
-  W.row[lane].g = (C)row.g;
-  W.row[lane].h = (C)row.h;
-  W.row[lane].inv = (C)(1.0 / (1.0 + rest));
-  W.row[lane].left = (C)(rest / (1.0 + rest));
-  W.row[lane].taken = (int)a;
-  W.row[lane].mode = bad ? 2 : part ? 1 : 0;
-  __syncwarp();
-
-  // derivatives, staged row by row
-  const bool want_h = A.out.hess != nullptr;
-#pragma unroll 1
-  for (int pass = 0; pass < (want_h ? 2 : 1); ++pass) {
+    } else {
 #pragma unroll
-    for (int b = 0; b < kBatches; ++b) {
-      const int i = b * kRows + lane / L;
-      const typename SmallWarp<T, OP>::Row R = W.row[i];
+      for (int e = 0; e < kSmallPer; ++e)
+        if (e * L < K) v[e] = l + e * L < K && mine ? ex((C)widen(z[l + e * L]) - m) : (C)0;
+    }
+
+    if (OP == ROW_LOGPROBS) {
+      if (mine && l == 0) {
+        const double lp = part && !bad ? za - (double)m - log1p(rest) : 0.0;
+        A.logp[r] = bad ? (Row)NAN : (Row)lp;
+        A.stats[2 * r] = bad ? (Row)NAN : (Row)m;
+        A.stats[2 * r + 1] = bad ? (Row)NAN : part ? (Row)rest : (Row)-1;
+      }
+      __syncwarp();
+      continue;
+    }
+    if (OP == ROW_POLICY) {
+      double lp = 0.0, loss = 0.0;
+      if (part && !bad) {
+        lp = za - (double)m - log1p(rest);
+        part = za != -INFINITY;
+      }
+      if (sizeof(C) == 4) {
+        const bool near = part && !bad && near_border(A.pol, lp - old, adv, border_slack(kSmallPer + 3, 4.9));
+        if (__any_sync(0xffffffffu, near)) {
+          double sum = 0.0;
+          for (int k = l; k < K && near; k += L) sum += exp((double)widen(z[k]) - (double)m);
+#pragma unroll
+          for (int k = L / 2; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+          if (near) lp = za - (double)m - log(sum);
+        }
+      }
+      if (bad) lp = loss = NAN;
+      else if (part) row = policy_terms(A.pol, lp, adv, old, ref, w, &loss);
+      if (mine && l == 0) {
+        if (A.pol.loss) A.pol.loss[r] = (Row)loss;
+        if (A.pol.logp) A.pol.logp[r] = (Row)lp;
+      }
+      if (!A.out.grad) {
+        __syncwarp();
+        continue;
+      }
+    }
+    __syncwarp();  // the scores are used up: the derivatives take their place
+    const double inv_total = 1.0 / (1.0 + rest);
+    const C inv = (C)inv_total, left = (C)(rest * inv_total), g = (C)row.g, h = (C)row.h;
+    const bool want_h = A.out.hess != nullptr;
+    unsigned char* tile_h = tile + kRows * out_rows.stride;
+    if (mine) {
+      Out* to_g = reinterpret_cast<Out*>(tile + i * out_rows.stride);
+      Out* to_h = reinterpret_cast<Out*>(tile_h + i * out_rows.stride);
+      const bool plain = part && !bad;
+      const C fill = bad ? (C)NAN : (C)0;
 #pragma unroll
       for (int e = 0; e < kSmallPer; ++e) {
-        const int k = l + L * e;
-        C dg, dh = 0;
-        derivative<C>(v[b][e], R.inv, R.left, k == R.taken, R.g, R.h, pass == 1, &dg, &dh);
-        const C d = pass == 1 ? dh : dg;
-        if (i < rows && k < K) narrow(R.mode == 1 ? d : R.mode == 0 ? (C)0 : (C)NAN, W.stage[i * K + k]);
+        const int k = l + e * L;
+        if (e * L < K && k < K) {
+          C dg, dh = 0;
+          derivative<C>(v[e], inv, left, k == (int)a, g, h, want_h, &dg, &dh);
+          narrow(plain ? dg : fill, to_g[k]);
+          if (want_h) narrow(plain ? dh : fill, to_h[k]);
+        }
       }
     }
     __syncwarp();
-    Out* to = pass == 1 ? A.out.hess : A.out.grad;
-    if (A.out.class_stride == 1 && A.out.row_stride == K) {
-      for (int j = lane; j < rows * K; j += 32) to[base * K + j] = W.stage[j];
-    } else {
-      for (int j = lane; j < rows * K; j += 32) {
-        const int k = j / rows, i = j % rows;
-        to[(base + i) * A.out.row_stride + k * A.out.class_stride] = W.stage[i * K + k];
-      }
-    }
+    const long long to = base * A.out.row_stride;
+    copy_rows<false>(A.out.grad + to, tile, out_rows, rows, K, A.out.row_stride, A.out.class_stride, lay.vec_out);
+    if (want_h)
+      copy_rows<false>(A.out.hess + to, tile_h, out_rows, rows, K, A.out.row_stride, A.out.class_stride, lay.vec_out);
     __syncwarp();
   }
 }
 
+inline bool on16(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+int multiprocessors() {
+  int dev = 0, n = 0;
+  MTB_CUDA_FB(cudaGetDevice(&dev));
+  MTB_CUDA_FB(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+  return n;
+}
+
 template <typename T, int OP, int L>
 void launch_small_t(const RowArgs<T>& A, cudaStream_t st) {
-  constexpr int per_block = (32 / L) * (kSmallBatch < L ? kSmallBatch : L) * (kSmallThreads / 32);
-  const size_t smem = sizeof(SmallWarp<T, OP>) * (kSmallThreads / 32);
-  k_feedback_small<T, OP, L><<<(unsigned)((A.in.n + per_block - 1) / per_block), kSmallThreads, smem, st>>>(A);
+  using Out = typename Types<T>::Out;
+  constexpr int rows = 32 / L, warps = kSmallThreads / 32;
+  const int K = A.in.K;
+  const TileRows in(K * (int)sizeof(T)), out(K * (int)sizeof(Out));
+  SmallLayout lay;
+  const int back = OP == ROW_LOGPROBS || !A.out.grad ? 0 : rows * out.stride * (A.out.hess ? 2 : 1);
+  lay.tile = (std::max(rows * in.stride, back) + 15) / 16 * 16;
+  lay.vec_in = on16(A.in.scores) && A.in.stride == K && rows * in.bytes % 16 == 0;
+  lay.vec_out = on16(A.out.grad) && on16(A.out.hess) && A.out.row_stride == K && A.out.class_stride == 1 &&
+                rows * out.bytes % 16 == 0;
+  const long long blocks = (A.in.n + rows * warps - 1) / (rows * warps);
+  const unsigned grid = (unsigned)std::min<long long>(blocks, 16ll * multiprocessors());
+  k_feedback_small<T, OP, L><<<grid, kSmallThreads, (size_t)lay.tile * warps, st>>>(A, lay);
 }
 
 template <typename T, int OP>
 void launch_rows_t(const RowArgs<T>& A, cudaStream_t st) {
   if (A.in.n == 0) return;
   if (A.in.K <= kSmallClasses) {
-    const int lanes = (A.in.K + kSmallPer - 1) / kSmallPer;
-    if (lanes <= 1) launch_small_t<T, OP, 1>(A, st);
-    else if (lanes <= 2) launch_small_t<T, OP, 2>(A, st);
-    else if (lanes <= 4) launch_small_t<T, OP, 4>(A, st);
-    else if (lanes <= 8) launch_small_t<T, OP, 8>(A, st);
-    else if (lanes <= 16) launch_small_t<T, OP, 16>(A, st);
-    else launch_small_t<T, OP, 32>(A, st);
+    if (A.in.K <= kSmallPer) launch_small_t<T, OP, 1>(A, st);
+    else if (A.in.K <= 2 * kSmallPer) launch_small_t<T, OP, 2>(A, st);
+    else if (A.in.K <= 4 * kSmallPer) launch_small_t<T, OP, 4>(A, st);
+    else launch_small_t<T, OP, 8>(A, st);
     MTB_CUDA_FB(cudaGetLastError());
     return;
   }

@@ -72,10 +72,12 @@ def exp_error(d, f64):
 
 def sum_error(K, p, d, f64):
     """Bound of the relative error of a row's sum: each term's own, and the
-    additions of at most ceil(K / 256) + 8 terms one after the other in the
-    scores' arithmetic (the sums across threads are in float64)."""
+    additions of n positive terms one after the other in the scores'
+    arithmetic, which change the sum by at most (n - 1) half steps.  Rows of up
+    to 128 classes: at most 16 terms in a lane, then 3 sums of lanes; longer
+    rows: ceil(K / 256) in a thread, and float64 across threads."""
     terms = (p * exp_error(d, f64)).sum(1)
-    return terms + (K // 256 + 9) * (2.0 ** -53 if f64 else U32)
+    return terms + (min(K, 16) + K // 256 + 4) * (2.0 ** -53 if f64 else U32)
 
 
 def pairs_loss(s, ref, i, j, w, beta, eps, kind):

@@ -160,7 +160,7 @@ def _row_bounds(z, p, stats, logp, f64):
     # the largest class's complement sums the others: each term's own error
     with np.errstate(invalid="ignore"):
         far = np.where(p > 0, fu.exp_error(d, f64), 0.0).max(1)
-    e_left = far + (z.shape[1] // 256 + 9) * unit + e_sum + 4 * unit
+    e_left = far + (min(z.shape[1], 16) + z.shape[1] // 256 + 4) * unit + e_sum + 4 * unit
     return e_l, e_p, e_left
 
 
