@@ -129,21 +129,21 @@ struct RowDerivative {
 };
 
 // Loss of a row with log probability l, and its derivatives in l.
-template <typename T>
+template <typename T, typename Exp>
 __device__ __forceinline__ RowDerivative policy_terms(const PolicyPointers<T>& t, double l, double adv, double old,
-                                                      double ref, double w, double* loss) {
+                                                      double ref, double w, double* loss, Exp exp_f) {
   const double d = l - old;
-  const double ra = exp(d) * adv;
+  const double ra = exp_f(d) * adv;
   const bool active = adv >= 0.0 ? d <= t.log_high : d >= t.log_low;
   double v = active ? -ra : (adv >= 0.0 ? -t.clip_high * adv : -t.clip_low * adv);
   double g = active ? -ra : 0.0;
   if (ra != ra) v = g = ra;
   double h = g > 0.0 ? g : 0.0;
   if (t.ref_logp) {
-    const double e = expm1(ref - l);
-    v += t.kl * (e - (ref - l));
-    g -= t.kl * e;
-    h += t.kl * (e + 1.0);
+    const double e = exp_f(ref - l);
+    v += t.kl * (e - 1.0 - (ref - l));
+    g -= t.kl * (e - 1.0);
+    h += t.kl * e;
   }
   *loss = w * v;
   return {w * g, w * h};
@@ -264,7 +264,8 @@ __global__ void __launch_bounds__(kRowThreads) k_feedback_rows(const RowArgs<T> 
             l = za - (double)m - log(block_reduce(s, sm_d, add_f64));
           }
           row = policy_terms(A.pol, l, adv, old, A.pol.ref_logp ? (double)A.pol.ref_logp[r] : 0.0,
-                             A.pol.weights ? (double)A.pol.weights[r] : 1.0, &loss);
+                             A.pol.weights ? (double)A.pol.weights[r] : 1.0, &loss,
+                             [](double d) { return exp(d); });
         }
       }
       if (threadIdx.x == 0) {
@@ -305,17 +306,17 @@ constexpr int kSmallThreads = 128;
 constexpr int kSmallPer = 16;  // classes a lane
 constexpr int kSmallClasses = 8 * kSmallPer;
 
-// exp(d) of d <= 0 in float64 by table and polynomial (P. T. P. Tang, "Table-
-// driven implementation of the exponential function in IEEE floating-point
+// exp(d) in float64 by table and polynomial (P. T. P. Tang, "Table-driven
+// implementation of the exponential function in IEEE floating-point
 // arithmetic", ACM TOMS 15(2), 1989): d = (n / 32) ln 2 + r, exp(d) =
 // 2^(n / 32) (1 + r + ... + r^6 / 720), the truncation below 2^-57 for |r| <=
 // ln 2 / 64.  NaN stays; below -708 (3e-308) the value is 0.
 struct ExpTable {
-  const double* two;  // 2^(j / 32), shared memory
-  __device__ __forceinline__ double operator()(double d) const {
+  const double* two;  // shared memory: 2^(j / 32) for j < 32, then 0
+  __device__ __forceinline__ double operator()(double d) const {  // d <= 709.78
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
     const bool none = d < -708.0;
-    d = none ? 0.0 : d;
+    d = __hiloint2double(none ? 0 : __double2hiint(d), __double2loint(d));
     const double t = fma(d, 46.166241308446828, kRound);
     const int n = __double2loint(t);
     const double k = t - kRound;
@@ -326,11 +327,17 @@ struct ExpTable {
     q = fma(q, r, 1.0 / 6.0);
     q = fma(q, r, 0.5);
     q = fma(q, r * r, r);
-    const double two_n = two[n & 31];
+    const double two_n = two[none ? 32 : n & 31];
     const double scaled = __hiloint2double(__double2hiint(two_n) + (n >> 5 << 20), __double2loint(two_n));
-    return none ? 0.0 : fma(scaled, q, scaled);
+    return fma(scaled, q, scaled);
   }
   __device__ __forceinline__ float operator()(float d) const { return __expf(d); }
+  __device__ __forceinline__ double scalar(double d) const { return d > 709.78 ? INFINITY : (*this)(d); }
+  __device__ __forceinline__ void fill(double* to) {
+    if (threadIdx.x < 33) to[threadIdx.x] = threadIdx.x < 32 ? exp2(threadIdx.x / 32.0) : 0.0;
+    __syncthreads();
+    two = to;
+  }
 };
 
 // Rows in shared memory: a row of a multiple of 16 bytes starts at an odd
@@ -357,146 +364,200 @@ struct RowWalk {
   }
 };
 
-// Copies `rows` rows of K elements between global memory (row_stride and
-// class_stride elements apart) and shared memory; the whole warp calls it.
-// vec: the rows are one piece of global memory that starts on 16 bytes.
-template <bool TO_SHARED, typename E>
-__device__ __forceinline__ void copy_rows(E* global, unsigned char* tile, TileRows R, int rows, int K,
-                                          long long row_stride, long long class_stride, bool vec) {
+// Asynchronous copy of 16 bytes to shared memory, past L1 and the registers.
+__device__ __forceinline__ void copy_async16(void* shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(shared)),
+               "l"(global)
+               : "memory");
+}
+
+// Starts the copy of `rows` rows of K elements, row_stride apart, into shared
+// memory; copies_wait ends it.  The whole warp calls both.  vec: the rows are
+// one piece of global memory that starts on 16 bytes.
+template <typename E>
+__device__ __forceinline__ void rows_in(const E* global, unsigned char* tile, TileRows R, int rows, int K,
+                                        long long row_stride, bool vec) {
   const int lane = threadIdx.x & 31;
   if (vec) {
     const int total = rows * R.bytes;
-    if (R.bytes % 16 == 0) {
+    const unsigned char* from = reinterpret_cast<const unsigned char*>(global);
+    if (R.stride != R.bytes) {
       RowWalk at(lane, R.bytes / 16);
-      for (int c = lane * 16; c < total; c += 512, at.next()) {
-        uint4* sh = reinterpret_cast<uint4*>(tile + at.row * R.stride + at.col * 16);
-        uint4* gl = reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(global) + c);
-        if (TO_SHARED) *sh = *gl;
-        else *gl = *sh;
-      }
+      for (int c = lane * 16; c < total; c += 512, at.next()) copy_async16(tile + at.row * R.stride + at.col * 16, from + c);
     } else {
-      for (int c = lane * 16; c + 16 <= total; c += 512) {
-        uint4* sh = reinterpret_cast<uint4*>(tile + c);
-        uint4* gl = reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(global) + c);
-        if (TO_SHARED) *sh = *gl;
-        else *gl = *sh;
+      for (int c = lane * 16; c + 16 <= total; c += 512) copy_async16(tile + c, from + c);
+      for (int j = total / 16 * 16 / (int)sizeof(E) + lane; j < total / (int)sizeof(E); j += 32)
+        reinterpret_cast<E*>(tile)[j] = global[j];
+    }
+  } else {
+    RowWalk at(lane, K);
+    while (at.row < rows) {  // four loads in flight
+      E x[4];
+      E* to[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q, at.next()) {
+        to[q] = nullptr;
+        if (at.row < rows) {
+          to[q] = reinterpret_cast<E*>(tile + at.row * R.stride) + at.col;
+          x[q] = global[at.row * row_stride + at.col];
+        }
       }
-      E* sh = reinterpret_cast<E*>(tile);
-      for (int j = total / 16 * 16 / (int)sizeof(E) + lane; j < total / (int)sizeof(E); j += 32) {
-        if (TO_SHARED) sh[j] = global[j];
-        else global[j] = sh[j];
-      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (to[q]) *to[q] = x[q];
+    }
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+template <int LATER>  // how many copies started after the one waited for may still run
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory");
+  __syncwarp();
+}
+
+// Rows from shared memory to global memory, elements row_stride and
+// class_stride apart; vec as above.
+template <typename E>
+__device__ __forceinline__ void rows_out(E* global, const unsigned char* tile, TileRows R, int rows, int K,
+                                         long long row_stride, long long class_stride, bool vec) {
+  const int lane = threadIdx.x & 31;
+  if (vec) {
+    const int total = rows * R.bytes;
+    unsigned char* to = reinterpret_cast<unsigned char*>(global);
+    if (R.stride != R.bytes) {
+      RowWalk at(lane, R.bytes / 16);
+      for (int c = lane * 16; c < total; c += 512, at.next())
+        *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(tile + at.row * R.stride + at.col * 16);
+    } else {
+      for (int c = lane * 16; c + 16 <= total; c += 512)
+        *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(tile + c);
+      for (int j = total / 16 * 16 / (int)sizeof(E) + lane; j < total / (int)sizeof(E); j += 32)
+        global[j] = reinterpret_cast<const E*>(tile)[j];
     }
   } else if (class_stride == 1) {
-    RowWalk at(lane, K);
-    for (; at.row < rows; at.next()) {
-      E& sh = reinterpret_cast<E*>(tile + at.row * R.stride)[at.col];
-      E& gl = global[at.row * row_stride + at.col];
-      if (TO_SHARED) sh = gl;
-      else gl = sh;
-    }
+    for (RowWalk at(lane, K); at.row < rows; at.next())
+      global[at.row * row_stride + at.col] = reinterpret_cast<const E*>(tile + at.row * R.stride)[at.col];
   } else {  // classes apart: rows next to each other
-    RowWalk at(lane, rows);
-    for (; at.row < K; at.next()) {
-      E& sh = reinterpret_cast<E*>(tile + at.col * R.stride)[at.row];
-      E& gl = global[at.col * row_stride + at.row * class_stride];
-      if (TO_SHARED) sh = gl;
-      else gl = sh;
-    }
+    for (RowWalk at(lane, rows); at.row < K; at.next())
+      global[at.col * row_stride + at.row * class_stride] = reinterpret_cast<const E*>(tile + at.col * R.stride)[at.row];
   }
 }
 
 struct SmallLayout {
-  int tile;              // bytes of a warp's tile
-  bool vec_in, vec_out;  // see copy_rows
+  int tile;              // bytes of a tile; a warp has two
+  bool vec_in, vec_out;  // see rows_in
 };
 
-template <typename T, int OP, int L>
+// A row's own values, loaded a step ahead of their use.
+struct RowValues {
+  long long a;
+  double adv, old, ref, w;  // ROW_POLICY
+  double m, rest, g, h;     // ROW_BACK
+};
+
+template <int OP, typename T>
+__device__ __forceinline__ RowValues load_row(const RowArgs<T>& A, long long r, bool there) {
+  RowValues v = {-1, 0.0, 0.0, 0.0, 1.0, 0.0, -1.0, 0.0, 0.0};
+  if (there) {
+    v.a = A.in.action(r);
+    if (OP == ROW_POLICY) {
+      v.adv = (double)A.pol.advantages[r];
+      v.old = (double)A.pol.old_logp[r];
+      if (A.pol.ref_logp) v.ref = (double)A.pol.ref_logp[r];
+      if (A.pol.weights) v.w = (double)A.pol.weights[r];
+    }
+    if (OP == ROW_BACK) {
+      v.m = (double)A.stats[2 * r];
+      v.rest = (double)A.stats[2 * r + 1];
+      v.g = (double)A.grad_logp[r];
+      if (A.hess_logp) v.h = (double)A.hess_logp[r];
+    }
+  }
+  return v;
+}
+
+// L lanes a row, P classes a lane: K <= L P.
+template <typename T, int OP, int L, int P>
 __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<T> A, const SmallLayout lay) {
   using C = typename Types<T>::C;
   using Row = typename Types<T>::Row;
   using Out = typename Types<T>::Out;
   constexpr int kRows = 32 / L;
   extern __shared__ __align__(16) unsigned char small_smem[];
-  __shared__ double two[32];
-  const ExpTable ex = {two};
-  if (sizeof(C) == 8) {
-    if (threadIdx.x < 32) two[threadIdx.x] = exp2(threadIdx.x / 32.0);
-    __syncthreads();
-  }
-  const int lane = threadIdx.x & 31, l = lane % L;
+  __shared__ double two[33];
+  ExpTable ex;
+  if (sizeof(C) == 8 || OP == ROW_POLICY) ex.fill(two);
+  const int lane = threadIdx.x & 31, l = lane % L, i = lane / L;  // this lane's row of a batch
   const int K = A.in.K;
-  unsigned char* tile = small_smem + (threadIdx.x >> 5) * lay.tile;
+  unsigned char* tile = small_smem + (threadIdx.x >> 5) * (2 * lay.tile);
+  int other = lay.tile;  // from this batch's tile to the next one's
   const TileRows in_rows(K * (int)sizeof(T)), out_rows(K * (int)sizeof(Out));
   const long long step = (long long)gridDim.x * (kSmallThreads / 32) * kRows;
-  for (long long base = ((long long)blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5)) * kRows; base < A.in.n;
-       base += step) {
-    const int rows = (int)min((long long)kRows, A.in.n - base);
-    copy_rows<true>(const_cast<T*>(A.in.scores) + base * A.in.stride, tile, in_rows, rows, K, A.in.stride, 1, lay.vec_in);
-    const int i = lane / L;  // this lane's row
-    const bool mine = i < rows;
+  long long base = ((long long)blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5)) * kRows;
+  auto rows_at = [&](long long b) { return (int)max(0ll, min((long long)kRows, A.in.n - b)); };
+  RowValues next = load_row<OP>(A, base + i, i < rows_at(base));
+  rows_in(A.in.scores + base * A.in.stride, tile, in_rows, rows_at(base), K, A.in.stride, lay.vec_in);
+  for (; base < A.in.n; base += step, tile += other, other = -other) {
+    const int rows = rows_at(base);
+    const bool mine = i < rows;  // the lanes of a missing row compute on what lies there, and store nothing
     const long long r = base + i;
-    long long a = -1;
-    double adv = 0.0, old = 0.0, ref = 0.0, w = 1.0, rest = -1.0;
-    RowDerivative row = {0.0, 0.0};
-    C m = 0;
-    if (mine) {
-      a = A.in.action(r);
-      if (OP == ROW_POLICY) {
-        adv = (double)A.pol.advantages[r];
-        old = (double)A.pol.old_logp[r];
-        if (A.pol.ref_logp) ref = (double)A.pol.ref_logp[r];
-        if (A.pol.weights) w = (double)A.pol.weights[r];
-      }
-      if (OP == ROW_BACK) {
-        m = A.stats[2 * r];
-        rest = (double)A.stats[2 * r + 1];
-        row.g = (double)A.grad_logp[r];
-        if (A.hess_logp) row.h = (double)A.hess_logp[r];
-      }
-    }
-    bool part = a >= 0 && w != 0.0 && (OP != ROW_BACK || rest != -1.0);
-    const bool bad = part && a >= K;
-    __syncwarp();
+    const RowValues now = next;
+    next = load_row<OP>(A, r + step, i < rows_at(base + step));
+    rows_in(A.in.scores + (base + step) * A.in.stride, tile + other, in_rows, rows_at(base + step), K, A.in.stride,
+            lay.vec_in);
+    copies_wait<1>();
     const T* z = reinterpret_cast<const T*>(tile + i * in_rows.stride);
-    const double za = (double)widen(part && !bad ? z[a] : z[0]);
-    C v[kSmallPer];
-    if (OP != ROW_BACK) {
-      C mx = -INFINITY;
+    RowDerivative row = {now.g, now.h};
+    C m = (C)now.m;
+    double rest = now.rest;
+    bool part = now.a >= 0 && now.w != 0.0 && (OP != ROW_BACK || rest != -1.0);
+    const bool bad = part && now.a >= K;
+    const int taken = part && !bad ? (int)now.a : 0;
+    const double za = (double)widen(z[taken]);
+    C v[P];
+    int top = -1;  // a class of this lane at the maximum
 #pragma unroll
-      for (int e = 0; e < kSmallPer; ++e) {
-        v[e] = -INFINITY;
-        if (e * L < K) {
-          if (l + e * L < K && mine) v[e] = widen(z[l + e * L]);
-          mx = max_nan(mx, v[e]);
-        }
+    for (int e = 0; e < P; ++e) v[e] = l + e * L < K ? (C)widen(z[l + e * L]) : (C)-INFINITY;
+    if (OP != ROW_BACK) {
+      C mx = v[0];
+#pragma unroll
+      for (int e = 1; e < P; ++e) mx = !(v[e] <= mx) ? v[e] : mx;  // may lose a NaN: the sum does not
+#pragma unroll
+      for (int k = L / 2; k > 0; k >>= 1) {
+        const C o = __shfl_xor_sync(0xffffffffu, mx, k);
+        mx = o > mx ? o : mx;
       }
 #pragma unroll
-      for (int k = L / 2; k > 0; k >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+      for (int e = 0; e < P; ++e) v[e] = ex(v[e] - mx);
       C sum = 0;
       int ties = 0;
 #pragma unroll
-      for (int e = 0; e < kSmallPer; ++e) {
-        if (e * L < K) {
-          v[e] = ex(v[e] - mx);
-          if (v[e] != (C)1) sum += v[e];
-          else ++ties;
-        }
+      for (int e = 0; e < P; ++e) {
+        const bool one = v[e] == (C)1;
+        sum += one ? (C)0 : v[e];
+        ties += one ? 1 : 0;
+        top = one ? l + e * L : top;
       }
 #pragma unroll
       for (int k = L / 2; k > 0; k >>= 1) {
         sum += __shfl_xor_sync(0xffffffffu, sum, k);
         ties += __shfl_xor_sync(0xffffffffu, ties, k);
       }
-      if (mx == (C)-INFINITY && !bad) part = false;
+      if (mx == (C)-INFINITY && part && !bad) {  // no class, unless a NaN hides among them
+        part = false;
+        for (int k = 0; k < K; ++k) part = part || widen(z[k]) != (C)-INFINITY;
+      }
+      m = 0;
       if (part) {
         m = mx;
         rest = (double)sum + (double)(ties - 1);
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < kSmallPer; ++e)
-        if (e * L < K) v[e] = l + e * L < K && mine ? ex((C)widen(z[l + e * L]) - m) : (C)0;
+      for (int e = 0; e < P; ++e) v[e] = ex(v[e] - m);
+#pragma unroll
+      for (int e = 0; e < P; ++e) top = v[e] == (C)1 ? l + e * L : top;
     }
 
     if (OP == ROW_LOGPROBS) {
@@ -513,10 +574,10 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
       double lp = 0.0, loss = 0.0;
       if (part && !bad) {
         lp = za - (double)m - log1p(rest);
-        part = za != -INFINITY;
+        part = za != -INFINITY;  // the class taken is masked
       }
       if (sizeof(C) == 4) {
-        const bool near = part && !bad && near_border(A.pol, lp - old, adv, border_slack(kSmallPer + 3, 4.9));
+        const bool near = part && !bad && near_border(A.pol, lp - now.old, now.adv, border_slack(P + 3, 4.9));
         if (__any_sync(0xffffffffu, near)) {
           double sum = 0.0;
           for (int k = l; k < K && near; k += L) sum += exp((double)widen(z[k]) - (double)m);
@@ -526,7 +587,8 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
         }
       }
       if (bad) lp = loss = NAN;
-      else if (part) row = policy_terms(A.pol, lp, adv, old, ref, w, &loss);
+      else if (part)
+        row = policy_terms(A.pol, lp, now.adv, now.old, now.ref, now.w, &loss, [&](double d) { return ex.scalar(d); });
       if (mine && l == 0) {
         if (A.pol.loss) A.pol.loss[r] = (Row)loss;
         if (A.pol.logp) A.pol.logp[r] = (Row)lp;
@@ -537,31 +599,47 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
       }
     }
     __syncwarp();  // the scores are used up: the derivatives take their place
-    const double inv_total = 1.0 / (1.0 + rest);
-    const C inv = (C)inv_total, left = (C)(rest * inv_total), g = (C)row.g, h = (C)row.h;
     const bool want_h = A.out.hess != nullptr;
     unsigned char* tile_h = tile + kRows * out_rows.stride;
-    if (mine) {
-      Out* to_g = reinterpret_cast<Out*>(tile + i * out_rows.stride);
-      Out* to_h = reinterpret_cast<Out*>(tile_h + i * out_rows.stride);
-      const bool plain = part && !bad;
-      const C fill = bad ? (C)NAN : (C)0;
+    Out* to_g = reinterpret_cast<Out*>(tile + i * out_rows.stride);
+    Out* to_h = reinterpret_cast<Out*>(tile_h + i * out_rows.stride);
+    const double inv_total = 1.0 / (1.0 + rest);
+    const C inv = (C)inv_total, share = (C)(rest * inv_total), g = (C)row.g, h = (C)row.h;
+    if (part && !bad) {
+      // every class as one that was not taken, and with 1 - p as it comes
+      const C down = -g * inv, ag = fabs(g), bend = h - ag;
 #pragma unroll
-      for (int e = 0; e < kSmallPer; ++e) {
-        const int k = l + e * L;
-        if (e * L < K && k < K) {
-          C dg, dh = 0;
-          derivative<C>(v[e], inv, left, k == (int)a, g, h, want_h, &dg, &dh);
-          narrow(plain ? dg : fill, to_g[k]);
-          if (want_h) narrow(plain ? dh : fill, to_h[k]);
+      for (int e = 0; e < P; ++e)
+        if (l + e * L < K) narrow(v[e] * down, to_g[l + e * L]);
+      if (want_h) {
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const C p = v[e] * inv;
+          if (l + e * L < K) narrow(p * fma(p, bend, ag), to_h[l + e * L]);
         }
+      }
+      // a class with more than half of the probability is alone at the
+      // maximum, and 1 - p is the others' share; then the class taken
+      const C pt = inv, lt = share;
+      if (want_h && inv > (C)0.5 && top >= 0) narrow(pt * (ag * lt + h * pt), to_h[top]);
+    }
+    __syncwarp();
+    if (l == 0 && part && !bad) {
+      const C e = ex((C)(za - (double)m)), p = e * inv, q = e == (C)1 ? share : (C)1 - p;
+      narrow(g * q, to_g[taken]);
+      if (want_h) narrow(q * (h * q + fabs(g) * p), to_h[taken]);
+    }
+    if (!part || bad) {
+      for (int k = l; k < K; k += L) {
+        narrow(bad ? (C)NAN : (C)0, to_g[k]);
+        if (want_h) narrow(bad ? (C)NAN : (C)0, to_h[k]);
       }
     }
     __syncwarp();
     const long long to = base * A.out.row_stride;
-    copy_rows<false>(A.out.grad + to, tile, out_rows, rows, K, A.out.row_stride, A.out.class_stride, lay.vec_out);
+    rows_out(A.out.grad + to, tile, out_rows, rows, K, A.out.row_stride, A.out.class_stride, lay.vec_out);
     if (want_h)
-      copy_rows<false>(A.out.hess + to, tile_h, out_rows, rows, K, A.out.row_stride, A.out.class_stride, lay.vec_out);
+      rows_out(A.out.hess + to, tile_h, out_rows, rows, K, A.out.row_stride, A.out.class_stride, lay.vec_out);
     __syncwarp();
   }
 }
@@ -575,7 +653,7 @@ int multiprocessors() {
   return n;
 }
 
-template <typename T, int OP, int L>
+template <typename T, int OP, int L, int P>
 void launch_small_t(const RowArgs<T>& A, cudaStream_t st) {
   using Out = typename Types<T>::Out;
   constexpr int rows = 32 / L, warps = kSmallThreads / 32;
@@ -589,17 +667,36 @@ void launch_small_t(const RowArgs<T>& A, cudaStream_t st) {
                 rows * out.bytes % 16 == 0;
   const long long blocks = (A.in.n + rows * warps - 1) / (rows * warps);
   const unsigned grid = (unsigned)std::min<long long>(blocks, 16ll * multiprocessors());
-  k_feedback_small<T, OP, L><<<grid, kSmallThreads, (size_t)lay.tile * warps, st>>>(A, lay);
+  k_feedback_small<T, OP, L, P><<<grid, kSmallThreads, (size_t)lay.tile * 2 * warps, st>>>(A, lay);
+}
+
+// Few classes fit one lane; a class too many in P costs a float64 exponential
+// a row (20 instructions of about 100 a class), a float32 one next to nothing.
+template <typename T, int OP>
+void launch_small(const RowArgs<T>& A, cudaStream_t st) {
+  const int K = A.in.K;
+  if (K > 64) return launch_small_t<T, OP, 8, 16>(A, st);
+  if (K > 32) return launch_small_t<T, OP, 4, 16>(A, st);
+  if (K > 16) return launch_small_t<T, OP, 2, 16>(A, st);
+  if constexpr (sizeof(T) == 8) {
+    if (K <= 2) return launch_small_t<T, OP, 1, 2>(A, st);
+    if (K <= 4) return launch_small_t<T, OP, 1, 4>(A, st);
+    if (K <= 6) return launch_small_t<T, OP, 1, 6>(A, st);
+    if (K <= 8) return launch_small_t<T, OP, 1, 8>(A, st);
+    if (K <= 10) return launch_small_t<T, OP, 1, 10>(A, st);
+    if (K <= 12) return launch_small_t<T, OP, 1, 12>(A, st);
+  } else if constexpr (sizeof(T) == 4) {
+    if (K <= 4) return launch_small_t<T, OP, 1, 4>(A, st);
+    if (K <= 8) return launch_small_t<T, OP, 1, 8>(A, st);
+  }
+  launch_small_t<T, OP, 1, 16>(A, st);
 }
 
 template <typename T, int OP>
 void launch_rows_t(const RowArgs<T>& A, cudaStream_t st) {
   if (A.in.n == 0) return;
   if (A.in.K <= kSmallClasses) {
-    if (A.in.K <= kSmallPer) launch_small_t<T, OP, 1>(A, st);
-    else if (A.in.K <= 2 * kSmallPer) launch_small_t<T, OP, 2>(A, st);
-    else if (A.in.K <= 4 * kSmallPer) launch_small_t<T, OP, 4>(A, st);
-    else launch_small_t<T, OP, 8>(A, st);
+    launch_small<T, OP>(A, st);
     MTB_CUDA_FB(cudaGetLastError());
     return;
   }
