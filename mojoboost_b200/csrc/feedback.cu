@@ -306,37 +306,73 @@ constexpr int kSmallThreads = 128;
 constexpr int kSmallPer = 16;  // classes a lane
 constexpr int kSmallClasses = 8 * kSmallPer;
 
-// exp(d) in float64 by table and polynomial (P. T. P. Tang, "Table-driven
-// implementation of the exponential function in IEEE floating-point
-// arithmetic", ACM TOMS 15(2), 1989): d = (n / 32) ln 2 + r, exp(d) =
-// 2^(n / 32) (1 + r + ... + r^6 / 720), the truncation below 2^-57 for |r| <=
-// ln 2 / 64.  NaN stays; below -708 (3e-308) the value is 0.
-struct ExpTable {
-  const double* two;  // shared memory: 2^(j / 32) for j < 32, then 0
-  __device__ __forceinline__ double operator()(double d) const {  // d <= 709.78
+// exp and log1p in float64 by tables in shared memory and polynomials (P. T. P.
+// Tang, "Table-driven implementation of the exponential function in IEEE
+// floating-point arithmetic", ACM TOMS 15(2), 1989, and "... of the logarithm
+// function ...", ACM TOMS 16(4), 1990): both without a branch, so that the
+// work of a lane's classes overlaps.
+struct MathTables {
+  double two[65];     // 2^(j / 64) for j < 64, then 0
+  double inv_c[64];   // 1 / c, c = 1 + j / 64
+  double log_c[64];
+};
+
+struct TableMath {
+  MathTables* t;
+  // The whole block calls it.
+  __device__ __forceinline__ explicit TableMath(MathTables& tables) : t(&tables) {
+    for (int j = threadIdx.x; j < 65; j += blockDim.x) t->two[j] = j < 64 ? exp2(j / 64.0) : 0.0;
+    for (int j = threadIdx.x; j < 64; j += blockDim.x) {
+      t->inv_c[j] = 64.0 / (64 + j);
+      t->log_c[j] = log(1.0 + j / 64.0);
+    }
+    __syncthreads();
+  }
+  // exp(d), d <= 709.78: d = (n / 64) ln 2 + r, exp(d) = 2^(n / 64) (1 + r +
+  // ... + r^5 / 120), |r| <= ln 2 / 128, truncation below 2^-54.  NaN stays;
+  // below -708 (3e-308) the value is 0.
+  __device__ __forceinline__ double exp(double d) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
     const bool none = d < -708.0;
     d = __hiloint2double(none ? 0 : __double2hiint(d), __double2loint(d));
-    const double t = fma(d, 46.166241308446828, kRound);
-    const int n = __double2loint(t);
-    const double k = t - kRound;
-    double r = fma(k, -2.1660849392498290e-2, d);  // ln 2 / 32, and its rounding error
-    r = fma(k, -7.2470212932696861e-19, r);
-    double q = fma(r, 1.0 / 720.0, 1.0 / 120.0);
-    q = fma(q, r, 1.0 / 24.0);
+    const double k0 = fma(d, 92.332482616893656, kRound);
+    const int n = __double2loint(k0);
+    const double k = k0 - kRound;
+    double r = fma(k, -1.0830424696249145e-2, d);  // ln 2 / 64, and its rounding error
+    r = fma(k, -3.6235106466348430e-19, r);
+    double q = fma(r, 1.0 / 120.0, 1.0 / 24.0);
     q = fma(q, r, 1.0 / 6.0);
     q = fma(q, r, 0.5);
     q = fma(q, r * r, r);
-    const double two_n = two[none ? 32 : n & 31];
-    const double scaled = __hiloint2double(__double2hiint(two_n) + (n >> 5 << 20), __double2loint(two_n));
+    const double two_n = t->two[none ? 64 : n & 63];
+    const double scaled = __hiloint2double(__double2hiint(two_n) + (n >> 6 << 20), __double2loint(two_n));
     return fma(scaled, q, scaled);
   }
-  __device__ __forceinline__ float operator()(float d) const { return __expf(d); }
-  __device__ __forceinline__ double scalar(double d) const { return d > 709.78 ? INFINITY : (*this)(d); }
-  __device__ __forceinline__ void fill(double* to) {
-    if (threadIdx.x < 33) to[threadIdx.x] = threadIdx.x < 32 ? exp2(threadIdx.x / 32.0) : 0.0;
-    __syncthreads();
-    two = to;
+  __device__ __forceinline__ float exp(float d) const { return __expf(d); }
+  __device__ __forceinline__ double operator()(double d) const { return d > 709.78 ? INFINITY : exp(d); }
+  // log(1 + x), 0 <= x < 2^1000: 1 + x = 2^e c (1 + f), c the multiple of 1/64
+  // next to its significand, |f| <= 1 / 128; f - f^2 / 2 + ... - f^8 / 8,
+  // truncation below 2^-59.  Next to 1, f is x itself.
+  __device__ __forceinline__ double log1p(double x) const {
+    const double s = 1.0 + x;
+    const int hi = __double2hiint(s) + 0x2000;
+    const int j = hi >> 14 & 63, e = (hi >> 20) - 1023;
+    const double c = __hiloint2double(hi & ~0x3fff, 0);
+    const double inv = t->inv_c[j];
+    const double f = c == 1.0 ? x : (s - c) * __hiloint2double(__double2hiint(inv) - (e << 20), __double2loint(inv));
+    double q = fma(f, -1.0 / 8.0, 1.0 / 7.0);
+    q = fma(q, f, -1.0 / 6.0);
+    q = fma(q, f, 1.0 / 5.0);
+    q = fma(q, f, -1.0 / 4.0);
+    q = fma(q, f, 1.0 / 3.0);
+    q = fma(q, f, -1.0 / 2.0);
+    return fma((double)e, 0.6931471805599453, t->log_c[j]) + fma(q, f * f, f);
+  }
+  // 1 / s for 1 <= s < 2^100, by Newton's iteration from a float32 quotient.
+  __device__ __forceinline__ static double inverse(double s) {
+    double r = (double)__fdividef(1.0f, (float)s);
+    r = fma(r, fma(-s, r, 1.0), r);
+    return fma(r, fma(-s, r, 1.0), r);
   }
 };
 
@@ -364,30 +400,43 @@ struct RowWalk {
   }
 };
 
-// Asynchronous copy of 16 bytes to shared memory, past L1 and the registers.
-__device__ __forceinline__ void copy_async16(void* shared, const void* global) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(shared)),
-               "l"(global)
+// Bulk copies between global and shared memory, of multiples of 16 bytes that
+// start on 16 bytes; those to shared memory count down a barrier.
+__device__ __forceinline__ unsigned shared_address(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void bulk_in(void* shared, const void* global, int bytes, unsigned long long* barrier) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   shared_address(shared)),
+               "l"(global), "r"(bytes), "r"(shared_address(barrier))
+               : "memory");
+}
+
+__device__ __forceinline__ void bulk_out(void* global, const void* shared, int bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(global), "r"(shared_address(shared)),
+               "r"(bytes)
                : "memory");
 }
 
 // Starts the copy of `rows` rows of K elements, row_stride apart, into shared
-// memory; copies_wait ends it.  The whole warp calls both.  vec: the rows are
-// one piece of global memory that starts on 16 bytes.
+// memory; rows_wait ends it.  The whole warp calls both.  vec: the rows are
+// one piece of global memory that starts on 16 bytes, copied whole, or row by
+// row where they lie apart in shared memory.
 template <typename E>
 __device__ __forceinline__ void rows_in(const E* global, unsigned char* tile, TileRows R, int rows, int K,
-                                        long long row_stride, bool vec) {
+                                        long long row_stride, bool vec, unsigned long long* barrier) {
   const int lane = threadIdx.x & 31;
   if (vec) {
-    const int total = rows * R.bytes;
-    const unsigned char* from = reinterpret_cast<const unsigned char*>(global);
+    const int bytes = rows * R.bytes & ~15;
+    if (lane == 0)
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(barrier)), "r"(bytes)
+                   : "memory");
+    __syncwarp();
     if (R.stride != R.bytes) {
-      RowWalk at(lane, R.bytes / 16);
-      for (int c = lane * 16; c < total; c += 512, at.next()) copy_async16(tile + at.row * R.stride + at.col * 16, from + c);
+      if (lane < rows) bulk_in(tile + lane * R.stride, reinterpret_cast<const char*>(global) + lane * R.bytes, R.bytes, barrier);
     } else {
-      for (int c = lane * 16; c + 16 <= total; c += 512) copy_async16(tile + c, from + c);
-      for (int j = total / 16 * 16 / (int)sizeof(E) + lane; j < total / (int)sizeof(E); j += 32)
-        reinterpret_cast<E*>(tile)[j] = global[j];
+      if (lane == 0 && bytes) bulk_in(tile, global, bytes, barrier);
+      const int j = bytes / (int)sizeof(E) + lane;  // fewer than 16 bytes are left
+      if (j < rows * K) reinterpret_cast<E*>(tile)[j] = global[j];
     }
   } else {
     RowWalk at(lane, K);
@@ -407,33 +456,36 @@ __device__ __forceinline__ void rows_in(const E* global, unsigned char* tile, Ti
         if (to[q]) *to[q] = x[q];
     }
   }
-  asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
-template <int LATER>  // how many copies started after the one waited for may still run
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory");
+// False when the copies did not end within the limit (about a second).
+__device__ __forceinline__ bool rows_wait(bool vec, unsigned long long* barrier, unsigned phase) {
+  unsigned done = vec ? 0 : 1;
+  for (int i = 0; i < 1 << 20 && !done; ++i)
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(shared_address(barrier)), "r"(phase)
+        : "memory");
   __syncwarp();
+  return done != 0;
 }
 
 // Rows from shared memory to global memory, elements row_stride and
-// class_stride apart; vec as above.
+// class_stride apart; vec as above.  The whole warp calls it, after writing
+// the rows; out_wait before they are overwritten.
 template <typename E>
 __device__ __forceinline__ void rows_out(E* global, const unsigned char* tile, TileRows R, int rows, int K,
                                          long long row_stride, long long class_stride, bool vec) {
   const int lane = threadIdx.x & 31;
   if (vec) {
-    const int total = rows * R.bytes;
-    unsigned char* to = reinterpret_cast<unsigned char*>(global);
+    const int bytes = rows * R.bytes & ~15;
     if (R.stride != R.bytes) {
-      RowWalk at(lane, R.bytes / 16);
-      for (int c = lane * 16; c < total; c += 512, at.next())
-        *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(tile + at.row * R.stride + at.col * 16);
+      if (lane < rows) bulk_out(reinterpret_cast<char*>(global) + lane * R.bytes, tile + lane * R.stride, R.bytes);
     } else {
-      for (int c = lane * 16; c + 16 <= total; c += 512)
-        *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(tile + c);
-      for (int j = total / 16 * 16 / (int)sizeof(E) + lane; j < total / (int)sizeof(E); j += 32)
-        global[j] = reinterpret_cast<const E*>(tile)[j];
+      if (lane == 0 && bytes) bulk_out(global, tile, bytes);
+      const int j = bytes / (int)sizeof(E) + lane;
+      if (j < rows * K) global[j] = reinterpret_cast<const E*>(tile)[j];
     }
   } else if (class_stride == 1) {
     for (RowWalk at(lane, K); at.row < rows; at.next())
@@ -443,6 +495,9 @@ __device__ __forceinline__ void rows_out(E* global, const unsigned char* tile, T
       global[at.col * row_stride + at.row * class_stride] = reinterpret_cast<const E*>(tile + at.col * R.stride)[at.row];
   }
 }
+
+// Ends the reads of this lane's copies out of shared memory.
+__device__ __forceinline__ void out_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
 struct SmallLayout {
   int tile;              // bytes of a tile; a warp has two
@@ -484,10 +539,15 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
   using Row = typename Types<T>::Row;
   using Out = typename Types<T>::Out;
   constexpr int kRows = 32 / L;
+  // In float64 a sum that holds the 1 of the largest class gives the others'
+  // to 2^-43 of it unless it is below 2^-10, far beyond what the float32
+  // derivatives keep; the statistics keep it whole.
+  constexpr bool kExact = sizeof(C) == 4 || OP == ROW_LOGPROBS;
+  constexpr double kNearOne = 0x1p-10;
   extern __shared__ __align__(16) unsigned char small_smem[];
-  __shared__ double two[33];
-  ExpTable ex;
-  if (sizeof(C) == 8 || OP == ROW_POLICY) ex.fill(two);
+  __shared__ MathTables tables;
+  __shared__ __align__(8) unsigned long long barriers[kSmallThreads / 32][2];
+  const TableMath math(tables);
   const int lane = threadIdx.x & 31, l = lane % L, i = lane / L;  // this lane's row of a batch
   const int K = A.in.K;
   unsigned char* tile = small_smem + (threadIdx.x >> 5) * (2 * lay.tile);
@@ -496,23 +556,30 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
   const long long step = (long long)gridDim.x * (kSmallThreads / 32) * kRows;
   long long base = ((long long)blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5)) * kRows;
   auto rows_at = [&](long long b) { return (int)max(0ll, min((long long)kRows, A.in.n - b)); };
+  // a barrier per tile; the warp waits for tile q of its barrier in phase q mod 2
+  unsigned long long* barrier = barriers[threadIdx.x >> 5];
+  if (lane < 2)
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(barrier + lane)) : "memory");
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
   RowValues next = load_row<OP>(A, base + i, i < rows_at(base));
-  rows_in(A.in.scores + base * A.in.stride, tile, in_rows, rows_at(base), K, A.in.stride, lay.vec_in);
-  for (; base < A.in.n; base += step, tile += other, other = -other) {
+  if (base < A.in.n)
+    rows_in(A.in.scores + base * A.in.stride, tile, in_rows, rows_at(base), K, A.in.stride, lay.vec_in, barrier);
+  unsigned turn = 0;  // bit 0: the tile's barrier, bit 1: its phase
+  for (; base < A.in.n; base += step, tile += other, other = -other, turn = (turn + 1) & 3) {
     const int rows = rows_at(base);
     const bool mine = i < rows;  // the lanes of a missing row compute on what lies there, and store nothing
     const long long r = base + i;
     const RowValues now = next;
     next = load_row<OP>(A, r + step, i < rows_at(base + step));
-    rows_in(A.in.scores + (base + step) * A.in.stride, tile + other, in_rows, rows_at(base + step), K, A.in.stride,
-            lay.vec_in);
-    copies_wait<1>();
+    const bool arrived = rows_wait(lay.vec_in, barrier + (turn & 1), turn >> 1);
     const T* z = reinterpret_cast<const T*>(tile + i * in_rows.stride);
     RowDerivative row = {now.g, now.h};
     C m = (C)now.m;
     double rest = now.rest;
     bool part = now.a >= 0 && now.w != 0.0 && (OP != ROW_BACK || rest != -1.0);
-    const bool bad = part && now.a >= K;
+    const bool bad = part && (now.a >= K || !arrived);
     const int taken = part && !bad ? (int)now.a : 0;
     const double za = (double)widen(z[taken]);
     C v[P];
@@ -529,20 +596,35 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
         mx = o > mx ? o : mx;
       }
 #pragma unroll
-      for (int e = 0; e < P; ++e) v[e] = ex(v[e] - mx);
-      C sum = 0;
-      int ties = 0;
+      for (int e = 0; e < P; ++e) v[e] = math.exp(v[e] - mx);
+      // the sum less the 1 of one class at the maximum
+      double others = 0.0;
+      bool exact = kExact;  // a matter of this row alone, whatever the warp's others are
+      if (!kExact) {
+        C sum = v[0];
 #pragma unroll
-      for (int e = 0; e < P; ++e) {
-        const bool one = v[e] == (C)1;
-        sum += one ? (C)0 : v[e];
-        ties += one ? 1 : 0;
-        top = one ? l + e * L : top;
+        for (int e = 1; e < P; ++e) sum += v[e];
+#pragma unroll
+        for (int k = L / 2; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        others = (double)sum - 1.0;
+        exact = others < kNearOne;
       }
+      if (kExact || __any_sync(0xffffffffu, exact)) {
+        C sum = 0;
+        int ties = 0;
 #pragma unroll
-      for (int k = L / 2; k > 0; k >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, k);
-        ties += __shfl_xor_sync(0xffffffffu, ties, k);
+        for (int e = 0; e < P; ++e) {
+          const bool one = v[e] == (C)1;
+          sum += one ? (C)0 : v[e];
+          ties += one ? 1 : 0;
+          top = one && exact ? l + e * L : top;
+        }
+#pragma unroll
+        for (int k = L / 2; k > 0; k >>= 1) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, k);
+          ties += __shfl_xor_sync(0xffffffffu, ties, k);
+        }
+        if (exact) others = (double)sum + (double)(ties - 1);
       }
       if (mx == (C)-INFINITY && part && !bad) {  // no class, unless a NaN hides among them
         part = false;
@@ -551,18 +633,25 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
       m = 0;
       if (part) {
         m = mx;
-        rest = (double)sum + (double)(ties - 1);
+        rest = others;
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < P; ++e) v[e] = ex(v[e] - m);
+      for (int e = 0; e < P; ++e) v[e] = math.exp(v[e] - m);
+      const bool exact = kExact || rest < kNearOne;
 #pragma unroll
-      for (int e = 0; e < P; ++e) top = v[e] == (C)1 ? l + e * L : top;
+      for (int e = 0; e < P; ++e) top = v[e] == (C)1 && exact ? l + e * L : top;
     }
+    // the next rows into the other tile, whose derivatives are on their way by now
+    out_wait();
+    __syncwarp();
+    if (base + step < A.in.n)
+      rows_in(A.in.scores + (base + step) * A.in.stride, tile + other, in_rows, rows_at(base + step), K, A.in.stride,
+              lay.vec_in, barrier + (turn + 1 & 1));
 
     if (OP == ROW_LOGPROBS) {
       if (mine && l == 0) {
-        const double lp = part && !bad ? za - (double)m - log1p(rest) : 0.0;
+        const double lp = part && !bad ? za - (double)m - math.log1p(rest) : 0.0;
         A.logp[r] = bad ? (Row)NAN : (Row)lp;
         A.stats[2 * r] = bad ? (Row)NAN : (Row)m;
         A.stats[2 * r + 1] = bad ? (Row)NAN : part ? (Row)rest : (Row)-1;
@@ -573,7 +662,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
     if (OP == ROW_POLICY) {
       double lp = 0.0, loss = 0.0;
       if (part && !bad) {
-        lp = za - (double)m - log1p(rest);
+        lp = za - (double)m - math.log1p(rest);
         part = za != -INFINITY;  // the class taken is masked
       }
       if (sizeof(C) == 4) {
@@ -588,7 +677,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
       }
       if (bad) lp = loss = NAN;
       else if (part)
-        row = policy_terms(A.pol, lp, now.adv, now.old, now.ref, now.w, &loss, [&](double d) { return ex.scalar(d); });
+        row = policy_terms(A.pol, lp, now.adv, now.old, now.ref, now.w, &loss, math);
       if (mine && l == 0) {
         if (A.pol.loss) A.pol.loss[r] = (Row)loss;
         if (A.pol.logp) A.pol.logp[r] = (Row)lp;
@@ -603,7 +692,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
     unsigned char* tile_h = tile + kRows * out_rows.stride;
     Out* to_g = reinterpret_cast<Out*>(tile + i * out_rows.stride);
     Out* to_h = reinterpret_cast<Out*>(tile_h + i * out_rows.stride);
-    const double inv_total = 1.0 / (1.0 + rest);
+    const double inv_total = TableMath::inverse(1.0 + rest);
     const C inv = (C)inv_total, share = (C)(rest * inv_total), g = (C)row.g, h = (C)row.h;
     if (part && !bad) {
       // every class as one that was not taken, and with 1 - p as it comes
@@ -625,7 +714,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
     }
     __syncwarp();
     if (l == 0 && part && !bad) {
-      const C e = ex((C)(za - (double)m)), p = e * inv, q = e == (C)1 ? share : (C)1 - p;
+      const C e = math.exp((C)(za - (double)m)), p = e * inv, q = e == (C)1 ? share : (C)1 - p;
       narrow(g * q, to_g[taken]);
       if (want_h) narrow(q * (h * q + fabs(g) * p), to_h[taken]);
     }
@@ -635,13 +724,16 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
         if (want_h) narrow(bad ? (C)NAN : (C)0, to_h[k]);
       }
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     const long long to = base * A.out.row_stride;
     rows_out(A.out.grad + to, tile, out_rows, rows, K, A.out.row_stride, A.out.class_stride, lay.vec_out);
     if (want_h)
       rows_out(A.out.hess + to, tile_h, out_rows, rows, K, A.out.row_stride, A.out.class_stride, lay.vec_out);
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     __syncwarp();
   }
+  out_wait();
 }
 
 inline bool on16(const void* p) { return (uintptr_t)p % 16 == 0; }
