@@ -15,6 +15,7 @@
 // of n_classes or more gives NaN in that row.
 #include "feedback.h"
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -23,6 +24,7 @@
 #include <memory>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "../../include/mojotrees.h"
 #include "capi_util.h"
@@ -784,6 +786,444 @@ void launch_small(const RowArgs<T>& A, cudaStream_t st) {
   launch_small_t<T, OP, 1, 16>(A, st);
 }
 
+// ---------------------------------------------------------------------------
+// Rows of more than 128 classes, scores of 32 and 16 bits
+//
+// A block (or a cluster of up to 8 of them, where a row is longer than 4096
+// vectors of 16 bytes, or rows are too few to fill the GPU) holds a row in its
+// registers: the scores are read once, and the bound is the memory system,
+// or for 16-bit scores the exponentials, two a class (the sum's, and the
+// gradient's again: kept in float32 they would take twice the registers).
+// Each warp sums relative to its own maximum, so one barrier joins maxima and
+// sums; the next row is fetched into L2 meanwhile.
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ float max_nan32(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Two float32 values in one register pair, with the paired instructions.
+struct Pair {
+  unsigned long long v;
+  __device__ __forceinline__ static Pair of(float x, float y) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(x), "f"(y));
+    return p;
+  }
+  __device__ __forceinline__ float2 get() const {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+  }
+  __device__ __forceinline__ Pair operator+(Pair o) const {
+    Pair p;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(v), "l"(o.v));
+    return p;
+  }
+  __device__ __forceinline__ Pair operator*(Pair o) const {
+    Pair p;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(v), "l"(o.v));
+    return p;
+  }
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ __half low_of(__half2 x) { return __low2half(x); }
+__device__ __forceinline__ __half high_of(__half2 x) { return __high2half(x); }
+__device__ __forceinline__ __nv_bfloat16 low_of(__nv_bfloat162 x) { return __low2bfloat16(x); }
+__device__ __forceinline__ __nv_bfloat16 high_of(__nv_bfloat162 x) { return __high2bfloat16(x); }
+
+// 16 bytes of scores.
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  uint4 raw;
+  __device__ __forceinline__ unsigned word(int i) const { return i == 0 ? raw.x : i == 1 ? raw.y : i == 2 ? raw.z : raw.w; }
+  __device__ __forceinline__ Pair pair(int i) const {  // elements 2 i, 2 i + 1
+    if constexpr (sizeof(T) == 4) {
+      return Pair::of(__uint_as_float(word(2 * i)), __uint_as_float(word(2 * i + 1)));
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return Pair::of(__uint_as_float(word(i) << 16), __uint_as_float(word(i) & 0xffff0000u));
+    } else {
+      const unsigned w = word(i);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+      return Pair::of(f.x, f.y);
+    }
+  }
+  __device__ __forceinline__ float max() const {  // NaN when one is
+    if constexpr (sizeof(T) == 4) {
+      return max_nan32(max_nan32(__uint_as_float(raw.x), __uint_as_float(raw.y)),
+                       max_nan32(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const T2* w = reinterpret_cast<const T2*>(&raw);
+      const T2 x = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
+      return max_nan32(widen(low_of(x)), widen(high_of(x)));
+    }
+  }
+  // Hides the value's history, so that what an earlier pass made of it is not
+  // kept in registers for a later one.
+  __device__ __forceinline__ void forget() {
+    asm volatile("" : "+r"(raw.x), "+r"(raw.y), "+r"(raw.z), "+r"(raw.w));
+  }
+  __device__ __forceinline__ static Vec lowest() {  // every element -inf
+    const unsigned w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __nv_bfloat16>::value ? 0xff80ff80u : 0xfc00fc00u;
+    return {make_uint4(w, w, w, w)};
+  }
+};
+
+// The elements [first, first + N) of a row that has elements [0, K): whole
+// where they all exist, else one by one, the others -inf.
+template <typename T>
+__device__ __forceinline__ Vec<T> load_vec(const T* row, int first, int K) {
+  constexpr int N = Vec<T>::N;
+  Vec<T> v;
+  if (first >= 0 && first + N <= K) {
+    v.raw = *reinterpret_cast<const uint4*>(row + first);
+  } else {
+    v = Vec<T>::lowest();
+    T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (first + j >= 0 && first + j < K) e[j] = row[first + j];
+  }
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(T* row, int first, int K, bool whole, const T (&e)[Vec<T>::N]) {
+  constexpr int N = Vec<T>::N;
+  if (whole && first >= 0 && first + N <= K) {
+    *reinterpret_cast<uint4*>(row + first) = *reinterpret_cast<const uint4*>(e);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (first + j >= 0 && first + j < K) row[first + j] = e[j];
+  }
+}
+
+// A part of a row: its maximum, and the sum of exp(z - maximum).
+struct Part {
+  double sum;
+  float m;
+  int ones;  // later: how many terms of 1 the sum leaves out
+};
+
+template <int THREADS>
+struct LargeShared {
+  MathTables tables;
+  Part warp[2][THREADS / 32], slow[2][THREADS / 32];  // by the parity of the row, as all here
+  Part block[2], slow_block[2];                       // read by the cluster
+  double near_sum[2][THREADS / 32], near_block[2];
+  float g, h;
+  int near;
+};
+
+// The parts of lanes below n joined: a maximum and a sum relative to it.
+__device__ __forceinline__ Part join_parts(Part p, int n, const TableMath& math) {
+  const bool there = (int)(threadIdx.x & 31) < n;
+  float m = there ? p.m : -INFINITY;
+  for (int k = 16; k > 0; k >>= 1) m = max_nan32(m, __shfl_xor_sync(0xffffffffu, m, k));
+  double s = there && p.m != -INFINITY ? p.sum * math.exp((double)p.m - (double)m) : 0.0;
+  for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+  return {s, m, 0};
+}
+
+// Sums of parts relative to one maximum.
+__device__ __forceinline__ Part add_parts(Part p, int n) {
+  if ((int)(threadIdx.x & 31) >= n) p.sum = 0.0, p.ones = 0;
+  for (int k = 16; k > 0; k >>= 1) {
+    p.sum += __shfl_xor_sync(0xffffffffu, p.sum, k);
+    p.ones += __shfl_xor_sync(0xffffffffu, p.ones, k);
+  }
+  return p;
+}
+
+template <typename T, int OP, int THREADS, int NV>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(const RowArgs<T> A) {
+  namespace cg = cooperative_groups;
+  using Row = typename Types<T>::Row;
+  constexpr int N = Vec<T>::N, kWarps = THREADS / 32;
+  constexpr float kLog2e = 1.4426950408889634f;
+  __shared__ LargeShared<THREADS> S;
+  const TableMath math(S.tables);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int K = A.in.K;
+  const long long clusters = gridDim.x / blocks;
+  int parity = 0;
+  for (long long r = blockIdx.x / blocks; r < A.in.n; r += clusters) {
+    const T* z = A.in.scores + r * A.in.stride;
+    const int lead = (int)((uintptr_t)z / sizeof(T) % N);  // elements from a 16-byte border to the row's first
+    const int vecs = (lead + K + N - 1) / N, per = (vecs + blocks - 1) / blocks;
+    const int v0 = min(vecs, rank * per), v1 = min(vecs, v0 + per);
+    const long long a = A.in.action(r);
+    const bool bad = a >= K;
+    bool part = a >= 0;
+    if (OP == ROW_POLICY && A.pol.weights) part = part && A.pol.weights[r] != (Row)0;
+    double rest = -1.0;
+    float m = 0.0f;
+    if (OP == ROW_BACK) {
+      m = A.stats[2 * r];
+      rest = (double)A.stats[2 * r + 1];
+      part = part && rest != -1.0;
+    }
+    bool live = part && !bad;
+    Vec<T> v[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int at = v0 + threadIdx.x + j * THREADS;
+      v[j] = live && at < v1 ? load_vec(z, at * N - lead, K) : Vec<T>::lowest();
+    }
+    if (threadIdx.x == 0 && r + clusters < A.in.n) {  // this block's part of its next row, the whole vectors of it
+      const T* zn = z + clusters * A.in.stride;
+      const int ln = (int)((uintptr_t)zn / sizeof(T) % N);
+      const int b = max(v0 * N - ln, ln ? N - ln : 0), e = min(v1 * N - ln, (K + ln) / N * N - ln);
+      if (b < e)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(zn + b), "r"((e - b) * (int)sizeof(T)) : "memory");
+    }
+    float za = 0.0f, adv = 0.0f, old = 0.0f, ref = 0.0f, w = 1.0f;
+    if (live) {
+      za = widen(z[a]);
+      if (OP == ROW_POLICY && warp == 0) {
+        adv = A.pol.advantages[r];
+        old = A.pol.old_logp[r];
+        if (A.pol.ref_logp) ref = A.pol.ref_logp[r];
+        if (A.pol.weights) w = A.pol.weights[r];
+      }
+    }
+
+    if (OP != ROW_BACK && live) {
+      parity ^= 1;
+      // the warp's maximum, and its sum relative to it
+      float wm = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        wm = max_nan32(wm, v[j].max());
+        v[j].forget();
+      }
+      for (int k = 16; k > 0; k >>= 1) wm = max_nan32(wm, __shfl_xor_sync(0xffffffffu, wm, k));
+      Part p = {0.0, wm, 0};
+      if (wm != -INFINITY) {
+        const Pair less = Pair::of(-wm, -wm), scale = Pair::of(kLog2e, kLog2e);
+        Pair sum = Pair::of(0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < N / 2; ++i) {
+            const float2 d = ((v[j].pair(i) + less) * scale).get();
+            sum = sum + Pair::of(exp2_approx(d.x), exp2_approx(d.y));
+            if (i == N / 2 - 1) v[j].forget();
+          }
+        float s = sum.get().x + sum.get().y;
+        for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+        p.sum = (double)s;
+      }
+      if (lane == 0) S.warp[parity][warp] = p;
+      __syncthreads();
+      Part all = join_parts(S.warp[parity][lane < kWarps ? lane : 0], kWarps, math);
+      if (blocks > 1) {
+        if (threadIdx.x == 0) S.block[parity] = all;
+        cluster.sync();
+        all = join_parts(*cluster.map_shared_rank(&S.block[parity], lane < blocks ? lane : 0), blocks, math);
+      }
+      if (all.m == -INFINITY) {
+        live = part = false;
+      } else {
+        m = all.m;
+        rest = all.sum - 1.0;
+        if (rest < 1.0) {
+          // One class has more than half, and its 1 took the last bits of the
+          // others: the sum without the terms of 1, of the warps that have any.
+          if (wm == m) {
+            float s = 0.0f;
+            int ones = 0;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+              for (int i = 0; i < N / 2; ++i) {
+                const float2 f = v[j].pair(i).get();
+                const float x = exp2_approx((f.x - m) * kLog2e), y = exp2_approx((f.y - m) * kLog2e);
+                s += (x == 1.0f ? 0.0f : x) + (y == 1.0f ? 0.0f : y);
+                ones += (x == 1.0f ? 1 : 0) + (y == 1.0f ? 1 : 0);
+                if (i == N / 2 - 1) v[j].forget();
+              }
+            for (int k = 16; k > 0; k >>= 1) {
+              s += __shfl_xor_sync(0xffffffffu, s, k);
+              ones += __shfl_xor_sync(0xffffffffu, ones, k);
+            }
+            p = {(double)s, m, ones};
+          } else if (wm != -INFINITY) {
+            p.sum *= math.exp((double)wm - (double)m);
+          }
+          if (lane == 0) S.slow[parity][warp] = p;
+          __syncthreads();
+          p = add_parts(S.slow[parity][lane < kWarps ? lane : 0], kWarps);
+          if (blocks > 1) {
+            if (threadIdx.x == 0) S.slow_block[parity] = p;
+            cluster.sync();
+            p = add_parts(*cluster.map_shared_rank(&S.slow_block[parity], lane < blocks ? lane : 0), blocks);
+          }
+          rest = p.sum + (double)(p.ones - 1);
+        }
+      }
+    }
+
+    float g = 0.0f, h = 0.0f;
+    if (OP == ROW_LOGPROBS) {
+      if (threadIdx.x == 0 && rank == 0) {
+        const bool nan = part && bad;
+        A.logp[r] = nan ? NAN : live ? (Row)((double)za - (double)m - math.log1p(rest)) : (Row)0;
+        A.stats[2 * r] = nan ? NAN : live ? m : 0.0f;
+        A.stats[2 * r + 1] = nan ? NAN : live ? (Row)rest : (Row)-1;
+      }
+      continue;
+    } else if (OP == ROW_BACK) {
+      if (live) {
+        g = A.grad_logp[r];
+        if (A.hess_logp) h = A.hess_logp[r];
+      }
+    } else {
+      double lp = 0.0;
+      if (live) {
+        lp = (double)za - (double)m - math.log1p(rest);
+        live = part = za != -INFINITY;  // the class taken is masked
+      }
+      if (live) {
+        if (threadIdx.x == 0)
+          S.near = near_border(A.pol, lp - (double)old, (double)adv, border_slack(NV * N / 2 + 7, 12.5)) ? 1 : 0;
+        __syncthreads();
+        if (S.near) {
+          double sum = 0.0;
+          for (int k = max(v0 * N - lead, 0) + threadIdx.x; k < min(v1 * N - lead, K); k += THREADS)
+            sum += math.exp((double)widen(z[k]) - (double)m);
+          for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+          if (lane == 0) S.near_sum[parity][warp] = sum;
+          __syncthreads();
+          sum = 0.0;
+          for (int i = 0; i < kWarps; ++i) sum += S.near_sum[parity][i];
+          if (blocks > 1) {
+            if (threadIdx.x == 0) S.near_block[parity] = sum;
+            cluster.sync();
+            sum = 0.0;
+            for (int i = 0; i < blocks; ++i) sum += *cluster.map_shared_rank(&S.near_block[parity], i);
+          }
+          lp = (double)za - (double)m - log(sum);
+        }
+      }
+      if (warp == 0) {
+        double loss = 0.0;
+        if (part && bad) {
+          lp = loss = NAN;
+        } else if (live) {
+          const RowDerivative d = policy_terms(A.pol, lp, (double)adv, (double)old, (double)ref, (double)w, &loss, math);
+          if (lane == 0) {
+            S.g = (float)d.g;
+            S.h = (float)d.h;
+          }
+        }
+        if (lane == 0 && rank == 0) {
+          if (A.pol.loss) A.pol.loss[r] = (Row)loss;
+          if (A.pol.logp) A.pol.logp[r] = (Row)lp;
+        }
+      }
+      __syncthreads();
+      if (!A.out.grad) continue;
+      if (live) {
+        g = S.g;
+        h = S.h;
+      }
+    }
+
+    const bool want_h = A.out.hess != nullptr;
+    T* to_g = A.out.grad + r * A.out.row_stride;
+    T* to_h = want_h ? A.out.hess + r * A.out.row_stride : nullptr;
+    const bool whole = (int)((uintptr_t)to_g / sizeof(T) % N) == lead &&
+                       (!want_h || (int)((uintptr_t)to_h / sizeof(T) % N) == lead);
+    const double inv_total = TableMath::inverse(1.0 + rest);
+    const float inv = (float)inv_total, share = (float)(rest * inv_total), down = -g * inv, ag = fabsf(g);
+    const float fill = part && bad ? NAN : 0.0f;
+    const Pair less = Pair::of(-m, -m), scale = Pair::of(kLog2e, kLog2e), times = Pair::of(down, down);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int at = v0 + threadIdx.x + j * THREADS;
+      if (at < v1) {
+        T og[N], oh[N];
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          const float2 d = ((v[j].pair(i) + less) * scale).get();
+          const float x = exp2_approx(d.x), y = exp2_approx(d.y);
+          const float2 f = (Pair::of(x, y) * times).get();
+          narrow(live ? f.x : fill, og[2 * i]);
+          narrow(live ? f.y : fill, og[2 * i + 1]);
+          if (want_h) {
+            const float px = x * inv, py = y * inv;
+            const float hx = px * (ag * (x == 1.0f ? share : 1.0f - px) + h * px);
+            const float hy = py * (ag * (y == 1.0f ? share : 1.0f - py) + h * py);
+            narrow(live ? hx : fill, oh[2 * i]);
+            narrow(live ? hy : fill, oh[2 * i + 1]);
+          }
+        }
+        store_vec(to_g, at * N - lead, K, whole, og);
+        if (want_h) store_vec(to_h, at * N - lead, K, whole, oh);
+      }
+    }
+    if (live) {  // the class taken, by the thread that has just stored it
+      const int at = ((int)a + lead) / N;
+      if (at >= v0 && at < v1 && (at - v0) % THREADS == threadIdx.x) {
+        const float e = exp2_approx((za - m) * kLog2e), p = e * inv, q = e == 1.0f ? share : 1.0f - p;
+        narrow(g * q, to_g[a]);
+        if (want_h) narrow(q * (h * q + ag * p), to_h[a]);
+      }
+    }
+  }
+  if (blocks > 1) cluster.sync();  // the others may still read this block's parts
+}
+
+template <typename T, int OP, int THREADS, int NV>
+void launch_large_t(const RowArgs<T>& A, int blocks, cudaStream_t st) {
+  const long long most = (long long)multiprocessors() * (1024 / THREADS) / blocks;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)(std::min(A.in.n, most) * blocks));
+  lc.blockDim = dim3(THREADS);
+  lc.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  lc.attrs = attr;
+  lc.numAttrs = blocks > 1 ? 1 : 0;
+  MTB_CUDA_FB(cudaLaunchKernelEx(&lc, k_feedback_large<T, OP, THREADS, NV>, A));
+}
+
+// False when a row does not fit a cluster's registers, or its derivatives are
+// not next to each other.
+template <typename T, int OP>
+bool launch_large(const RowArgs<T>& A, cudaStream_t st) {
+  constexpr int N = Vec<T>::N;
+  const bool on_border = on16(A.in.scores) && A.in.stride % N == 0;  // every row
+  const int vecs = ((on_border ? 0 : N - 1) + A.in.K + N - 1) / N;
+  if (OP != ROW_LOGPROBS && A.out.grad && A.out.class_stride != 1) return false;
+  int blocks = 1;
+  while (blocks < 8 && (vecs > 4096 * blocks || (vecs > 512 * blocks && A.in.n * blocks * 2 <= multiprocessors()))) blocks *= 2;
+  const int per = (vecs + blocks - 1) / blocks;
+  if (per > 4096) return false;
+  if (per > 2048) launch_large_t<T, OP, 512, 8>(A, blocks, st);
+  else if (per > 1024) launch_large_t<T, OP, 512, 4>(A, blocks, st);
+  else if (per > 512) launch_large_t<T, OP, 256, 4>(A, blocks, st);
+  else if (per > 128) launch_large_t<T, OP, 128, 4>(A, blocks, st);
+  else launch_large_t<T, OP, 32, 4>(A, blocks, st);
+  return true;
+}
+
 template <typename T, int OP>
 void launch_rows_t(const RowArgs<T>& A, cudaStream_t st) {
   if (A.in.n == 0) return;
@@ -792,6 +1232,8 @@ void launch_rows_t(const RowArgs<T>& A, cudaStream_t st) {
     MTB_CUDA_FB(cudaGetLastError());
     return;
   }
+  if constexpr (sizeof(T) <= 4)
+    if (launch_large<T, OP>(A, st)) return;
   const unsigned grid = (unsigned)std::min<long long>(A.in.n, 1 << 20);
   k_feedback_rows<T, OP><<<grid, kRowThreads, 0, st>>>(A);
   MTB_CUDA_FB(cudaGetLastError());
@@ -1103,6 +1545,10 @@ int device_of(const void* p) {
   return a.device;
 }
 
+void require_aligned(int bytes, std::initializer_list<const void*> arrays) {
+  for (const void* p : arrays) require((uintptr_t)p % bytes == 0, "array is not aligned to its element size");
+}
+
 int common_device(std::initializer_list<const void*> arrays) {
   int dev = -1;
   for (const void* p : arrays) {
@@ -1114,6 +1560,11 @@ int common_device(std::initializer_list<const void*> arrays) {
   return dev;
 }
 
+// Element sizes by score type: scores, per-row values, derivatives.
+int score_bytes(int32_t type) { return type == mtb::SCORE_F64 ? 8 : type == mtb::SCORE_F32 ? 4 : 2; }
+int row_bytes(int32_t type) { return type == mtb::SCORE_F64 ? 8 : 4; }
+int out_bytes(int32_t type) { return std::min(score_bytes(type), 4); }
+
 mtb::ScoreRows score_rows(const void* scores, int32_t type, int64_t n_rows, int64_t n_classes, int64_t stride,
                           const void* actions, int32_t action_bytes) {
   require(type >= mtb::SCORE_F64 && type <= mtb::SCORE_BF16, "unknown score type");
@@ -1123,6 +1574,8 @@ mtb::ScoreRows score_rows(const void* scores, int32_t type, int64_t n_rows, int6
   require(n_rows == 0 || stride <= (int64_t)1 << 46 && n_rows <= ((int64_t)1 << 46) / stride, "scores are too large");
   require(action_bytes == 4 || action_bytes == 8, "actions must be 4 or 8 byte integers");
   require(n_rows == 0 || (scores && actions), "null pointer argument");
+  require_aligned(score_bytes(type), {scores});
+  require_aligned(action_bytes, {actions});
   return {scores, type, n_rows, (int)n_classes, stride, actions, action_bytes == 8};
 }
 
@@ -1142,6 +1595,7 @@ int32_t mojotrees_b200_action_logprobs(const void* scores, int32_t score_type, i
   return checked(error, [&] {
     const mtb::ScoreRows in = score_rows(scores, score_type, n_rows, n_classes, row_stride, actions, action_bytes);
     require(n_rows == 0 || (out_logp && out_stats), "null pointer argument");
+    require_aligned(row_bytes(score_type), {out_logp, out_stats});
     require_cuda();
     if (n_rows == 0) return;
     DeviceScope on(common_device({scores, actions, out_logp, out_stats}));
@@ -1158,6 +1612,9 @@ int32_t mojotrees_b200_action_logprobs_grad(const void* scores, int32_t score_ty
     const mtb::ScoreRows in = score_rows(scores, score_type, n_rows, n_classes, row_stride, actions, action_bytes);
     require(n_rows == 0 || (stats && grad_logp && out_grad), "null pointer argument");
     require(!hess_logp == !out_hess, "hess_logp and out_hess go together");
+    require_aligned(row_bytes(score_type), {stats});
+    require_aligned(4, {grad_logp, hess_logp});
+    require_aligned(out_bytes(score_type), {out_grad, out_hess});
     const mtb::ScoreDerivatives out = derivatives(out_grad, out_hess, n_rows, n_classes, out_stride);
     require_cuda();
     if (n_rows == 0) return;
@@ -1180,6 +1637,8 @@ int32_t mojotrees_b200_policy_loss(const void* scores, int32_t score_type, int64
     require(kl_coef >= 0.0 && std::isfinite(kl_coef), "kl_coef must be finite and non-negative");
     require(kl_coef == 0.0 || ref_logp || n_rows == 0, "kl_coef needs ref_logp");
     require(out_grad || !out_hess, "out_hess needs out_grad");
+    require_aligned(row_bytes(score_type), {advantages, old_logp, ref_logp, weights, out_loss, out_logp});
+    require_aligned(out_bytes(score_type), {out_grad, out_hess});
     const mtb::ScoreDerivatives out =
         out_grad ? derivatives(out_grad, out_hess, n_rows, n_classes, out_stride) : mtb::ScoreDerivatives{};
     require_cuda();
@@ -1227,6 +1686,8 @@ int32_t mojotrees_b200_preference_loss(const MojoTreesPreferencePlan* plan, cons
     const mtb::PreferencePlan& p = plan->plan;
     require(p.n_items == 0 || scores, "null pointer argument");
     require(!out_grad == !out_hess, "out_grad and out_hess go together");
+    require_aligned(score_bytes(score_type), {scores, reference, out_loss});
+    require_aligned(4, {out_grad, out_hess});
     require_cuda();
     if (p.n_items == 0) return;
     const int dev = common_device({scores, reference, out_loss, out_grad, out_hess});

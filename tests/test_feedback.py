@@ -43,7 +43,8 @@ def _logprobs(lib, e, scores=P, kind=1, n=2, k=3, stride=3, actions=P, bytes_=4,
     (dict(scores=None), "null"), (dict(actions=None), "null"), (dict(logp=None), "null"), (dict(stats=None), "null"),
     (dict(kind=4), "score type"), (dict(kind=-1), "score type"), (dict(n=-1), "n_rows"), (dict(k=0), "n_classes"),
     (dict(k=262145, stride=262145), "n_classes"), (dict(stride=2), "row_stride"), (dict(bytes_=2), "actions"),
-    (dict(n=1 << 40, stride=1 << 20), "too large"),
+    (dict(n=1 << 40, stride=1 << 20), "too large"), (dict(scores=P + 2), "aligned"), (dict(actions=P + 4, bytes_=8), "aligned"),
+    (dict(logp=P + 2), "aligned"), (dict(stats=P + 1), "aligned"), (dict(kind=0, logp=P + 4), "aligned"),
 ])
 def test_logprobs_refusals(mtlib, err, kw, needle):
     assert _logprobs(mtlib.lib(), err, **kw) == -1
@@ -56,7 +57,7 @@ def _back(lib, e, stats=P, g=P, h=None, og=P, oh=None, ostride=3):
 
 @pytest.mark.parametrize("kw,needle", [
     (dict(stats=None), "null"), (dict(g=None), "null"), (dict(og=None), "null"), (dict(h=P), "go together"),
-    (dict(oh=P), "go together"), (dict(ostride=2), "out_stride"),
+    (dict(oh=P), "go together"), (dict(ostride=2), "out_stride"), (dict(g=P + 2), "aligned"), (dict(og=P + 1), "aligned"),
 ])
 def test_logprobs_grad_refusals(mtlib, err, kw, needle):
     assert _back(mtlib.lib(), err, **kw) == -1
@@ -73,7 +74,7 @@ def _policy(lib, e, adv=P, old=P, ref=P, low=0.2, high=0.2, kl=0.1, loss=P, og=P
     (dict(low=-0.1), "clip_low"), (dict(low=1.1), "clip_low"), (dict(low=math.nan), "clip_low"),
     (dict(high=-0.1), "clip_high"), (dict(high=math.nan), "clip_high"), (dict(kl=-1.0), "kl_coef"),
     (dict(kl=math.inf), "kl_coef"), (dict(kl=math.nan), "kl_coef"), (dict(og=None, oh=P), "out_grad"),
-    (dict(ostride=1), "out_stride"),
+    (dict(ostride=1), "out_stride"), (dict(adv=P + 2), "aligned"), (dict(og=P + 2), "aligned"),
 ])
 def test_policy_refusals(mtlib, err, kw, needle):
     assert _policy(mtlib.lib(), err, **kw) == -1
