@@ -822,6 +822,11 @@ struct Pair {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(v), "l"(o.v));
     return p;
   }
+  __device__ __forceinline__ Pair times_plus(Pair o, Pair c) const {
+    Pair p;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(v), "l"(o.v), "l"(c.v));
+    return p;
+  }
   __device__ __forceinline__ Pair operator*(Pair o) const {
     Pair p;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(v), "l"(o.v));
@@ -857,6 +862,20 @@ struct Vec {
       return Pair::of(f.x, f.y);
     }
   }
+  __device__ __forceinline__ void set(int i, Pair p) {  // rounds elements 2 i, 2 i + 1
+    const float2 f = p.get();
+    unsigned* w = reinterpret_cast<unsigned*>(&raw);
+    if constexpr (sizeof(T) == 4) {
+      w[2 * i] = __float_as_uint(f.x);
+      w[2 * i + 1] = __float_as_uint(f.y);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
+      w[i] = *reinterpret_cast<const unsigned*>(&b);
+    } else {
+      const __half2 b = __floats2half2_rn(f.x, f.y);
+      w[i] = *reinterpret_cast<const unsigned*>(&b);
+    }
+  }
   __device__ __forceinline__ float max() const {  // NaN when one is
     if constexpr (sizeof(T) == 4) {
       return max_nan32(max_nan32(__uint_as_float(raw.x), __uint_as_float(raw.y)),
@@ -879,61 +898,43 @@ struct Vec {
   }
 };
 
-// The elements [first, first + N) of a row that has elements [0, K): whole
-// where they all exist, else one by one, the others -inf.
-template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* row, int first, int K) {
-  constexpr int N = Vec<T>::N;
-  Vec<T> v;
-  if (first >= 0 && first + N <= K) {
-    v.raw = *reinterpret_cast<const uint4*>(row + first);
-  } else {
-    v = Vec<T>::lowest();
-    T* e = reinterpret_cast<T*>(&v);
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (first + j >= 0 && first + j < K) e[j] = row[first + j];
-  }
-  return v;
-}
-
-template <typename T>
-__device__ __forceinline__ void store_vec(T* row, int first, int K, bool whole, const T (&e)[Vec<T>::N]) {
-  constexpr int N = Vec<T>::N;
-  if (whole && first >= 0 && first + N <= K) {
-    *reinterpret_cast<uint4*>(row + first) = *reinterpret_cast<const uint4*>(e);
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (first + j >= 0 && first + j < K) row[first + j] = e[j];
-  }
-}
-
-// A part of a row: its maximum, and the sum of exp(z - maximum).
+// A part of a row: its maximum m, and a sum of 2^(log2(e) z - c) for a float32
+// c next to log2(e) m, `shift` being log2(e) m - c.  One rounding takes each
+// score to its exponent that way, and the error of c is a factor of the whole
+// sum, which the scalars take out again.
 struct Part {
   double sum;
-  float m;
-  int ones;  // later: how many terms of 1 the sum leaves out
+  float m, shift;
+  int ones;  // terms at the maximum that a later sum leaves out
 };
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.6931471805599453;
+
+// c of the comment above, negated.
+__device__ __forceinline__ float exponent_offset(float m) { return -__fmul_rn(m, kLog2e); }
+
+enum RowState : int { ROW_EMPTY = 0, ROW_DONE = 1, ROW_SLOW = 2, ROW_NEAR = 3 };
 
 template <int THREADS>
 struct LargeShared {
   MathTables tables;
-  Part warp[2][THREADS / 32], slow[2][THREADS / 32];  // by the parity of the row, as all here
+  Part warp[2][THREADS / 32], slow[2][THREADS / 32];  // by the parity of the row, as all arrays here
   Part block[2], slow_block[2];                       // read by the cluster
-  double near_sum[2][THREADS / 32], near_block[2];
-  float g, h;
-  int near;
+  double near[2][THREADS / 32], near_block[2];
+  int state;  // RowState, and what goes with it
+  float m, g, h, inv, share;
 };
 
-// The parts of lanes below n joined: a maximum and a sum relative to it.
+// The parts of lanes below n joined: the maximum, the sum of exp(z - maximum).
 __device__ __forceinline__ Part join_parts(Part p, int n, const TableMath& math) {
   const bool there = (int)(threadIdx.x & 31) < n;
   float m = there ? p.m : -INFINITY;
   for (int k = 16; k > 0; k >>= 1) m = max_nan32(m, __shfl_xor_sync(0xffffffffu, m, k));
-  double s = there && p.m != -INFINITY ? p.sum * math.exp((double)p.m - (double)m) : 0.0;
+  double s = 0.0;
+  if (there && p.m != -INFINITY) s = p.sum * math.exp((double)p.m - (double)m - (double)p.shift * kLn2);
   for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-  return {s, m, 0};
+  return {s, m, 0.0f, 0};
 }
 
 // Sums of parts relative to one maximum.
@@ -951,238 +952,311 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
   namespace cg = cooperative_groups;
   using Row = typename Types<T>::Row;
   constexpr int N = Vec<T>::N, kWarps = THREADS / 32;
-  constexpr float kLog2e = 1.4426950408889634f;
   __shared__ LargeShared<THREADS> S;
   const TableMath math(S.tables);
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int K = A.in.K;
+  const bool want_h = A.out.hess != nullptr;
+  const Pair scale = Pair::of(kLog2e, kLog2e);
   const long long clusters = gridDim.x / blocks;
   int parity = 0;
   for (long long r = blockIdx.x / blocks; r < A.in.n; r += clusters) {
+    // The row's whole vectors of 16 bytes are divided among the blocks.  The
+    // up to 2 (N - 1) elements before and behind them lie with the first
+    // block's first warp: head ones in the lanes from 0, tail ones from 16.
     const T* z = A.in.scores + r * A.in.stride;
-    const int lead = (int)((uintptr_t)z / sizeof(T) % N);  // elements from a 16-byte border to the row's first
-    const int vecs = (lead + K + N - 1) / N, per = (vecs + blocks - 1) / blocks;
+    const int lead = (int)(-(uintptr_t)z / sizeof(T) % N);  // elements before the first whole vector
+    const int vecs = (K - lead) / N, per = (vecs + blocks - 1) / blocks;
     const int v0 = min(vecs, rank * per), v1 = min(vecs, v0 + per);
+    const int tail = K - lead - vecs * N;
+    int edge = -1;
+    if (warp == 0 && rank == 0) edge = lane < lead ? lane : lane >= 16 && lane < 16 + tail ? K - tail + lane - 16 : -1;
+    const T* zv = z + lead + (long long)(v0 + (int)threadIdx.x) * N;
+    const int mine = v1 - v0 - (int)threadIdx.x;  // vector j is this thread's if j * THREADS < mine
     const long long a = A.in.action(r);
     const bool bad = a >= K;
     bool part = a >= 0;
     if (OP == ROW_POLICY && A.pol.weights) part = part && A.pol.weights[r] != (Row)0;
-    double rest = -1.0;
-    float m = 0.0f;
+    float m = 0.0f, g = 0.0f, h = 0.0f, inv = 0.0f, share = 0.0f;
     if (OP == ROW_BACK) {
       m = A.stats[2 * r];
-      rest = (double)A.stats[2 * r + 1];
+      const double rest = (double)A.stats[2 * r + 1];
       part = part && rest != -1.0;
+      if (part && !bad) {
+        g = A.grad_logp[r];
+        if (want_h) h = A.hess_logp[r];
+        const double inv_total = TableMath::inverse(1.0 + rest);
+        const double shift = (double)fmaf(m, kLog2e, exponent_offset(m));
+        inv = (float)(inv_total * math.exp(-shift * kLn2));
+        share = (float)(rest * inv_total);
+      }
     }
     bool live = part && !bad;
     Vec<T> v[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int at = v0 + threadIdx.x + j * THREADS;
-      v[j] = live && at < v1 ? load_vec(z, at * N - lead, K) : Vec<T>::lowest();
-    }
-    if (threadIdx.x == 0 && r + clusters < A.in.n) {  // this block's part of its next row, the whole vectors of it
-      const T* zn = z + clusters * A.in.stride;
-      const int ln = (int)((uintptr_t)zn / sizeof(T) % N);
-      const int b = max(v0 * N - ln, ln ? N - ln : 0), e = min(v1 * N - ln, (K + ln) / N * N - ln);
-      if (b < e)
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(zn + b), "r"((e - b) * (int)sizeof(T)) : "memory");
-    }
-    float za = 0.0f, adv = 0.0f, old = 0.0f, ref = 0.0f, w = 1.0f;
+    float ze = -INFINITY, za = 0.0f;
     if (live) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        v[j] = Vec<T>::lowest();
+        if (j * THREADS < mine) v[j].raw = *reinterpret_cast<const uint4*>(zv + j * THREADS * N);
+      }
+      if (edge >= 0) ze = widen(z[edge]);
       za = widen(z[a]);
+    }
+    if (threadIdx.x == 0 && r + clusters < A.in.n) {  // the next row's vectors of this block
+      const T* zn = z + clusters * A.in.stride;
+      const int ln = (int)(-(uintptr_t)zn / sizeof(T) % N);
+      const int e = min(v1, (K - ln) / N);
+      if (v0 < e)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(zn + ln + v0 * N), "r"((e - v0) * 16) : "memory");
+    }
+
+    if (OP != ROW_BACK && live) {
+      parity ^= 1;
+      float adv = 0.0f, old = 0.0f, ref = 0.0f, w = 1.0f;
       if (OP == ROW_POLICY && warp == 0) {
         adv = A.pol.advantages[r];
         old = A.pol.old_logp[r];
         if (A.pol.ref_logp) ref = A.pol.ref_logp[r];
         if (A.pol.weights) w = A.pol.weights[r];
       }
-    }
+      // the first warp's end of a row; near: l is right whatever the border
+      auto finish = [&](float top, double rest, double lp, bool near_known) {
+        const double total = 1.0 + rest, inv_total = TableMath::inverse(total);
+        if (OP == ROW_LOGPROBS) {
+          if (threadIdx.x == 0) {
+            S.state = ROW_DONE;
+            if (rank == 0) {
+              A.logp[r] = (Row)lp;
+              A.stats[2 * r] = top;
+              A.stats[2 * r + 1] = (Row)rest;
+            }
+          }
+          return;
+        }
+        const bool masked = za == -INFINITY;
+        const bool near = !near_known && !masked && near_border(A.pol, lp - (double)old, (double)adv,
+                                                                border_slack(NV * N / 2 + 8, 12.5));
+        double loss = 0.0;
+        RowDerivative d = {0.0, 0.0};
+        if (!near && !masked)
+          d = policy_terms(A.pol, lp, (double)adv, (double)old, (double)ref, (double)w, &loss, math);
+        if (threadIdx.x == 0) {
+          const double shift = (double)fmaf(top, kLog2e, exponent_offset(top));
+          S.state = near ? ROW_NEAR : masked ? ROW_EMPTY : ROW_DONE;
+          S.m = top;
+          S.g = (float)d.g;
+          S.h = (float)d.h;
+          S.inv = (float)(inv_total * math.exp(-shift * kLn2));
+          S.share = (float)(rest * inv_total);
+          if (rank == 0 && !near) {
+            if (A.pol.loss) A.pol.loss[r] = (Row)loss;
+            if (A.pol.logp) A.pol.logp[r] = (Row)lp;
+          }
+        }
+      };
 
-    if (OP != ROW_BACK && live) {
-      parity ^= 1;
       // the warp's maximum, and its sum relative to it
-      float wm = -INFINITY;
+      float wm = ze;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         wm = max_nan32(wm, v[j].max());
         v[j].forget();
       }
       for (int k = 16; k > 0; k >>= 1) wm = max_nan32(wm, __shfl_xor_sync(0xffffffffu, wm, k));
-      Part p = {0.0, wm, 0};
+      Part p = {0.0, wm, 0.0f, 0};
       if (wm != -INFINITY) {
-        const Pair less = Pair::of(-wm, -wm), scale = Pair::of(kLog2e, kLog2e);
-        Pair sum = Pair::of(0.0f, 0.0f);
+        const float c = exponent_offset(wm);
+        const Pair offset = Pair::of(c, c);
+        Pair sum = Pair::of(exp2_approx(fmaf(ze, kLog2e, c)), 0.0f);
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
 #pragma unroll
           for (int i = 0; i < N / 2; ++i) {
-            const float2 d = ((v[j].pair(i) + less) * scale).get();
+            const float2 d = v[j].pair(i).times_plus(scale, offset).get();
             sum = sum + Pair::of(exp2_approx(d.x), exp2_approx(d.y));
-            if (i == N / 2 - 1) v[j].forget();
           }
+          v[j].forget();
+        }
         float s = sum.get().x + sum.get().y;
         for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
         p.sum = (double)s;
+        p.shift = fmaf(wm, kLog2e, c);
       }
       if (lane == 0) S.warp[parity][warp] = p;
       __syncthreads();
-      Part all = join_parts(S.warp[parity][lane < kWarps ? lane : 0], kWarps, math);
+      Part all;
+      if (warp == 0) all = join_parts(S.warp[parity][lane < kWarps ? lane : 0], kWarps, math);
       if (blocks > 1) {
         if (threadIdx.x == 0) S.block[parity] = all;
         cluster.sync();
-        all = join_parts(*cluster.map_shared_rank(&S.block[parity], lane < blocks ? lane : 0), blocks, math);
-      }
-      if (all.m == -INFINITY) {
-        live = part = false;
-      } else {
-        m = all.m;
-        rest = all.sum - 1.0;
-        if (rest < 1.0) {
-          // One class has more than half, and its 1 took the last bits of the
-          // others: the sum without the terms of 1, of the warps that have any.
-          if (wm == m) {
-            float s = 0.0f;
-            int ones = 0;
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-#pragma unroll
-              for (int i = 0; i < N / 2; ++i) {
-                const float2 f = v[j].pair(i).get();
-                const float x = exp2_approx((f.x - m) * kLog2e), y = exp2_approx((f.y - m) * kLog2e);
-                s += (x == 1.0f ? 0.0f : x) + (y == 1.0f ? 0.0f : y);
-                ones += (x == 1.0f ? 1 : 0) + (y == 1.0f ? 1 : 0);
-                if (i == N / 2 - 1) v[j].forget();
-              }
-            for (int k = 16; k > 0; k >>= 1) {
-              s += __shfl_xor_sync(0xffffffffu, s, k);
-              ones += __shfl_xor_sync(0xffffffffu, ones, k);
-            }
-            p = {(double)s, m, ones};
-          } else if (wm != -INFINITY) {
-            p.sum *= math.exp((double)wm - (double)m);
-          }
-          if (lane == 0) S.slow[parity][warp] = p;
-          __syncthreads();
-          p = add_parts(S.slow[parity][lane < kWarps ? lane : 0], kWarps);
-          if (blocks > 1) {
-            if (threadIdx.x == 0) S.slow_block[parity] = p;
-            cluster.sync();
-            p = add_parts(*cluster.map_shared_rank(&S.slow_block[parity], lane < blocks ? lane : 0), blocks);
-          }
-          rest = p.sum + (double)(p.ones - 1);
-        }
-      }
-    }
-
-    float g = 0.0f, h = 0.0f;
-    if (OP == ROW_LOGPROBS) {
-      if (threadIdx.x == 0 && rank == 0) {
-        const bool nan = part && bad;
-        A.logp[r] = nan ? NAN : live ? (Row)((double)za - (double)m - math.log1p(rest)) : (Row)0;
-        A.stats[2 * r] = nan ? NAN : live ? m : 0.0f;
-        A.stats[2 * r + 1] = nan ? NAN : live ? (Row)rest : (Row)-1;
-      }
-      continue;
-    } else if (OP == ROW_BACK) {
-      if (live) {
-        g = A.grad_logp[r];
-        if (A.hess_logp) h = A.hess_logp[r];
-      }
-    } else {
-      double lp = 0.0;
-      if (live) {
-        lp = (double)za - (double)m - math.log1p(rest);
-        live = part = za != -INFINITY;  // the class taken is masked
-      }
-      if (live) {
-        if (threadIdx.x == 0)
-          S.near = near_border(A.pol, lp - (double)old, (double)adv, border_slack(NV * N / 2 + 7, 12.5)) ? 1 : 0;
-        __syncthreads();
-        if (S.near) {
-          double sum = 0.0;
-          for (int k = max(v0 * N - lead, 0) + threadIdx.x; k < min(v1 * N - lead, K); k += THREADS)
-            sum += math.exp((double)widen(z[k]) - (double)m);
-          for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-          if (lane == 0) S.near_sum[parity][warp] = sum;
-          __syncthreads();
-          sum = 0.0;
-          for (int i = 0; i < kWarps; ++i) sum += S.near_sum[parity][i];
-          if (blocks > 1) {
-            if (threadIdx.x == 0) S.near_block[parity] = sum;
-            cluster.sync();
-            sum = 0.0;
-            for (int i = 0; i < blocks; ++i) sum += *cluster.map_shared_rank(&S.near_block[parity], i);
-          }
-          lp = (double)za - (double)m - log(sum);
-        }
+        if (warp == 0) all = join_parts(*cluster.map_shared_rank(&S.block[parity], lane < blocks ? lane : 0), blocks, math);
       }
       if (warp == 0) {
-        double loss = 0.0;
-        if (part && bad) {
-          lp = loss = NAN;
-        } else if (live) {
-          const RowDerivative d = policy_terms(A.pol, lp, (double)adv, (double)old, (double)ref, (double)w, &loss, math);
+        const double rest = all.sum - 1.0;
+        if (all.m == -INFINITY || rest < 1.0) {
           if (lane == 0) {
-            S.g = (float)d.g;
-            S.h = (float)d.h;
+            S.state = all.m == -INFINITY ? ROW_EMPTY : ROW_SLOW;
+            S.m = all.m;
+            if (OP == ROW_POLICY && rank == 0 && S.state == ROW_EMPTY) {
+              if (A.pol.loss) A.pol.loss[r] = 0.0f;
+              if (A.pol.logp) A.pol.logp[r] = 0.0f;
+            }
           }
-        }
-        if (lane == 0 && rank == 0) {
-          if (A.pol.loss) A.pol.loss[r] = (Row)loss;
-          if (A.pol.logp) A.pol.logp[r] = (Row)lp;
+        } else {
+          finish(all.m, rest, (double)za - (double)all.m - math.log1p(rest), false);
         }
       }
       __syncthreads();
-      if (!A.out.grad) continue;
-      if (live) {
+      if (S.state == ROW_SLOW) {
+        // One class has more than half, and its 1 took the last bits of the
+        // others: the sum without the terms at the maximum, of the warps that
+        // have any.
+        const float top = S.m;
+        if (wm == top) {
+          const float c = exponent_offset(top);
+          float s = ze == top ? 0.0f : exp2_approx(fmaf(ze, kLog2e, c));
+          int ones = ze == top ? 1 : 0;
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+              const float2 f = v[j].pair(i).get();
+              s += f.x == top ? 0.0f : exp2_approx(fmaf(f.x, kLog2e, c));
+              s += f.y == top ? 0.0f : exp2_approx(fmaf(f.y, kLog2e, c));
+              ones += (f.x == top ? 1 : 0) + (f.y == top ? 1 : 0);
+            }
+            v[j].forget();
+          }
+          for (int k = 16; k > 0; k >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, k);
+            ones += __shfl_xor_sync(0xffffffffu, ones, k);
+          }
+          p.sum = (double)s;
+          p.ones = ones;
+        }
+        if (wm != -INFINITY) p.sum *= math.exp((double)wm - (double)top - (double)p.shift * kLn2);
+        if (lane == 0) S.slow[parity][warp] = p;
+        __syncthreads();
+        if (warp == 0) p = add_parts(S.slow[parity][lane < kWarps ? lane : 0], kWarps);
+        if (blocks > 1) {
+          if (threadIdx.x == 0) S.slow_block[parity] = p;
+          cluster.sync();
+          if (warp == 0) p = add_parts(*cluster.map_shared_rank(&S.slow_block[parity], lane < blocks ? lane : 0), blocks);
+        }
+        if (warp == 0) {
+          const double rest = p.sum + (double)(p.ones - 1);
+          finish(top, rest, (double)za - (double)top - math.log1p(rest), false);
+        }
+        __syncthreads();
+      }
+      if (OP == ROW_POLICY && S.state == ROW_NEAR) {
+        const float top = S.m;
+        const double share64 = (double)S.share, inv64 = (double)S.inv;
+        double sum = ze == -INFINITY ? 0.0 : math.exp((double)ze - (double)top);
+        for (int k = threadIdx.x; k < (v1 - v0) * N; k += THREADS)
+          sum += math.exp((double)widen(z[lead + v0 * N + k]) - (double)top);
+        for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        if (lane == 0) S.near[parity][warp] = sum;
+        __syncthreads();
+        sum = 0.0;
+        for (int i = 0; i < kWarps; ++i) sum += S.near[parity][i];
+        if (blocks > 1) {
+          if (threadIdx.x == 0) S.near_block[parity] = sum;
+          cluster.sync();
+          sum = 0.0;
+          for (int i = 0; i < blocks; ++i) sum += *cluster.map_shared_rank(&S.near_block[parity], i);
+        }
+        if (warp == 0) finish(top, sum - 1.0, (double)za - (double)top - log(sum), true);
+        if (threadIdx.x == 0) {  // as the row's other paths have them
+          S.share = (float)share64;
+          S.inv = (float)inv64;
+        }
+        __syncthreads();
+      }
+      live = part = S.state == ROW_DONE;
+      if (live && OP == ROW_POLICY) {
+        m = S.m;
         g = S.g;
         h = S.h;
+        inv = S.inv;
+        share = S.share;
       }
     }
+    if (OP != ROW_BACK && !live && threadIdx.x == 0 && rank == 0) {
+      const float none = part && bad ? NAN : 0.0f;
+      if (OP == ROW_LOGPROBS) {
+        A.logp[r] = none;
+        A.stats[2 * r] = none;
+        A.stats[2 * r + 1] = part && bad ? NAN : -1.0f;
+      } else if (za != -INFINITY) {  // else the row's values are written
+        if (A.pol.loss) A.pol.loss[r] = none;
+        if (A.pol.logp) A.pol.logp[r] = none;
+      }
+    }
+    if (OP == ROW_LOGPROBS || !A.out.grad) continue;
 
-    const bool want_h = A.out.hess != nullptr;
     T* to_g = A.out.grad + r * A.out.row_stride;
     T* to_h = want_h ? A.out.hess + r * A.out.row_stride : nullptr;
-    const bool whole = (int)((uintptr_t)to_g / sizeof(T) % N) == lead &&
-                       (!want_h || (int)((uintptr_t)to_h / sizeof(T) % N) == lead);
-    const double inv_total = TableMath::inverse(1.0 + rest);
-    const float inv = (float)inv_total, share = (float)(rest * inv_total), down = -g * inv, ag = fabsf(g);
-    const float fill = part && bad ? NAN : 0.0f;
-    const Pair less = Pair::of(-m, -m), scale = Pair::of(kLog2e, kLog2e), times = Pair::of(down, down);
+    if (!live) {
+      T fill;
+      narrow(part && bad ? NAN : 0.0f, fill);
+      for (int k = rank * THREADS + threadIdx.x; k < K; k += blocks * THREADS) {
+        to_g[k] = fill;
+        if (want_h) to_h[k] = fill;
+      }
+      continue;
+    }
+    // whether the derivatives' vectors start on 16 bytes where the scores' do
+    const bool whole = (uintptr_t)(to_g + lead) % 16 == 0 && (!want_h || (uintptr_t)(to_h + lead) % 16 == 0);
+    const float c = exponent_offset(m), down = -g * inv, ag = fabsf(g);
+    const Pair offset = Pair::of(c, c), times = Pair::of(down, down);
+    const long long at = lead + (long long)(v0 + (int)threadIdx.x) * N;
+    auto hess_of = [&](float score, float e) {
+      const float p = e * inv;
+      return p * (ag * (score == m ? share : 1.0f - p) + h * p);
+    };
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int at = v0 + threadIdx.x + j * THREADS;
-      if (at < v1) {
-        T og[N], oh[N];
+      if (j * THREADS < mine) {
+        Vec<T> og, oh;
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
-          const float2 d = ((v[j].pair(i) + less) * scale).get();
+          const float2 d = v[j].pair(i).times_plus(scale, offset).get();
           const float x = exp2_approx(d.x), y = exp2_approx(d.y);
-          const float2 f = (Pair::of(x, y) * times).get();
-          narrow(live ? f.x : fill, og[2 * i]);
-          narrow(live ? f.y : fill, og[2 * i + 1]);
+          og.set(i, Pair::of(x, y) * times);
           if (want_h) {
-            const float px = x * inv, py = y * inv;
-            const float hx = px * (ag * (x == 1.0f ? share : 1.0f - px) + h * px);
-            const float hy = py * (ag * (y == 1.0f ? share : 1.0f - py) + h * py);
-            narrow(live ? hx : fill, oh[2 * i]);
-            narrow(live ? hy : fill, oh[2 * i + 1]);
+            const float2 f = v[j].pair(i).get();
+            oh.set(i, Pair::of(hess_of(f.x, x), hess_of(f.y, y)));
           }
         }
-        store_vec(to_g, at * N - lead, K, whole, og);
-        if (want_h) store_vec(to_h, at * N - lead, K, whole, oh);
+        T* pg = to_g + at + j * THREADS * N;
+        T* ph = to_h + at + j * THREADS * N;
+        if (whole) {
+          *reinterpret_cast<uint4*>(pg) = og.raw;
+          if (want_h) *reinterpret_cast<uint4*>(ph) = oh.raw;
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            pg[i] = reinterpret_cast<const T*>(&og)[i];
+            if (want_h) ph[i] = reinterpret_cast<const T*>(&oh)[i];
+          }
+        }
       }
     }
-    if (live) {  // the class taken, by the thread that has just stored it
-      const int at = ((int)a + lead) / N;
-      if (at >= v0 && at < v1 && (at - v0) % THREADS == threadIdx.x) {
-        const float e = exp2_approx((za - m) * kLog2e), p = e * inv, q = e == 1.0f ? share : 1.0f - p;
-        narrow(g * q, to_g[a]);
-        if (want_h) narrow(q * (h * q + ag * p), to_h[a]);
-      }
+    if (edge >= 0) {
+      const float e = exp2_approx(fmaf(ze, kLog2e, c));
+      narrow(e * down, to_g[edge]);
+      if (want_h) narrow(hess_of(ze, e), to_h[edge]);
+    }
+    // the class taken, by the thread that has just stored it
+    const int taken = (int)a, tv = taken >= lead ? (taken - lead) / N : vecs;
+    if (edge == taken || (tv >= v0 && tv < v1 && (tv - v0) % THREADS == (int)threadIdx.x)) {
+      const float p = exp2_approx(fmaf(za, kLog2e, c)) * inv, q = za == m ? share : 1.0f - p;
+      narrow(g * q, to_g[taken]);
+      if (want_h) narrow(q * (h * q + ag * p), to_h[taken]);
     }
   }
   if (blocks > 1) cluster.sync();  // the others may still read this block's parts
@@ -1209,8 +1283,7 @@ void launch_large_t(const RowArgs<T>& A, int blocks, cudaStream_t st) {
 template <typename T, int OP>
 bool launch_large(const RowArgs<T>& A, cudaStream_t st) {
   constexpr int N = Vec<T>::N;
-  const bool on_border = on16(A.in.scores) && A.in.stride % N == 0;  // every row
-  const int vecs = ((on_border ? 0 : N - 1) + A.in.K + N - 1) / N;
+  const int vecs = A.in.K / N;  // or one fewer, where a row does not start on 16 bytes
   if (OP != ROW_LOGPROBS && A.out.grad && A.out.class_stride != 1) return false;
   int blocks = 1;
   while (blocks < 8 && (vecs > 4096 * blocks || (vecs > 512 * blocks && A.in.n * blocks * 2 <= multiprocessors()))) blocks *= 2;
