@@ -947,8 +947,17 @@ __device__ __forceinline__ Part add_parts(Part p, int n) {
   return p;
 }
 
-template <typename T, int OP, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(const RowArgs<T> A) {
+// A vector's elements one by one, for derivatives whose vectors do not start
+// on 16 bytes where the scores' do.
+template <typename T>
+__device__ __noinline__ void store_elements(T* to, Vec<T> v) {
+#pragma unroll
+  for (int i = 0; i < Vec<T>::N; ++i) to[i] = reinterpret_cast<const T*>(&v)[i];
+}
+
+// per: whole vectors of a row that a block takes at most.
+template <typename T, int OP, bool HESS, int THREADS, int NV>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(const RowArgs<T> A, const int per) {
   namespace cg = cooperative_groups;
   using Row = typename Types<T>::Row;
   constexpr int N = Vec<T>::N, kWarps = THREADS / 32;
@@ -958,7 +967,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int K = A.in.K;
-  const bool want_h = A.out.hess != nullptr;
   const Pair scale = Pair::of(kLog2e, kLog2e);
   const long long clusters = gridDim.x / blocks;
   int parity = 0;
@@ -968,7 +976,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
     // block's first warp: head ones in the lanes from 0, tail ones from 16.
     const T* z = A.in.scores + r * A.in.stride;
     const int lead = (int)(-(uintptr_t)z / sizeof(T) % N);  // elements before the first whole vector
-    const int vecs = (K - lead) / N, per = (vecs + blocks - 1) / blocks;
+    const int vecs = (int)((unsigned)(K - lead) / N);
     const int v0 = min(vecs, rank * per), v1 = min(vecs, v0 + per);
     const int tail = K - lead - vecs * N;
     int edge = -1;
@@ -982,15 +990,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
     float m = 0.0f, g = 0.0f, h = 0.0f, inv = 0.0f, share = 0.0f;
     if (OP == ROW_BACK) {
       m = A.stats[2 * r];
-      const double rest = (double)A.stats[2 * r + 1];
-      part = part && rest != -1.0;
+      const float rest = A.stats[2 * r + 1];
+      part = part && rest != -1.0f;
       if (part && !bad) {
         g = A.grad_logp[r];
-        if (want_h) h = A.hess_logp[r];
-        const double inv_total = TableMath::inverse(1.0 + rest);
-        const double shift = (double)fmaf(m, kLog2e, exponent_offset(m));
-        inv = (float)(inv_total * math.exp(-shift * kLn2));
-        share = (float)(rest * inv_total);
+        if (HESS) h = A.hess_logp[r];
+        const float inv_total = __frcp_rn(1.0f + rest);
+        inv = inv_total * exp2_approx(-fmaf(m, kLog2e, exponent_offset(m)));
+        share = rest * inv_total;
       }
     }
     bool live = part && !bad;
@@ -1088,7 +1095,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
       if (lane == 0) S.warp[parity][warp] = p;
       __syncthreads();
       Part all;
-      if (warp == 0) all = join_parts(S.warp[parity][lane < kWarps ? lane : 0], kWarps, math);
+      if (kWarps == 1) all = {p.sum * math.exp(-(double)p.shift * kLn2), wm, 0.0f, 0};
+      else if (warp == 0) all = join_parts(S.warp[parity][lane < kWarps ? lane : 0], kWarps, math);
       if (blocks > 1) {
         if (threadIdx.x == 0) S.block[parity] = all;
         cluster.sync();
@@ -1199,18 +1207,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
     if (OP == ROW_LOGPROBS || !A.out.grad) continue;
 
     T* to_g = A.out.grad + r * A.out.row_stride;
-    T* to_h = want_h ? A.out.hess + r * A.out.row_stride : nullptr;
+    T* to_h = HESS ? A.out.hess + r * A.out.row_stride : nullptr;
     if (!live) {
       T fill;
       narrow(part && bad ? NAN : 0.0f, fill);
       for (int k = rank * THREADS + threadIdx.x; k < K; k += blocks * THREADS) {
         to_g[k] = fill;
-        if (want_h) to_h[k] = fill;
+        if (HESS) to_h[k] = fill;
       }
       continue;
     }
-    // whether the derivatives' vectors start on 16 bytes where the scores' do
-    const bool whole = (uintptr_t)(to_g + lead) % 16 == 0 && (!want_h || (uintptr_t)(to_h + lead) % 16 == 0);
+    const bool whole = (uintptr_t)(to_g + lead) % 16 == 0 && (!HESS || (uintptr_t)(to_h + lead) % 16 == 0);
     const float c = exponent_offset(m), down = -g * inv, ag = fabsf(g);
     const Pair offset = Pair::of(c, c), times = Pair::of(down, down);
     const long long at = lead + (long long)(v0 + (int)threadIdx.x) * N;
@@ -1225,45 +1232,42 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
           const float2 d = v[j].pair(i).times_plus(scale, offset).get();
-          const float x = exp2_approx(d.x), y = exp2_approx(d.y);
-          og.set(i, Pair::of(x, y) * times);
-          if (want_h) {
+          const Pair e = Pair::of(exp2_approx(d.x), exp2_approx(d.y));
+          og.set(i, e * times);
+          if (HESS) {
             const float2 f = v[j].pair(i).get();
-            oh.set(i, Pair::of(hess_of(f.x, x), hess_of(f.y, y)));
+            oh.set(i, Pair::of(hess_of(f.x, e.get().x), hess_of(f.y, e.get().y)));
           }
         }
         T* pg = to_g + at + j * THREADS * N;
-        T* ph = to_h + at + j * THREADS * N;
+        T* ph = HESS ? to_h + at + j * THREADS * N : nullptr;
         if (whole) {
           *reinterpret_cast<uint4*>(pg) = og.raw;
-          if (want_h) *reinterpret_cast<uint4*>(ph) = oh.raw;
+          if (HESS) *reinterpret_cast<uint4*>(ph) = oh.raw;
         } else {
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            pg[i] = reinterpret_cast<const T*>(&og)[i];
-            if (want_h) ph[i] = reinterpret_cast<const T*>(&oh)[i];
-          }
+          store_elements(pg, og);
+          if (HESS) store_elements(ph, oh);
         }
       }
     }
     if (edge >= 0) {
       const float e = exp2_approx(fmaf(ze, kLog2e, c));
       narrow(e * down, to_g[edge]);
-      if (want_h) narrow(hess_of(ze, e), to_h[edge]);
+      if (HESS) narrow(hess_of(ze, e), to_h[edge]);
     }
     // the class taken, by the thread that has just stored it
     const int taken = (int)a, tv = taken >= lead ? (taken - lead) / N : vecs;
     if (edge == taken || (tv >= v0 && tv < v1 && (tv - v0) % THREADS == (int)threadIdx.x)) {
       const float p = exp2_approx(fmaf(za, kLog2e, c)) * inv, q = za == m ? share : 1.0f - p;
       narrow(g * q, to_g[taken]);
-      if (want_h) narrow(q * (h * q + ag * p), to_h[taken]);
+      if (HESS) narrow(q * (h * q + ag * p), to_h[taken]);
     }
   }
   if (blocks > 1) cluster.sync();  // the others may still read this block's parts
 }
 
-template <typename T, int OP, int THREADS, int NV>
-void launch_large_t(const RowArgs<T>& A, int blocks, cudaStream_t st) {
+template <typename T, int OP, bool HESS, int THREADS, int NV>
+void launch_large_t(const RowArgs<T>& A, int blocks, int per, cudaStream_t st) {
   const long long most = (long long)multiprocessors() * (1024 / THREADS) / blocks;
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3((unsigned)(std::min(A.in.n, most) * blocks));
@@ -1275,25 +1279,31 @@ void launch_large_t(const RowArgs<T>& A, int blocks, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   lc.attrs = attr;
   lc.numAttrs = blocks > 1 ? 1 : 0;
-  MTB_CUDA_FB(cudaLaunchKernelEx(&lc, k_feedback_large<T, OP, THREADS, NV>, A));
+  MTB_CUDA_FB(cudaLaunchKernelEx(&lc, k_feedback_large<T, OP, HESS, THREADS, NV>, A, per));
+}
+
+template <typename T, int OP, bool HESS>
+void launch_large_h(const RowArgs<T>& A, int blocks, int per, cudaStream_t st) {
+  if (per > 2048) launch_large_t<T, OP, HESS, 512, 8>(A, blocks, per, st);
+  else if (per > 1024) launch_large_t<T, OP, HESS, 512, 4>(A, blocks, per, st);
+  else if (per > 512) launch_large_t<T, OP, HESS, 256, 4>(A, blocks, per, st);
+  else if (per > 128) launch_large_t<T, OP, HESS, 128, 4>(A, blocks, per, st);
+  else launch_large_t<T, OP, HESS, 32, 4>(A, blocks, per, st);
 }
 
 // False when a row does not fit a cluster's registers, or its derivatives are
 // not next to each other.
 template <typename T, int OP>
 bool launch_large(const RowArgs<T>& A, cudaStream_t st) {
-  constexpr int N = Vec<T>::N;
-  const int vecs = A.in.K / N;  // or one fewer, where a row does not start on 16 bytes
+  const int vecs = A.in.K / Vec<T>::N;  // or one fewer, where a row does not start on 16 bytes
   if (OP != ROW_LOGPROBS && A.out.grad && A.out.class_stride != 1) return false;
   int blocks = 1;
   while (blocks < 8 && (vecs > 4096 * blocks || (vecs > 512 * blocks && A.in.n * blocks * 2 <= multiprocessors()))) blocks *= 2;
   const int per = (vecs + blocks - 1) / blocks;
   if (per > 4096) return false;
-  if (per > 2048) launch_large_t<T, OP, 512, 8>(A, blocks, st);
-  else if (per > 1024) launch_large_t<T, OP, 512, 4>(A, blocks, st);
-  else if (per > 512) launch_large_t<T, OP, 256, 4>(A, blocks, st);
-  else if (per > 128) launch_large_t<T, OP, 128, 4>(A, blocks, st);
-  else launch_large_t<T, OP, 32, 4>(A, blocks, st);
+  if constexpr (OP == ROW_LOGPROBS) launch_large_h<T, OP, false>(A, blocks, per, st);
+  else if (A.out.hess) launch_large_h<T, OP, true>(A, blocks, per, st);
+  else launch_large_h<T, OP, false>(A, blocks, per, st);
   return true;
 }
 
