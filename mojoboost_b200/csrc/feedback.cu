@@ -1361,83 +1361,213 @@ void by_type(int type, F&& f) {
 //   squared   L = (u - 1 / (2 beta))^2
 // in float64 throughout: u is the difference of log probabilities of whole
 // answers, tens or hundreds each.
+//
+// An item's derivatives are a sum over its pairs, which the plan lists item by
+// item: no atomics, and the same bits at every call.  Each pair's terms are
+// computed for both of its items (a dozen float64 operations on top of what
+// each loads) rather than once and stored, which would take memory that calls
+// share; the winner's side also writes the pair's loss.  What bounds it is
+// the other item's score and reference: a sector of L2 each per entry.
 struct PairMath {
   double beta, smoothing, target;  // target: 1 / (2 beta)
   int kind;
-  __device__ __forceinline__ double loss(double u) const {
-    if (kind == PREFERENCE_SQUARED) return (u - target) * (u - target);
-    const double x = beta * u, soft = log1p(exp(-fabs(x)));
-    if (x != x) return x;
-    const double won = (1.0 - smoothing) * (soft + fmax(-x, 0.0));
-    return smoothing > 0.0 ? won + smoothing * (soft + fmax(x, 0.0)) : won;  // an infinite x times 0 is no NaN
+};
+
+struct PairTerms {
+  double g, h, loss;
+};
+
+__device__ __forceinline__ PairTerms pair_terms(const PairMath& pm, double u, const TableMath& math) {
+  if (pm.kind == PREFERENCE_SQUARED) {
+    const double d = u - pm.target;
+    return {2.0 * d, 2.0, d * d};
   }
-  __device__ __forceinline__ RowDerivative derivative(double u) const {
-    if (kind == PREFERENCE_SQUARED) return {2.0 * (u - target), 2.0};
-    const double x = beta * u, e = exp(-fabs(x)), big = 1.0 / (1.0 + e), small = e * big;
-    const double up = x >= 0.0 ? big : small, down = x >= 0.0 ? small : big;
-    return {beta * (smoothing * up - (1.0 - smoothing) * down), beta * beta * big * small};
+  const double x = pm.beta * u, e = math.exp(-fabs(x)), big = TableMath::inverse(1.0 + e), small = e * big;
+  const double up = x >= 0.0 ? big : small, down = x >= 0.0 ? small : big, soft = math.log1p(e);
+  PairTerms t = {-pm.beta * (1.0 - pm.smoothing) * down, pm.beta * pm.beta * big * small,
+                 (1.0 - pm.smoothing) * (soft + fmax(-x, 0.0))};
+  if (pm.smoothing > 0.0) {  // an infinite x times 0 would be NaN
+    t.g += pm.beta * pm.smoothing * up;
+    t.loss += pm.smoothing * (soft + fmax(x, 0.0));
   }
+  if (x != x) t.loss = x;
+  return t;
+}
+
+template <typename T>
+struct PreferenceArgs {
+  const int* offsets;
+  const int2* entries;
+  const float* entry_w;
+  const int* zero_pairs;
+  int n_zero, n_items;
+  const T *s, *ref;
+  PairMath pm;
+  T* loss;
+  float *grad, *hess;
 };
 
 template <typename T>
-__device__ __forceinline__ double lean(const T* s, const T* ref, int i) {
-  return ref ? (double)s[i] - (double)ref[i] : (double)s[i];
+__device__ __forceinline__ double lean(const PreferenceArgs<T>& A, int i) {
+  return A.ref ? (double)A.s[i] - (double)A.ref[i] : (double)A.s[i];
 }
 
-// u from each item's distance to its reference: what an infinite reference
-// or score leaves undefined is NaN.
+// One entry of item i's list; `own` is the item's own distance to its reference.
 template <typename T>
-__global__ void __launch_bounds__(256) k_preference_items(const int* __restrict__ offsets,
-                                                          const int* __restrict__ partners,
-                                                          const float* __restrict__ entry_w, long long n,
-                                                          const T* __restrict__ s, const T* __restrict__ ref,
-                                                          PairMath pm, float* __restrict__ grad,
-                                                          float* __restrict__ hess) {
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-    const int e1 = offsets[i + 1];
+__device__ __forceinline__ void add_entry(const PreferenceArgs<T>& A, int2 entry, double w, double own, double other,
+                                          const TableMath& math, double* g, double* h) {
+  const bool lost = entry.x < 0;
+  const PairTerms t = pair_terms(A.pm, lost ? other - own : own - other, math);
+  *g += lost ? -(w * t.g) : w * t.g;
+  *h += w * t.h;
+  if (!lost && A.loss) A.loss[entry.y] = (T)(w * t.loss);
+}
+
+constexpr int kPairThreads = 256;
+// Items of more pairs than a warp takes in this many steps have a block, or
+// from kHuge pairs a cluster of 8, to themselves: a warp's steps are one
+// after the other, about 0.5 us each with four loads in flight.
+constexpr int kWarpSteps = 16;
+constexpr int kLong = 32 * kWarpSteps;
+constexpr int kHuge = 16384;
+constexpr int kPairCluster = 8;
+
+// G lanes an item.
+template <typename T, int G>
+__global__ void __launch_bounds__(kPairThreads) k_preference_items(const PreferenceArgs<T> A) {
+  __shared__ MathTables tables;
+  const TableMath math(tables);
+  const long long thread = (long long)blockIdx.x * kPairThreads + threadIdx.x;
+  const long long threads = (long long)gridDim.x * kPairThreads;
+  if (A.loss)
+    for (long long z = thread; z < A.n_zero; z += threads) A.loss[A.zero_pairs[z]] = (T)0;
+  const int l = threadIdx.x % G;
+  for (long long at = thread / G; at < (A.n_items + 31) / 32 * 32ll; at += threads / G) {  // whole warps
+    const int i = (int)min(at, (long long)A.n_items - 1);
+    const int e0 = A.offsets[i], e1 = A.offsets[i + 1];
+    const bool skip = at >= A.n_items || e1 - e0 > kLong;
     double g = 0.0, h = 0.0;
-    for (int e = offsets[i]; e < e1; ++e) {
-      const int code = partners[e], j = code & 0x7fffffff;
-      const double sign = code < 0 ? -1.0 : 1.0;
-      const double u = sign * (lean(s, ref, (int)i) - lean(s, ref, j));
-      RowDerivative d = pm.derivative(u);
-      const double w = entry_w ? (double)entry_w[e] : 1.0;
-      g += w * sign * d.g;
-      h += w * d.h;
+    if (!skip && e0 < e1) {
+      const double own = lean(A, i);
+      for (int e = e0 + l; e < e1; e += 2 * G) {  // two entries' loads in flight
+        const bool two = e + G < e1;
+        const int2 a = A.entries[e], b = two ? A.entries[e + G] : a;
+        const double wa = A.entry_w ? (double)A.entry_w[e] : 1.0, wb = two && A.entry_w ? (double)A.entry_w[e + G] : 1.0;
+        const double la = lean(A, a.x & 0x7fffffff), lb = two ? lean(A, b.x & 0x7fffffff) : 0.0;
+        add_entry(A, a, wa, own, la, math, &g, &h);
+        if (two) add_entry(A, b, wb, own, lb, math, &g, &h);
+      }
     }
-    grad[i] = (float)g;
-    hess[i] = (float)h;
+#pragma unroll
+    for (int k = G / 2; k > 0; k >>= 1) {
+      g += __shfl_xor_sync(0xffffffffu, g, k);
+      h += __shfl_xor_sync(0xffffffffu, h, k);
+    }
+    if (!skip && l == 0 && A.grad) {
+      A.grad[i] = (float)g;
+      A.hess[i] = (float)h;
+    }
   }
 }
 
+// A block or cluster an item of the list.
 template <typename T>
-__global__ void __launch_bounds__(256) k_preference_pairs(const int2* __restrict__ pairs,
-                                                          const float* __restrict__ pair_w, long long n,
-                                                          const T* __restrict__ s, const T* __restrict__ ref,
-                                                          PairMath pm, T* __restrict__ loss) {
-  for (long long p = (long long)blockIdx.x * blockDim.x + threadIdx.x; p < n; p += (long long)gridDim.x * blockDim.x) {
-    const int2 c = pairs[p];
-    const double w = pair_w ? (double)pair_w[p] : 1.0;
-    loss[p] = w == 0.0 ? (T)0 : (T)(w * pm.loss(lean(s, ref, c.x) - lean(s, ref, c.y)));
+__global__ void __launch_bounds__(kPairThreads) k_preference_long(const PreferenceArgs<T> A, const int* __restrict__ items) {
+  namespace cg = cooperative_groups;
+  __shared__ MathTables tables;
+  __shared__ double sm[2][kPairThreads / 32], sum[2];
+  const TableMath math(tables);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int i = items[blockIdx.x / blocks], e1 = A.offsets[i + 1], step = blocks * kPairThreads;
+  const double own = lean(A, i);
+  double g = 0.0, h = 0.0;
+  for (int e = A.offsets[i] + rank * kPairThreads + threadIdx.x; e < e1; e += 4 * step) {
+    int2 c[4];
+    double other[4], w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) c[q] = e1 - e > q * step ? A.entries[e + q * step] : make_int2(i, -1);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      other[q] = lean(A, c[q].x & 0x7fffffff);
+      w[q] = A.entry_w && c[q].y >= 0 ? (double)A.entry_w[e + q * step] : 1.0;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (c[q].y >= 0) add_entry(A, c[q], w[q], own, other[q], math, &g, &h);
   }
+  for (int k = 16; k > 0; k >>= 1) {
+    g += __shfl_xor_sync(0xffffffffu, g, k);
+    h += __shfl_xor_sync(0xffffffffu, h, k);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    sm[0][threadIdx.x >> 5] = g;
+    sm[1][threadIdx.x >> 5] = h;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    double t = 0.0;
+    for (int k = 0; k < kPairThreads / 32; ++k) t += sm[threadIdx.x][k];
+    sum[threadIdx.x] = t;
+  }
+  if (blocks > 1) cluster.sync();
+  if (rank == 0 && threadIdx.x < 2 && A.grad) {
+    double t = 0.0;
+    for (int k = 0; k < blocks; ++k) t += *cluster.map_shared_rank(&sum[threadIdx.x], k);
+    (threadIdx.x ? A.hess : A.grad)[i] = (float)t;
+  }
+  if (blocks > 1) cluster.sync();  // until the first block has read the sums
+}
+
+template <typename T>
+void launch_preference_long(const PreferenceArgs<T>& A, const int* items, long long n, int blocks, cudaStream_t st) {
+  if (n == 0) return;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)(n * blocks));
+  lc.blockDim = dim3(kPairThreads);
+  lc.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  lc.attrs = attr;
+  lc.numAttrs = blocks > 1 ? 1 : 0;
+  MTB_CUDA_FB(cudaLaunchKernelEx(&lc, k_preference_long<T>, A, items));
+}
+
+template <typename T, int G>
+void launch_preference_items(const PreferenceArgs<T>& A, cudaStream_t st) {
+  const long long blocks = ((long long)A.n_items * G + kPairThreads - 1) / kPairThreads;
+  const unsigned grid = (unsigned)std::min<long long>(blocks, 16ll * multiprocessors());
+  k_preference_items<T, G><<<grid, kPairThreads, 0, st>>>(A);
+  MTB_CUDA_FB(cudaGetLastError());
 }
 
 template <typename T>
 void launch_preference_t(const PreferencePlan& plan, const PreferenceTerms& t, cudaStream_t st) {
-  const PairMath pm = {t.beta, t.smoothing, 1.0 / (2.0 * t.beta), t.kind};
-  const T* s = static_cast<const T*>(t.scores);
-  const T* ref = static_cast<const T*>(t.reference);
-  auto blocks = [](long long n) { return (unsigned)std::min<long long>((n + 255) / 256, 1 << 20); };
-  if (plan.n_items > 0 && t.grad) {
-    k_preference_items<T><<<blocks(plan.n_items), 256, 0, st>>>(plan.offsets, plan.partners, plan.entry_w,
-                                                                plan.n_items, s, ref, pm, t.grad, t.hess);
-    MTB_CUDA_FB(cudaGetLastError());
-  }
-  if (plan.n_pairs > 0 && t.loss) {
-    k_preference_pairs<T><<<blocks(plan.n_pairs), 256, 0, st>>>(plan.pairs, plan.pair_w, plan.n_pairs, s, ref, pm,
-                                                                static_cast<T*>(t.loss));
-    MTB_CUDA_FB(cudaGetLastError());
-  }
+  if (plan.n_items == 0) return;
+  PreferenceArgs<T> A;
+  A.offsets = plan.offsets;
+  A.entries = plan.entries;
+  A.entry_w = plan.entry_w;
+  A.zero_pairs = plan.zero_pairs;
+  A.n_zero = (int)plan.n_zero;
+  A.n_items = (int)plan.n_items;
+  A.s = static_cast<const T*>(t.scores);
+  A.ref = static_cast<const T*>(t.reference);
+  A.pm = {t.beta, t.smoothing, 1.0 / (2.0 * t.beta), t.kind};
+  A.loss = static_cast<T*>(t.loss);
+  A.grad = t.grad;
+  A.hess = t.hess;
+  // long items first: they take longest
+  launch_preference_long(A, plan.huge_items, plan.n_huge, kPairCluster, st);
+  launch_preference_long(A, plan.long_items, plan.n_long, 1, st);
+  // lanes for half of the mean number of pairs, so that most items take two steps
+  const long long mean = plan.n_entries / plan.n_items;
+  if (mean < 4) launch_preference_items<T, 1>(A, st);
+  else if (mean < 16) launch_preference_items<T, 4>(A, st);
+  else if (mean < 48) launch_preference_items<T, 16>(A, st);
+  else launch_preference_items<T, 32>(A, st);
 }
 
 }  // namespace
@@ -1486,74 +1616,139 @@ void launch_policy(const ScoreRows& in, const PolicyTerms& t, const ScoreDerivat
   });
 }
 
-PreferencePlan::~PreferencePlan() {
-  cudaFree(offsets);
-  cudaFree(partners);
-  cudaFree(entry_w);
-  cudaFree(pairs);
-  cudaFree(pair_w);
-}
-
-namespace {
-
-template <typename T>
-T* to_device(const std::vector<T>& v) {
-  T* p = nullptr;
-  MTB_CUDA_FB(cudaMalloc(&p, sizeof(T) * std::max<size_t>(1, v.size())));
-  const cudaError_t e = v.empty() ? cudaSuccess : cudaMemcpy(p, v.data(), sizeof(T) * v.size(), cudaMemcpyHostToDevice);
-  if (e != cudaSuccess) {
-    cudaFree(p);
-    throw std::runtime_error(std::string("CUDA error: ") + cudaGetErrorString(e) + " (preference plan)");
-  }
-  return p;
-}
-
-}  // namespace
+PreferencePlan::~PreferencePlan() { cudaFree(memory); }
 
 void PreferencePlan::check(const int64_t* winners, const int64_t* losers, const float* weights, long long np,
                            long long ni) {
+  int fault = 0;  // the largest of: 1 weight, 2 itself, 3 range
+#pragma omp parallel for schedule(static) reduction(max : fault) if (np > 65536)
   for (long long p = 0; p < np; ++p) {
     const int64_t a = winners[p], b = losers[p];
-    if (a < 0 || a >= ni || b < 0 || b >= ni) throw std::invalid_argument("pair item out of range");
-    if (a == b) throw std::invalid_argument("an item is paired with itself");
-    if (weights && !(weights[p] >= 0.0f && std::isfinite(weights[p])))
-      throw std::invalid_argument("pair weights must be finite and non-negative");
+    if (a < 0 || a >= ni || b < 0 || b >= ni) fault = std::max(fault, 3);
+    else if (a == b) fault = std::max(fault, 2);
+    else if (weights && !(weights[p] >= 0.0f && std::isfinite(weights[p]))) fault = std::max(fault, 1);
   }
+  if (fault == 3) throw std::invalid_argument("pair item out of range");
+  if (fault == 2) throw std::invalid_argument("an item is paired with itself");
+  if (fault == 1) throw std::invalid_argument("pair weights must be finite and non-negative");
 }
 
+// Two passes of a counting sort, both in the pairs' order and on all host
+// threads: pairs into ranges of items, then each range's by item, within a
+// core's cache.
 void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const float* weights, long long np,
                            long long ni) {
-  std::vector<int> off((size_t)ni + 1, 0);
-  std::vector<int2> pr((size_t)np);
-  for (long long p = 0; p < np; ++p) {
-    const int64_t a = winners[p], b = losers[p];
-    pr[p] = make_int2((int)a, (int)b);
-    if (weights && weights[p] == 0.0f) continue;
-    ++off[a + 1];
-    ++off[b + 1];
+  struct Entry {
+    int item;
+    int2 e;
+    float w;
+  };
+  constexpr int kRanges = 256, kMostThreads = 64;
+  const int parts = (int)std::min<long long>(kMostThreads, 1 + np / 16384);
+  const long long range = std::max<long long>(1, (ni + kRanges - 1) / kRanges);
+  std::vector<long long> count((size_t)parts * kRanges, 0), zeros(parts, 0);
+  auto slice = [&](int t) { return np * t / parts; };
+#pragma omp parallel for schedule(static, 1) if (parts > 1)
+  for (int t = 0; t < parts; ++t) {
+    long long* c = &count[(size_t)t * kRanges];
+    for (long long p = slice(t); p < slice(t + 1); ++p) {
+      if (weights && weights[p] == 0.0f) {
+        ++zeros[t];
+        continue;
+      }
+      ++c[winners[p] / range];
+      ++c[losers[p] / range];
+    }
   }
-  for (long long i = 0; i < ni; ++i) off[i + 1] += off[i];
-  n_entries = off[ni];
-  std::vector<int> at(off.begin(), off.end() - 1), part((size_t)n_entries);
-  std::vector<float> ew(weights ? (size_t)n_entries : 0);
-  for (long long p = 0; p < np; ++p) {  // an item's entries stay in the pairs' order
-    if (weights && weights[p] == 0.0f) continue;
-    const int ea = at[pr[p].x]++, eb = at[pr[p].y]++;
-    part[ea] = pr[p].y;
-    part[eb] = pr[p].x | (int)0x80000000;
-    if (weights) ew[ea] = ew[eb] = weights[p];
+  std::vector<long long> start(kRanges + 1, 0), zero_at(parts + 1, 0);
+  long long total = 0;
+  for (int q = 0; q < kRanges; ++q) {
+    start[q] = total;
+    for (int t = 0; t < parts; ++t) {
+      const long long c = count[(size_t)t * kRanges + q];
+      count[(size_t)t * kRanges + q] = total;
+      total += c;
+    }
   }
+  start[kRanges] = total;
+  for (int t = 0; t < parts; ++t) zero_at[t + 1] = zero_at[t] + zeros[t];
+  std::unique_ptr<Entry[]> sorted(new Entry[std::max(1ll, total)]);
+  std::vector<int> zero((size_t)zero_at[parts]), off((size_t)ni + 1);
+  std::unique_ptr<int2[]> ent(new int2[std::max(1ll, total)]);
+  std::unique_ptr<float[]> ew(new float[weights ? std::max(1ll, total) : 1]);
+#pragma omp parallel for schedule(static, 1) if (parts > 1)
+  for (int t = 0; t < parts; ++t) {
+    long long* c = &count[(size_t)t * kRanges];
+    long long z = zero_at[t];
+    for (long long p = slice(t); p < slice(t + 1); ++p) {
+      const int a = (int)winners[p], b = (int)losers[p];
+      const float w = weights ? weights[p] : 1.0f;
+      if (w == 0.0f) {
+        zero[z++] = (int)p;
+        continue;
+      }
+      sorted[c[a / range]++] = {a, make_int2(b, (int)p), w};
+      sorted[c[b / range]++] = {b, make_int2(a | (int)0x80000000, (int)p), w};
+    }
+  }
+#pragma omp parallel for schedule(dynamic, 1) if (parts > 1)
+  for (int q = 0; q < kRanges; ++q) {
+    const long long i0 = std::min(ni, q * range), i1 = std::min(ni, i0 + range);
+    if (i0 >= i1) continue;
+    std::vector<int> at((size_t)(i1 - i0) + 1, 0);
+    for (long long e = start[q]; e < start[q + 1]; ++e) ++at[sorted[e].item - i0 + 1];
+    int sum = (int)start[q];
+    for (long long i = i0; i < i1; ++i) {
+      off[i] = sum;
+      const int n = at[i - i0 + 1];
+      at[i - i0] = sum;
+      sum += n;
+    }
+    for (long long e = start[q]; e < start[q + 1]; ++e) {
+      const int to = at[sorted[e].item - i0]++;
+      ent[to] = sorted[e].e;
+      if (weights) ew[to] = sorted[e].w;
+    }
+  }
+  off[ni] = (int)total;
+  std::vector<int> lng, huge;
+  for (long long i = 0; i < ni; ++i) {
+    const int d = off[i + 1] - off[i];
+    if (d > kHuge) huge.push_back((int)i);
+    else if (d > kLong) lng.push_back((int)i);
+  }
+  // one allocation, each array on 256 bytes
   MTB_CUDA_FB(cudaGetDevice(&device));
+  size_t bytes = 0;
+  struct Copy {
+    const void* from;
+    size_t n, at;
+  };
+  std::vector<Copy> copies;
+  auto add = [&](const void* from, size_t n) {
+    copies.push_back({from, n, bytes});
+    bytes += (n + 255) / 256 * 256;
+    return copies.back().at;
+  };
+  const size_t at_off = add(off.data(), 4 * off.size()), at_ent = add(ent.get(), 8 * (size_t)total),
+               at_w = add(ew.get(), weights ? 4 * (size_t)total : 0), at_zero = add(zero.data(), 4 * zero.size()),
+               at_long = add(lng.data(), 4 * lng.size()), at_huge = add(huge.data(), 4 * huge.size());
+  MTB_CUDA_FB(cudaMalloc(&memory, bytes));
+  char* base = static_cast<char*>(memory);
+  for (const Copy& c : copies)
+    if (c.n) MTB_CUDA_FB(cudaMemcpy(base + c.at, c.from, c.n, cudaMemcpyHostToDevice));
   n_items = ni;
   n_pairs = np;
-  weighted = weights != nullptr;
-  offsets = to_device(off);
-  partners = to_device(part);
-  pairs = to_device(pr);
-  if (weighted) {
-    entry_w = to_device(ew);
-    pair_w = to_device(std::vector<float>(weights, weights + np));
-  }
+  n_entries = total;
+  n_zero = (long long)zero.size();
+  n_long = (long long)lng.size();
+  n_huge = (long long)huge.size();
+  offsets = reinterpret_cast<int*>(base + at_off);
+  entries = reinterpret_cast<int2*>(base + at_ent);
+  entry_w = weights ? reinterpret_cast<float*>(base + at_w) : nullptr;
+  zero_pairs = reinterpret_cast<int*>(base + at_zero);
+  long_items = reinterpret_cast<int*>(base + at_long);
+  huge_items = reinterpret_cast<int*>(base + at_huge);
 }
 
 void launch_preference(const PreferencePlan& plan, const PreferenceTerms& t, cudaStream_t st) {
@@ -1741,7 +1936,7 @@ int32_t mojotrees_b200_preference_plan_create(const int64_t* winners, const int6
     require(out_plan, "null pointer argument");
     require(n_pairs >= 0 && n_items >= 0, "n_pairs and n_items must be non-negative");
     require(n_items < (int64_t)1 << 31, "more than 2^31-1 items");
-    require(n_pairs < (int64_t)1 << 30, "more than 2^30-1 pairs");
+    require(n_pairs < (int64_t)1 << 29, "more than 2^29-1 pairs");  // entry numbers and steps beyond them fit 32 bits
     require(n_pairs == 0 || (winners && losers), "null pointer argument");
     mtb::PreferencePlan::check(winners, losers, weights, n_pairs, n_items);
     require_cuda();

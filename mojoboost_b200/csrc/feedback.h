@@ -60,12 +60,15 @@ void launch_policy(const ScoreRows& in, const PolicyTerms& t, const ScoreDerivat
 struct PreferencePlan {
   int device = 0;
   long long n_items = 0, n_pairs = 0, n_entries = 0;
-  bool weighted = false;
-  int* offsets = nullptr;      // [n_items + 1]
-  int* partners = nullptr;     // [n_entries] the other item, sign bit set where this item lost
-  float* entry_w = nullptr;    // [n_entries] when weighted
-  int2* pairs = nullptr;       // [n_pairs] winner, loser
-  float* pair_w = nullptr;     // [n_pairs] when weighted
+  // Device arrays, all in `memory`.  Pairs of weight 0 have no entries.
+  int* offsets = nullptr;    // [n_items + 1] into the entries
+  int2* entries = nullptr;   // [n_entries] the other item, sign bit set where this item lost; the pair
+  float* entry_w = nullptr;  // [n_entries] weights, or null
+  int* zero_pairs = nullptr;  // pairs of weight 0
+  int* long_items = nullptr;  // items of many pairs, and of very many
+  int* huge_items = nullptr;
+  long long n_zero = 0, n_long = 0, n_huge = 0;
+  void* memory = nullptr;
   PreferencePlan() = default;
   PreferencePlan(const PreferencePlan&) = delete;
   PreferencePlan& operator=(const PreferencePlan&) = delete;
