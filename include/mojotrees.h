@@ -357,20 +357,20 @@ int32_t mojotrees_b200_check_quotients(int64_t n, uint64_t seed, int64_t *out_mi
 /* log softmax(scores)[action] per row (row type [n_rows]), and what its
  * gradient needs (row type [n_rows][2]): the row's maximum, and the sum of
  * exp(score - maximum) less 1 (0 and -1 for a row that takes no part). */
-int32_t mojotrees_b200_action_logprobs(const void* scores, int32_t score_type, int64_t n_rows, int64_t n_classes,
-                                       int64_t row_stride, const void* actions, int32_t action_bytes, void* out_logp,
-                                       void* out_stats, void* stream, MojoTreesError* error);
+int32_t mojotrees_b200_action_logprobs(const void *scores, int32_t score_type, int64_t n_rows, int64_t n_classes,
+                                       int64_t row_stride, const void *actions, int32_t action_bytes, void *out_logp,
+                                       void *out_stats, void *stream, MojoTreesError *error);
 
 /* Derivatives of a loss with respect to the scores from its first and second
  * derivative g, h with respect to the log probabilities (float [n_rows]):
  * with p = softmax(scores), grad = g ([k = action] - p_k) and
  * hess = h ([k = action] - p_k)^2 + |g| p_k (1 - p_k), which is not negative
  * for h >= 0.  hess_logp and out_hess may both be NULL. */
-int32_t mojotrees_b200_action_logprobs_grad(const void* scores, int32_t score_type, int64_t n_rows, int64_t n_classes,
-                                            int64_t row_stride, const void* actions, int32_t action_bytes,
-                                            const void* stats, const float* grad_logp, const float* hess_logp,
-                                            void* out_grad, void* out_hess, int64_t out_stride, void* stream,
-                                            MojoTreesError* error);
+int32_t mojotrees_b200_action_logprobs_grad(const void *scores, int32_t score_type, int64_t n_rows, int64_t n_classes,
+                                            int64_t row_stride, const void *actions, int32_t action_bytes,
+                                            const void *stats, const float *grad_logp, const float *hess_logp,
+                                            void *out_grad, void *out_hess, int64_t out_stride, void *stream,
+                                            MojoTreesError *error);
 
 /* Clipped policy loss of logged decisions, with l the log probability of the
  * row's action, ratio = exp(l - old_logp) and t = ref_logp - l:
@@ -384,12 +384,12 @@ int32_t mojotrees_b200_action_logprobs_grad(const void* scores, int32_t score_ty
  * them from dloss/dl and max(0, the ratio term's d2loss/dl2) + the KL term's;
  * out_hess may be NULL, and both for the loss alone.  A row whose action's
  * score is -inf has log probability -inf and otherwise takes no part. */
-int32_t mojotrees_b200_policy_loss(const void* scores, int32_t score_type, int64_t n_rows, int64_t n_classes,
-                                   int64_t row_stride, const void* actions, int32_t action_bytes,
-                                   const void* advantages, const void* old_logp, const void* ref_logp,
-                                   const void* weights, double clip_low, double clip_high, double kl_coef,
-                                   void* out_loss, void* out_logp, void* out_grad, void* out_hess, int64_t out_stride,
-                                   void* stream, MojoTreesError* error);
+int32_t mojotrees_b200_policy_loss(const void *scores, int32_t score_type, int64_t n_rows, int64_t n_classes,
+                                   int64_t row_stride, const void *actions, int32_t action_bytes,
+                                   const void *advantages, const void *old_logp, const void *ref_logp,
+                                   const void *weights, double clip_low, double clip_high, double kl_coef,
+                                   void *out_loss, void *out_logp, void *out_grad, void *out_hess, int64_t out_stride,
+                                   void *stream, MojoTreesError *error);
 
 /* The pairs of a preference loss, laid out on a device once for any number
  * of calls: item winners[p] was preferred to losers[p] (both in
@@ -398,10 +398,10 @@ int32_t mojotrees_b200_policy_loss(const void* scores, int32_t score_type, int64
  * calls that use it, which may overlap; free it when none is running and no
  * graph holds one. */
 typedef struct MojoTreesPreferencePlan MojoTreesPreferencePlan;
-int32_t mojotrees_b200_preference_plan_create(const int64_t* winners, const int64_t* losers, const float* weights,
+int32_t mojotrees_b200_preference_plan_create(const int64_t *winners, const int64_t *losers, const float *weights,
                                               int64_t n_pairs, int64_t n_items, int32_t gpu_device_id,
-                                              MojoTreesPreferencePlan** out_plan, MojoTreesError* error);
-void mojotrees_b200_preference_plan_free(MojoTreesPreferencePlan* plan);
+                                              MojoTreesPreferencePlan **out_plan, MojoTreesError *error);
+void mojotrees_b200_preference_plan_free(MojoTreesPreferencePlan *plan);
 
 /* Paired preference loss of the items' scores (raw scores or log
  * probabilities of whole answers, double or float [n_items]) relative to a
@@ -416,10 +416,60 @@ void mojotrees_b200_preference_plan_free(MojoTreesPreferencePlan* plan);
  * to its score, in a fixed order; 0 for an item without pairs. */
 #define MOJOTREES_B200_PREFERENCE_LOGISTIC 0
 #define MOJOTREES_B200_PREFERENCE_SQUARED 1
-int32_t mojotrees_b200_preference_loss(const MojoTreesPreferencePlan* plan, const void* scores, const void* reference,
+int32_t mojotrees_b200_preference_loss(const MojoTreesPreferencePlan *plan, const void *scores, const void *reference,
                                        int32_t score_type, double beta, double label_smoothing, int32_t loss_kind,
-                                       void* out_loss, float* out_grad, float* out_hess, void* stream,
-                                       MojoTreesError* error);
+                                       void *out_loss, float *out_grad, float *out_hess, void *stream,
+                                       MojoTreesError *error);
+
+/* Fits whose rounds descend these losses instead of a loss against labels
+ * (objective=preference and objective=policy, which the parameters may name;
+ * other entry points answer them with MOJOTREES_ERROR_UNSUPPORTED).  Host
+ * arrays; data, bins and the other parameters as for mojotrees_train_dense and
+ * mojotrees_b200_train_binned_u8.  The scores start from initial_scores
+ * (double [n_rows][num_class], e.g. another model's raw scores) or, when NULL,
+ * from 0; the model holds what the fit added to them, so its predictions are
+ * added to the initial scores of the rows at hand.  It is saved, loaded and
+ * evaluated as a regression model (one score per row) or a multiclass model
+ * (class scores: the response is each class's probability).  Data-parallel
+ * fits do not cover these objectives.
+ *
+ * Preference: row winners[p] was preferred to row losers[p].  Parameters
+ * preference_beta (1), preference_label_smoothing (0), preference_loss
+ * (logistic, squared).  With num_class > 1 a row stands for the class that
+ * actions (int32 [n_rows]) says it took, and its score is that class's log
+ * probability; else actions is NULL.  reference: a reference model's score or
+ * log probability per row (double [n_rows], NULL: 0).
+ *
+ * Policy: row r took actions[r] in [0, num_class) (-1: it takes no part) with
+ * advantage advantages[r].  Parameters num_class, policy_clip_low (0.2),
+ * policy_clip_high (0.2), policy_kl (0).  old_logp and ref_logp are the log
+ * probabilities of the action under the policy that took it and under the
+ * reference (double [n_rows]; NULL: under the initial scores), weights the
+ * rows' weights (NULL: 1). */
+int32_t mojotrees_b200_train_dense_preference(const double *data, int64_t n_rows, int64_t n_features,
+                                              const int64_t *winners, const int64_t *losers,
+                                              const float *pair_weights, int64_t n_pairs, const int32_t *actions,
+                                              const double *reference, const double *initial_scores,
+                                              const char *parameters, MojoTreesModel **out_model,
+                                              MojoTreesError *error);
+int32_t mojotrees_b200_train_binned_u8_preference(const uint8_t *bins, int64_t n_rows, int64_t n_features,
+                                                  int32_t n_bins, const int32_t *missing_bin,
+                                                  const int32_t *n_categories, const int64_t *winners,
+                                                  const int64_t *losers, const float *pair_weights, int64_t n_pairs,
+                                                  const int32_t *actions, const double *reference,
+                                                  const double *initial_scores, const char *parameters,
+                                                  MojoTreesModel **out_model, MojoTreesError *error);
+int32_t mojotrees_b200_train_dense_policy(const double *data, int64_t n_rows, int64_t n_features,
+                                          const int32_t *actions, const double *advantages, const double *old_logp,
+                                          const double *ref_logp, const double *weights,
+                                          const double *initial_scores, const char *parameters,
+                                          MojoTreesModel **out_model, MojoTreesError *error);
+int32_t mojotrees_b200_train_binned_u8_policy(const uint8_t *bins, int64_t n_rows, int64_t n_features, int32_t n_bins,
+                                              const int32_t *missing_bin, const int32_t *n_categories,
+                                              const int32_t *actions, const double *advantages,
+                                              const double *old_logp, const double *ref_logp, const double *weights,
+                                              const double *initial_scores, const char *parameters,
+                                              MojoTreesModel **out_model, MojoTreesError *error);
 
 #ifdef __cplusplus
 } /* extern "C" */

@@ -11,9 +11,11 @@ from ._capi import (  # noqa: F401
 )
 from ._feedback import (  # noqa: F401
     PreferencePlan, action_logprobs, action_logprobs_grad, policy_loss, preference_loss,
+    train_binned_policy, train_binned_preference, train_dense_policy, train_dense_preference,
 )
 
 __all__ = ["Model", "MojoTreesError", "UnsupportedError", "abi_version", "bin_dense",
            "check_quotients", "gpu_available", "histogram_u8", "lib", "nccl_unique_id", "shared_atomic_peak", "train_binned", "train_csc", "bin_csc",
            "train_binned_dp", "train_dense",
-           "PreferencePlan", "action_logprobs", "action_logprobs_grad", "policy_loss", "preference_loss"]
+           "PreferencePlan", "action_logprobs", "action_logprobs_grad", "policy_loss", "preference_loss",
+           "train_binned_policy", "train_binned_preference", "train_dense_policy", "train_dense_preference"]

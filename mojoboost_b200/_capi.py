@@ -75,6 +75,13 @@ SIGNATURES = {
     "mojotrees_b200_histogram_u8_noalloc": (_I32, [_P, _I64, _I64, _I32, _P, _I64, _P, _I32, _P, _P, _P]),
     "mojotrees_b200_train_binned_u8_dp": (_I32, [_P, _I64, _I64, _I32, _P, _P, _P, _P, ctypes.c_char_p, _P, _I32,
                                                  _I32, _I64, _I64, _P, _P]),
+    "mojotrees_b200_train_dense_preference": (_I32, [_P, _I64, _I64, _P, _P, _P, _I64, _P, _P, _P, ctypes.c_char_p,
+                                                     _P, _P]),
+    "mojotrees_b200_train_binned_u8_preference": (_I32, [_P, _I64, _I64, _I32, _P, _P, _P, _P, _P, _I64, _P, _P, _P,
+                                                         ctypes.c_char_p, _P, _P]),
+    "mojotrees_b200_train_dense_policy": (_I32, [_P, _I64, _I64, _P, _P, _P, _P, _P, _P, ctypes.c_char_p, _P, _P]),
+    "mojotrees_b200_train_binned_u8_policy": (_I32, [_P, _I64, _I64, _I32, _P, _P, _P, _P, _P, _P, _P, _P,
+                                                     ctypes.c_char_p, _P, _P]),
     "mojotrees_b200_action_logprobs": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _I32, _P, _P, _P, _P]),
     "mojotrees_b200_action_logprobs_grad": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _I32, _P, _P, _P, _P, _P, _I64,
                                                    _P, _P]),

@@ -1,7 +1,10 @@
-"""Losses that learn from feedback instead of labels, on device scores.
+"""Losses that learn from feedback instead of labels: fits, and their losses on
+device scores.
 
-The losses behind the policy and preference fits, for callers whose scores
-are torch tensors on a CUDA device: the log probabilities of taken classes,
+train_dense_policy and train_dense_preference (and their train_binned_ twins)
+fit trees to logged decisions with advantages and to pairs of which one row
+was preferred.  The other calls are the losses behind them, for callers whose
+scores are torch tensors on a CUDA device: the log probabilities of taken classes,
 the clipped policy loss of logged decisions and the paired preference loss,
 each with its first and second derivative (include/mojotrees.h has the
 formulas).  Calls run on torch's current stream of the scores' device, do not
@@ -9,14 +12,14 @@ wait for the device and can be captured into a CUDA graph.
 
 A row takes no part, with outputs 0, when its action is negative, its weight
 is 0 or every score is -inf; an action of n_classes or more gives NaN there.
-torch is imported by the first call.
+torch is imported by the first call on device scores.
 """
 import ctypes
 
 import numpy as np
 
 from . import _capi
-from ._capi import MojoTreesError, _Err, _ptr, lib
+from ._capi import Model, MojoTreesError, _Err, _ptr, lib, params_string
 
 PREFERENCE_LOSSES = {"logistic": 0, "squared": 1}
 
@@ -184,3 +187,124 @@ def preference_loss(plan, scores, reference=None, beta=1.0, label_smoothing=0.0,
                                                  PREFERENCE_LOSSES[loss], out.data_ptr(), grad.data_ptr(),
                                                  hess.data_ptr(), _stream(torch, dev), e.h))
     return out, grad, hess
+
+
+def _row_array(name, v, shape, dtype=np.float64):
+    if v is None:
+        return None
+    v = np.asarray(v)
+    if dtype != np.float64 and v.dtype.kind not in "iu" and v.size:
+        raise _invalid(f"{name} must be integers, got {v.dtype}")
+    if v.shape != shape:
+        raise _invalid(f"{name} must have shape {shape}, got {v.shape}")
+    if dtype == np.int32 and v.size and (v.min() < -2 ** 31 or v.max() >= 2 ** 31):
+        raise _invalid(f"{name} must fit 32 bits")
+    return np.ascontiguousarray(v, dtype=dtype)
+
+
+def _scores_array(v, n):
+    if v is None:
+        return None
+    v = np.asarray(v)
+    return _row_array("initial_scores", v, (n,) if v.ndim == 1 else (n, v.shape[-1]))
+
+
+def _num_class(params):
+    """num_class of the parameters, 1 when they do not give it."""
+    for token in params_string(params).decode().split():
+        key, _, value = token.partition("=")
+        if key.lower() in ("num_class", "num_classes") and value.lstrip("-").isdigit():
+            return int(value)
+    return 1
+
+
+def _check_initial(initial, params):
+    k = _num_class(params)
+    if initial is not None and (1 if initial.ndim == 1 else initial.shape[1]) != max(k, 1):
+        raise _invalid(f"initial_scores must have num_class = {max(k, 1)} values a row, got shape {initial.shape}")
+    return initial
+
+
+def _dense(X):
+    X = np.asarray(X, dtype=np.float64)
+    if X.ndim != 2:
+        raise _invalid(f"X must be [n_rows, n_features], got shape {X.shape}")
+    n, f = X.shape
+    Xc = np.asfortranarray(X)
+    return n, (Xc.ctypes.data_as(ctypes.c_void_p), n, f), Xc
+
+
+def _binned(bins_fm, n_bins, missing_bin, n_categories):
+    bins = np.ascontiguousarray(bins_fm, dtype=np.uint8)
+    if bins.ndim != 2:
+        raise _invalid(f"bins must be [n_features, n_rows], got shape {bins.shape}")
+    f, n = bins.shape
+    mb = None if missing_bin is None else _row_array("missing_bin", missing_bin, (f,), np.int32)
+    nc = None if n_categories is None else _row_array("n_categories", n_categories, (f,), np.int32)
+    return n, (_ptr(bins), n, f, n_bins, _ptr(mb), _ptr(nc)), (bins, mb, nc)
+
+
+def _fit(fn, data, keep, args, params):
+    e = _Err()
+    h = ctypes.c_void_p()
+    e.check(fn(*data, *args, params_string(params), ctypes.byref(h), e.h))
+    del keep
+    return Model(h.value)
+
+
+def _preference_args(n, winners, losers, pair_weights, actions, reference, initial_scores, params):
+    w, l = _index_array("winners", winners), _index_array("losers", losers)
+    pw = None if pair_weights is None else np.ascontiguousarray(pair_weights, dtype=np.float32)
+    if w.ndim != 1 or w.shape != l.shape or (pw is not None and pw.shape != w.shape):
+        raise _invalid("winners, losers and pair_weights must be one-dimensional and of one length")
+    a = _row_array("actions", actions, (n,), np.int32)
+    r = _row_array("reference", reference, (n,))
+    s = _check_initial(_scores_array(initial_scores, n), params)
+    return (_ptr(w), _ptr(l), _ptr(pw), w.size, _ptr(a), _ptr(r), _ptr(s)), (w, l, pw, a, r, s)
+
+
+def _policy_args(n, actions, advantages, old_logp, ref_logp, weights, initial_scores, params):
+    a = _row_array("actions", actions, (n,), np.int32)
+    rows = [_row_array(name, v, (n,)) for name, v in (("advantages", advantages), ("old_logp", old_logp),
+                                                      ("ref_logp", ref_logp), ("weights", weights))]
+    s = _check_initial(_scores_array(initial_scores, n), params)
+    return (_ptr(a), *[_ptr(v) for v in rows], _ptr(s)), (a, rows, s)
+
+
+def train_dense_preference(X, winners, losers, params=None, pair_weights=None, actions=None, reference=None,
+                           initial_scores=None):
+    """Fit a float64 matrix [n_rows, n_features] to pairs of rows, row
+    winners[p] preferred to row losers[p].  With num_class > 1 in params a row
+    stands for the class actions says it took.  The model adds to
+    initial_scores ([n_rows] or [n_rows, num_class]; default 0)."""
+    n, data, keep = _dense(X)
+    args, more = _preference_args(n, winners, losers, pair_weights, actions, reference, initial_scores, params)
+    return _fit(lib().mojotrees_b200_train_dense_preference, data, (keep, more), args, params)
+
+
+def train_binned_preference(bins_fm, n_bins, winners, losers, params=None, pair_weights=None, actions=None,
+                            reference=None, initial_scores=None, missing_bin=None, n_categories=None):
+    """train_dense_preference on feature-major uint8 bins [n_features, n_rows]."""
+    n, data, keep = _binned(bins_fm, n_bins, missing_bin, n_categories)
+    args, more = _preference_args(n, winners, losers, pair_weights, actions, reference, initial_scores, params)
+    return _fit(lib().mojotrees_b200_train_binned_u8_preference, data, (keep, more), args, params)
+
+
+def train_dense_policy(X, actions, advantages, params=None, old_logp=None, ref_logp=None, weights=None,
+                       initial_scores=None):
+    """Fit a policy over params' num_class classes to logged decisions: row r
+    took actions[r] (-1: takes no part) with advantage advantages[r].
+    old_logp and ref_logp are the actions' log probabilities under the policy
+    that took them and under the reference; by default both are the policy
+    that the fit starts from, softmax(initial_scores [n_rows, num_class])."""
+    n, data, keep = _dense(X)
+    args, more = _policy_args(n, actions, advantages, old_logp, ref_logp, weights, initial_scores, params)
+    return _fit(lib().mojotrees_b200_train_dense_policy, data, (keep, more), args, params)
+
+
+def train_binned_policy(bins_fm, n_bins, actions, advantages, params=None, old_logp=None, ref_logp=None, weights=None,
+                        initial_scores=None, missing_bin=None, n_categories=None):
+    """train_dense_policy on feature-major uint8 bins [n_features, n_rows]."""
+    n, data, keep = _binned(bins_fm, n_bins, missing_bin, n_categories)
+    args, more = _policy_args(n, actions, advantages, old_logp, ref_logp, weights, initial_scores, params)
+    return _fit(lib().mojotrees_b200_train_binned_u8_policy, data, (keep, more), args, params)

@@ -29,6 +29,7 @@
 #include "model.h"
 #include "predict.h"
 #include "device_binning.h"
+#include "feedback.h"
 #include "trainer.h"
 
 struct MojoTreesError {
@@ -113,6 +114,12 @@ const std::vector<std::pair<std::string, std::vector<std::string>>>& param_table
       {"verbosity", {"verbose"}},
       {"seed", {"random_seed", "random_state"}},
       {"num_threads", {"num_thread", "nthread", "nthreads", "n_jobs"}},
+      {"preference_beta", {}},
+      {"preference_label_smoothing", {}},
+      {"preference_loss", {}},
+      {"policy_clip_low", {}},
+      {"policy_clip_high", {}},
+      {"policy_kl", {}},
       {"keep_training_scores", {}},
       {"profile_phases", {}},
       {"profile_histogram", {}},
@@ -173,6 +180,7 @@ TrainConfig parse_config(const char* params, bool need_training) {
     const std::string& v = p.second;
     if (k == "objective") {
       std::string o = lower(v);
+      c.objective_given = true;
       if (o == "regression" || o == "regression_l2" || o == "l2" || o == "mse" || o == "mean_squared_error" ||
           o == "rmse" || o == "root_mean_squared_error" || o == "l2_root")
         c.objective = mtb::OBJECTIVE_L2;
@@ -180,6 +188,10 @@ TrainConfig parse_config(const char* params, bool need_training) {
         c.objective = mtb::OBJECTIVE_BINARY;
       else if (o == "multiclass" || o == "softmax")
         c.objective = mtb::OBJECTIVE_MULTICLASS;
+      else if (o == "preference")
+        c.objective = mtb::OBJECTIVE_PREFERENCE;
+      else if (o == "policy")
+        c.objective = mtb::OBJECTIVE_POLICY;
       else
         throw mtb::Unsupported("objective '" + v + "' is not covered by the device path (regression, binary, multiclass are)");
     } else if (k == "num_class") c.num_class = (int)to_int(k, v);
@@ -240,6 +252,27 @@ TrainConfig parse_config(const char* params, bool need_training) {
       if (!(b == "gbdt" || b == "gbrt")) throw mtb::Unsupported("boosting '" + v + "' is not covered by the device path");
     } else if (k == "data_sample_strategy") {
       if (lower(v) != "bagging") throw mtb::Unsupported("data_sample_strategy '" + v + "' (GOSS) is not covered by the device path");
+    } else if (k == "preference_beta") {
+      c.preference_beta = to_double(k, v);
+      if (!(c.preference_beta > 0.0 && std::isfinite(c.preference_beta))) throw InvalidArgument("preference_beta must be positive");
+    } else if (k == "preference_label_smoothing") {
+      c.preference_label_smoothing = to_double(k, v);
+      if (!(c.preference_label_smoothing >= 0.0 && c.preference_label_smoothing <= 0.5))
+        throw InvalidArgument("preference_label_smoothing must be in [0, 0.5]");
+    } else if (k == "preference_loss") {
+      const std::string d = lower(v);
+      if (d == "logistic") c.preference_loss = 0;
+      else if (d == "squared") c.preference_loss = 1;
+      else throw InvalidArgument("preference_loss must be logistic or squared, got '" + v + "'");
+    } else if (k == "policy_clip_low") {
+      c.policy_clip_low = to_double(k, v);
+      if (!(c.policy_clip_low >= 0.0 && c.policy_clip_low <= 1.0)) throw InvalidArgument("policy_clip_low must be in [0, 1]");
+    } else if (k == "policy_clip_high") {
+      c.policy_clip_high = to_double(k, v);
+      if (!(c.policy_clip_high >= 0.0)) throw InvalidArgument("policy_clip_high must be non-negative");
+    } else if (k == "policy_kl") {
+      c.policy_kl = to_double(k, v);
+      if (!(c.policy_kl >= 0.0 && std::isfinite(c.policy_kl))) throw InvalidArgument("policy_kl must be finite and non-negative");
     } else if (k == "keep_training_scores") c.keep_training_scores = to_bool(k, v);
     else if (k == "profile_phases") c.profile_phases = to_bool(k, v);
     else if (k == "profile_histogram") c.profile_histogram = to_bool(k, v);
@@ -255,7 +288,9 @@ TrainConfig parse_config(const char* params, bool need_training) {
     if (c.lambda_l2 < 0.0 || c.lambda_l1 < 0.0) throw InvalidArgument("lambda_l1 and lambda_l2 must be non-negative");
     if (c.objective == mtb::OBJECTIVE_MULTICLASS && c.num_class < 2)
       throw InvalidArgument("multiclass needs num_class >= 2");
-    if (c.objective != mtb::OBJECTIVE_MULTICLASS) c.num_class = 1;
+    if (c.objective < mtb::OBJECTIVE_MULTICLASS) c.num_class = 1;
+    if (c.preference_loss == 1 && c.preference_label_smoothing > 0.0)
+      throw InvalidArgument("preference_label_smoothing needs preference_loss=logistic");
   }
   return c;
 }
@@ -399,10 +434,15 @@ int32_t train_binned(const uint8_t* bins, int64_t n_rows, int64_t n_features, in
                      const std::vector<int>& missing, const std::vector<int>& ncats, const double* labels,
                      const TrainConfig& cfg, MojoTreesModel** out_model, const mtb::BinMapper* mapper,
                      mtb::Collective* coll = nullptr, int64_t row_offset = 0, int64_t n_rows_global = 0,
-                     const double* dense = nullptr) {
-  for (int64_t r = 0; r < n_rows; ++r)
-    if (!std::isfinite(labels[r])) throw InvalidArgument("labels must be finite");
+                     const double* dense = nullptr, const mtb::Feedback* feedback = nullptr) {
+  if (!feedback && cfg.objective >= mtb::OBJECTIVE_PREFERENCE)
+    throw mtb::Unsupported("objectives preference and policy learn from feedback, not labels: use the "
+                           "mojotrees_b200_train_*_preference and _policy entry points");
+  if (!feedback)
+    for (int64_t r = 0; r < n_rows; ++r)
+      if (!std::isfinite(labels[r])) throw InvalidArgument("labels must be finite");
   mtb::BinnedInput in{bins, n_rows, (int)n_features, n_bins, missing.data(), ncats.data(), labels};
+  in.feedback = feedback;
   in.dense_fm = dense;
   in.mapper = dense ? mapper : nullptr;
   in.coll = coll;
@@ -434,6 +474,120 @@ int32_t train_binned(const uint8_t* bins, int64_t n_rows, int64_t n_features, in
   }
   *out_model = h.release();
   return MOJOTREES_OK;
+}
+
+// Checks a feedback fit's per-row values: finite, and from `least` on.
+void check_values(const char* name, const double* v, int64_t n, double least = -HUGE_VAL) {
+  if (!v) return;
+  bool ok = true;
+#pragma omp parallel for schedule(static) reduction(&& : ok)
+  for (int64_t i = 0; i < n; ++i) ok = ok && std::isfinite(v[i]) && v[i] >= least;
+  if (!ok) throw InvalidArgument(std::string(name) + (least == 0.0 ? " must be finite and non-negative" : " must be finite"));
+}
+
+void check_actions(const int32_t* actions, int64_t n, int least, int num_class) {
+  bool ok = true;
+#pragma omp parallel for schedule(static) reduction(&& : ok)
+  for (int64_t i = 0; i < n; ++i) ok = ok && actions[i] >= least && actions[i] < num_class;
+  if (!ok) throw InvalidArgument("actions must be in " + std::to_string(least) + "..num_class-1");
+}
+
+// The configuration of a fit of `objective`, which the parameters may name.
+TrainConfig feedback_config(const char* parameters, int objective, const char* name) {
+  TrainConfig c = parse_config(parameters, true);
+  if (c.objective_given && c.objective != objective)
+    throw InvalidArgument(std::string("this entry point trains objective=") + name);
+  // without a name the defaults were another objective's
+  if (!c.objective_given) c = parse_config((std::string(parameters ? parameters : "") + " objective=" + name).c_str(), true);
+  return c;
+}
+
+mtb::Feedback preference_feedback(const TrainConfig& cfg, int64_t n_rows, const int64_t* winners,
+                                  const int64_t* losers, const float* pair_weights, int64_t n_pairs,
+                                  const int32_t* actions, const double* reference, const double* initial_scores) {
+  if (!winners || !losers) throw InvalidArgument("null pointer argument");
+  if (n_pairs < 1) throw InvalidArgument("n_pairs must be positive");
+  if (n_rows >= (int64_t)1 << 31) throw mtb::Unsupported("more than 2^31-1 rows on one device");
+  if (n_pairs >= (int64_t)1 << 29) throw InvalidArgument("more than 2^29-1 pairs");
+  if (cfg.num_class > 1 && !actions) throw InvalidArgument("preference with num_class > 1 needs the actions taken");
+  if (cfg.num_class <= 1 && actions) throw InvalidArgument("actions need num_class > 1");
+  try {
+    mtb::PreferencePlan::check(winners, losers, pair_weights, n_pairs, n_rows);
+  } catch (const std::invalid_argument& e) {
+    throw InvalidArgument(e.what());
+  }
+  if (actions) check_actions(actions, n_rows, 0, cfg.num_class);
+  check_values("reference", reference, n_rows);
+  check_values("initial_scores", initial_scores, n_rows * (actions ? cfg.num_class : 1));
+  mtb::Feedback f;
+  f.actions = actions;
+  f.initial = initial_scores;
+  f.winners = winners;
+  f.losers = losers;
+  f.pair_weights = pair_weights;
+  f.n_pairs = n_pairs;
+  f.reference = reference;
+  return f;
+}
+
+mtb::Feedback policy_feedback(const TrainConfig& cfg, int64_t n_rows, const int32_t* actions,
+                              const double* advantages, const double* old_logp, const double* ref_logp,
+                              const double* weights, const double* initial_scores) {
+  if (!actions || !advantages) throw InvalidArgument("null pointer argument");
+  if (cfg.num_class < 2) throw InvalidArgument("policy needs num_class >= 2");
+  check_actions(actions, n_rows, -1, cfg.num_class);
+  check_values("advantages", advantages, n_rows);
+  check_values("old_logp", old_logp, n_rows);
+  check_values("ref_logp", ref_logp, n_rows);
+  check_values("weights", weights, n_rows, 0.0);
+  check_values("initial_scores", initial_scores, n_rows * cfg.num_class);
+  mtb::Feedback f;
+  f.actions = actions;
+  f.initial = initial_scores;
+  f.advantages = advantages;
+  f.old_logp = old_logp;
+  f.ref_logp = ref_logp;
+  f.weights = weights;
+  return f;
+}
+
+// A feedback fit on a float64 matrix, binned as mojotrees_train_dense does.
+int32_t train_dense_feedback(const double* data, int64_t n_rows, int64_t n_features, const TrainConfig& cfg,
+                             const mtb::Feedback& feedback, MojoTreesModel** out_model) {
+  auto t0 = std::chrono::steady_clock::now();
+  mtb::BinMapper mapper = mtb::fit_bins(data, n_rows, (int)n_features, cfg.binning);
+  const double bin_s = std::chrono::duration<double>(std::chrono::steady_clock::now() - t0).count();
+  std::vector<int> ncats(n_features, -1);
+  for (int f = 0; f < n_features; ++f)
+    if (mapper.is_cat[f]) ncats[f] = mapper.n_categories(f);
+  int32_t rc = train_binned(nullptr, n_rows, n_features, mapper.n_bins, mapper.missing_bin, ncats, nullptr, cfg,
+                            out_model, &mapper, nullptr, 0, 0, data, &feedback);
+  if (rc == MOJOTREES_OK && *out_model) (*out_model)->m.stats.binning_seconds = bin_s;
+  return rc;
+}
+
+int32_t train_binned_feedback(const uint8_t* bins, int64_t n_rows, int64_t n_features, int32_t n_bins,
+                              const int32_t* missing_bin, const int32_t* n_categories, const TrainConfig& cfg,
+                              const mtb::Feedback& feedback, MojoTreesModel** out_model) {
+  std::vector<int> missing(n_features, -1), ncats(n_features, -1);
+  for (int64_t f = 0; f < n_features; ++f) {
+    if (missing_bin) missing[f] = missing_bin[f];
+    if (n_categories) ncats[f] = n_categories[f];
+    if (missing[f] >= n_bins) throw InvalidArgument("missing_bin out of range");
+  }
+  return train_binned(bins, n_rows, n_features, n_bins, missing, ncats, nullptr, cfg, out_model, nullptr, nullptr, 0,
+                      0, nullptr, &feedback);
+}
+
+void check_dense(const double* data, int64_t n_rows, int64_t n_features, MojoTreesModel** out_model) {
+  if (!data || !out_model) throw InvalidArgument("null pointer argument");
+  if (n_rows < 1 || n_features < 1) throw InvalidArgument("n_rows and n_features must be positive");
+}
+
+void check_binned(const uint8_t* bins, int64_t n_rows, int64_t n_features, int32_t n_bins, MojoTreesModel** out_model) {
+  if (!bins || !out_model) throw InvalidArgument("null pointer argument");
+  if (n_rows < 1 || n_features < 1) throw InvalidArgument("n_rows and n_features must be positive");
+  if (n_bins < 2 || n_bins > 256) throw InvalidArgument("n_bins must be in [2, 256]");
 }
 
 }  // namespace
@@ -496,6 +650,68 @@ int32_t mojotrees_b200_train_binned_u8(const uint8_t* bins, int64_t n_rows, int6
       if (missing[f] >= n_bins) throw InvalidArgument("missing_bin out of range");
     }
     return train_binned(bins, n_rows, n_features, n_bins, missing, ncats, labels, cfg, out_model, nullptr);
+  });
+}
+
+int32_t mojotrees_b200_train_dense_preference(const double* data, int64_t n_rows, int64_t n_features,
+                                              const int64_t* winners, const int64_t* losers,
+                                              const float* pair_weights, int64_t n_pairs, const int32_t* actions,
+                                              const double* reference, const double* initial_scores,
+                                              const char* parameters, MojoTreesModel** out_model,
+                                              MojoTreesError* error) {
+  return guarded(error, [&]() -> int32_t {
+    check_dense(data, n_rows, n_features, out_model);
+    const TrainConfig cfg = feedback_config(parameters, mtb::OBJECTIVE_PREFERENCE, "preference");
+    return train_dense_feedback(data, n_rows, n_features, cfg,
+                                preference_feedback(cfg, n_rows, winners, losers, pair_weights, n_pairs, actions,
+                                                    reference, initial_scores),
+                                out_model);
+  });
+}
+
+int32_t mojotrees_b200_train_binned_u8_preference(const uint8_t* bins, int64_t n_rows, int64_t n_features,
+                                                  int32_t n_bins, const int32_t* missing_bin,
+                                                  const int32_t* n_categories, const int64_t* winners,
+                                                  const int64_t* losers, const float* pair_weights, int64_t n_pairs,
+                                                  const int32_t* actions, const double* reference,
+                                                  const double* initial_scores, const char* parameters,
+                                                  MojoTreesModel** out_model, MojoTreesError* error) {
+  return guarded(error, [&]() -> int32_t {
+    check_binned(bins, n_rows, n_features, n_bins, out_model);
+    const TrainConfig cfg = feedback_config(parameters, mtb::OBJECTIVE_PREFERENCE, "preference");
+    return train_binned_feedback(bins, n_rows, n_features, n_bins, missing_bin, n_categories, cfg,
+                                 preference_feedback(cfg, n_rows, winners, losers, pair_weights, n_pairs, actions,
+                                                     reference, initial_scores),
+                                 out_model);
+  });
+}
+
+int32_t mojotrees_b200_train_dense_policy(const double* data, int64_t n_rows, int64_t n_features,
+                                          const int32_t* actions, const double* advantages, const double* old_logp,
+                                          const double* ref_logp, const double* weights,
+                                          const double* initial_scores, const char* parameters,
+                                          MojoTreesModel** out_model, MojoTreesError* error) {
+  return guarded(error, [&]() -> int32_t {
+    check_dense(data, n_rows, n_features, out_model);
+    const TrainConfig cfg = feedback_config(parameters, mtb::OBJECTIVE_POLICY, "policy");
+    return train_dense_feedback(
+        data, n_rows, n_features, cfg,
+        policy_feedback(cfg, n_rows, actions, advantages, old_logp, ref_logp, weights, initial_scores), out_model);
+  });
+}
+
+int32_t mojotrees_b200_train_binned_u8_policy(const uint8_t* bins, int64_t n_rows, int64_t n_features, int32_t n_bins,
+                                              const int32_t* missing_bin, const int32_t* n_categories,
+                                              const int32_t* actions, const double* advantages,
+                                              const double* old_logp, const double* ref_logp, const double* weights,
+                                              const double* initial_scores, const char* parameters,
+                                              MojoTreesModel** out_model, MojoTreesError* error) {
+  return guarded(error, [&]() -> int32_t {
+    check_binned(bins, n_rows, n_features, n_bins, out_model);
+    const TrainConfig cfg = feedback_config(parameters, mtb::OBJECTIVE_POLICY, "policy");
+    return train_binned_feedback(
+        bins, n_rows, n_features, n_bins, missing_bin, n_categories, cfg,
+        policy_feedback(cfg, n_rows, actions, advantages, old_logp, ref_logp, weights, initial_scores), out_model);
   });
 }
 

@@ -1572,7 +1572,7 @@ void launch_preference_t(const PreferencePlan& plan, const PreferenceTerms& t, c
 
 }  // namespace
 
-void launch_logprobs(const ScoreRows& in, void* logp, void* stats, cudaStream_t st) {
+int launch_logprobs(const ScoreRows& in, void* logp, void* stats, cudaStream_t st) {
   by_type(in.type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     RowArgs<T> A = row_args<T>(in);
@@ -1580,9 +1580,10 @@ void launch_logprobs(const ScoreRows& in, void* logp, void* stats, cudaStream_t 
     A.stats = static_cast<typename Types<T>::Row*>(stats);
     launch_rows_t<T, ROW_LOGPROBS>(A, st);
   });
+  return in.n > 0 ? 1 : 0;
 }
 
-void launch_logprobs_grad(const ScoreRows& in, const void* stats, const float* grad_logp, const float* hess_logp,
+int launch_logprobs_grad(const ScoreRows& in, const void* stats, const float* grad_logp, const float* hess_logp,
                           const ScoreDerivatives& out, cudaStream_t st) {
   by_type(in.type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
@@ -1593,9 +1594,10 @@ void launch_logprobs_grad(const ScoreRows& in, const void* stats, const float* g
     set_out(A, out);
     launch_rows_t<T, ROW_BACK>(A, st);
   });
+  return in.n > 0 ? 1 : 0;
 }
 
-void launch_policy(const ScoreRows& in, const PolicyTerms& t, const ScoreDerivatives& out, cudaStream_t st) {
+int launch_policy(const ScoreRows& in, const PolicyTerms& t, const ScoreDerivatives& out, cudaStream_t st) {
   by_type(in.type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     using Row = typename Types<T>::Row;
@@ -1614,6 +1616,7 @@ void launch_policy(const ScoreRows& in, const PolicyTerms& t, const ScoreDerivat
     set_out(A, out);
     launch_rows_t<T, ROW_POLICY>(A, st);
   });
+  return in.n > 0 ? 1 : 0;
 }
 
 PreferencePlan::~PreferencePlan() { cudaFree(memory); }
@@ -1751,9 +1754,10 @@ void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const 
   huge_items = reinterpret_cast<int*>(base + at_huge);
 }
 
-void launch_preference(const PreferencePlan& plan, const PreferenceTerms& t, cudaStream_t st) {
+int launch_preference(const PreferencePlan& plan, const PreferenceTerms& t, cudaStream_t st) {
   if (t.type == SCORE_F64) launch_preference_t<double>(plan, t, st);
   else launch_preference_t<float>(plan, t, st);
+  return plan.n_items > 0 ? 1 + (plan.n_huge > 0 ? 1 : 0) + (plan.n_long > 0 ? 1 : 0) : 0;
 }
 
 }  // namespace mtb

@@ -49,11 +49,12 @@ struct PolicyTerms {
   void* logp;  // may be null
 };
 
-void launch_logprobs(const ScoreRows& in, void* logp, void* stats, cudaStream_t st);
-void launch_logprobs_grad(const ScoreRows& in, const void* stats, const float* grad_logp, const float* hess_logp,
+// Each launcher returns how many kernels it launched.
+int launch_logprobs(const ScoreRows& in, void* logp, void* stats, cudaStream_t st);
+int launch_logprobs_grad(const ScoreRows& in, const void* stats, const float* grad_logp, const float* hess_logp,
                           const ScoreDerivatives& out, cudaStream_t st);
 // out.grad null: the loss alone.
-void launch_policy(const ScoreRows& in, const PolicyTerms& t, const ScoreDerivatives& out, cudaStream_t st);
+int launch_policy(const ScoreRows& in, const PolicyTerms& t, const ScoreDerivatives& out, cudaStream_t st);
 
 // The pairs of a preference loss, laid out on a device per item, so that an
 // item's derivatives are one sum in a fixed order (no atomics).
@@ -94,6 +95,6 @@ struct PreferenceTerms {
   float* hess;   // [n_items]
 };
 
-void launch_preference(const PreferencePlan& plan, const PreferenceTerms& t, cudaStream_t st);
+int launch_preference(const PreferencePlan& plan, const PreferenceTerms& t, cudaStream_t st);
 
 }  // namespace mtb

@@ -227,6 +227,31 @@ __global__ void __launch_bounds__(1024) k_grad_softmax(const double* __restrict_
   }
 }
 
+// Derivatives that a feedback loss left in g32, h32: the hessian's floor, and
+// the same partial/maximum side outputs as k_grad.
+__global__ void __launch_bounds__(1024) k_grad_given(const float* __restrict__ g32, float* __restrict__ h32,
+                                                     long long n, int mode, double* __restrict__ part_g,
+                                                     double* __restrict__ part_h, RoundScales* sc) {
+  __shared__ double sm[32];
+  long long r = (long long)blockIdx.x * 1024 + threadIdx.x;
+  double g = 0.0, h = 0.0;
+  if (r < n) {
+    g = (double)g32[r];
+    float hh = h32[r];
+    if (hh < 1e-16f) h32[r] = hh = 1e-16f;
+    h = (double)hh;
+    if (g != g || h != h) g = INFINITY;  // the maxima would pass over a NaN; the host refuses infinite totals
+  }
+  if (mode == MODE_FIXED) {
+    double sg = block_pairwise_1024(fabs(g), sm);
+    if (threadIdx.x == 0) part_g[blockIdx.x] = sg;
+    double sh = block_pairwise_1024(fabs(h), sm);
+    if (threadIdx.x == 0) part_h[blockIdx.x] = sh;
+  } else {
+    block_max_to(fabs(g), fabs(h), sm, sc);
+  }
+}
+
 // One level of the pairwise reduction of block partials (1024 -> 1).
 __global__ void __launch_bounds__(1024) k_pairwise_level(const double* __restrict__ in_g, const double* __restrict__ in_h,
                                                          long long n, double* __restrict__ out_g,

@@ -28,10 +28,20 @@ struct HostNode {
   long long count;
 };
 
-enum ObjectiveKind { OBJECTIVE_L2 = 0, OBJECTIVE_BINARY = 1, OBJECTIVE_MULTICLASS = 2 };
+// The objectives from OBJECTIVE_PREFERENCE on learn from feedback instead of
+// labels (BinnedInput::feedback).  They are training objectives only: a model
+// keeps OBJECTIVE_L2 (one score per row) or OBJECTIVE_MULTICLASS instead.
+enum ObjectiveKind {
+  OBJECTIVE_L2 = 0,
+  OBJECTIVE_BINARY = 1,
+  OBJECTIVE_MULTICLASS = 2,
+  OBJECTIVE_PREFERENCE = 3,
+  OBJECTIVE_POLICY = 4
+};
 
 struct TrainConfig {
   int objective = OBJECTIVE_L2;
+  bool objective_given = false;
   int num_class = 1;
   int num_iterations = 100;
   double learning_rate = 0.1;
@@ -53,6 +63,12 @@ struct TrainConfig {
   int gpu_device_id = -1;      // -1: current device
   double dp_timeout_seconds = 300.0;
   bool hist_int64 = false;     // fixed-point histograms with the 2^52 bound and Int64 cells  // data-parallel fits: bound of every wait on the other ranks
+  double preference_beta = 1.0;
+  double preference_label_smoothing = 0.0;
+  int preference_loss = 0;  // PreferenceKind
+  double policy_clip_low = 0.2;
+  double policy_clip_high = 0.2;
+  double policy_kl = 0.0;
   bool keep_training_scores = false;
   bool profile_phases = false;    // CUDA events around every kernel phase
   bool profile_histogram = false; // CUDA events around the histogram launches only

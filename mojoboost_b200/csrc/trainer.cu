@@ -27,6 +27,7 @@
 #include "sparse_hist.cuh"
 #include "collective.h"
 #include "device_binning.h"
+#include "feedback.h"
 #include "trainer.h"
 
 namespace mtb {
@@ -208,8 +209,10 @@ void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
     throw Unsupported("num_leaves must be in [2, " + std::to_string(kMaxLeaves) + "] on the device path");
   if (cfg.feature_fraction <= 0.0 || cfg.feature_fraction > 1.0)
     throw std::runtime_error("feature_fraction must be in (0, 1]");
-  const int K = cfg.objective == OBJECTIVE_MULTICLASS ? cfg.num_class : 1;
-  if (cfg.objective == OBJECTIVE_MULTICLASS && (K < 2 || K > 64))
+  const Feedback* fb = in.feedback;
+  if (fb && in.coll) throw Unsupported("feedback objectives are not covered by data-parallel fits");
+  const int K = cfg.objective == OBJECTIVE_MULTICLASS || (fb && fb->actions) ? cfg.num_class : 1;
+  if ((cfg.objective == OBJECTIVE_MULTICLASS || (fb && fb->actions)) && (K < 2 || K > 64))
     throw Unsupported("num_class must be in [2, 64] on the device path");
   const int mode = cfg.use_quantized_grad ? MODE_QUANT : MODE_FIXED;
   // fixed point with the 2^52 bound and Int64 cells (gpu_histogram_precision=int64)
@@ -265,10 +268,12 @@ void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
   }
   DevBuf<double> d_y, d_raw, d_prob;
   mark("bins uploaded, transposed");
-  d_y.alloc(N);
-  upload_host(in.labels, (int64_t)sizeof(double) * N, d_y.p, st);
+  if (!fb) {
+    d_y.alloc(N);
+    upload_host(in.labels, (int64_t)sizeof(double) * N, d_y.p, st);
+  }
   d_raw.alloc((size_t)N * K);
-  if (K > 1) d_prob.alloc((size_t)N * K);
+  if (K > 1 && !fb) d_prob.alloc((size_t)N * K);
 
   // Initial scores (boosting.mojo:521-577; multiclass :4207-4225).  Across
   // devices the label sum is each shard's sequential sum combined in rank
@@ -310,8 +315,10 @@ void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
   agree(coll && mode == MODE_FIXED && coll->rank() < world - 1 && N % 1024 != 0
             ? "fixed-point data-parallel shards other than the last must hold a multiple of 1024 rows"
             : "");
-  std::vector<double> base(K);
-  if (K == 1) {
+  std::vector<double> base(K, 0.0);
+  if (fb) {
+    // feedback objectives start from the caller's scores, or 0
+  } else if (K == 1) {
     double mean = 0.0;
     std::string err;
     if (cfg.objective == OBJECTIVE_BINARY) {
@@ -377,7 +384,9 @@ void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
     MTB_CUDA(cudaMemcpyAsync(d_red.p, base.data(), sizeof(double) * K, cudaMemcpyHostToDevice, st));
     const long long n_raw = N * (long long)K;
     const unsigned blocks = (unsigned)std::min<long long>((n_raw + 255) / 256, 148ll * 16);
-    if (n_raw > 0) {
+    if (fb && fb->initial) {
+      upload_host(fb->initial, (int64_t)sizeof(double) * n_raw, d_raw.p, st);
+    } else if (n_raw > 0) {
       k_fill_raw<<<blocks, 256, 0, st>>>(d_raw.p, d_red.p, n_raw, K);
       MTB_CUDA(cudaGetLastError());
       stats.kernel_launches++;
@@ -386,6 +395,71 @@ void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
   }
 
   mark("initial scores");
+  // Feedback objectives: their inputs, and the derivatives of all classes
+  // (class-major), made once a round.
+  DevBuf<int> d_actions;
+  DevBuf<double> d_adv, d_old, d_ref, d_wt, d_logp, d_stats;
+  DevBuf<float> d_G, d_H, d_gl, d_hl;
+  PreferencePlan plan;
+  ScoreRows fb_rows = {d_raw.p, SCORE_F64, N, K, K, nullptr, false};
+  if (fb) {
+    d_G.alloc((size_t)N * K);
+    d_H.alloc((size_t)N * K);
+    auto up = [&](const double* host, DevBuf<double>& buf) {
+      if (!host) return;
+      buf.alloc(N);
+      upload_host(host, (int64_t)sizeof(double) * N, buf.p, st);
+    };
+    if (fb->actions) {
+      d_actions.alloc(N);
+      upload_host(fb->actions, (int64_t)sizeof(int) * N, d_actions.p, st);
+      fb_rows.actions = d_actions.p;
+    }
+    if (cfg.objective == OBJECTIVE_POLICY) {
+      up(fb->advantages, d_adv);
+      up(fb->old_logp, d_old);
+      up(fb->ref_logp, d_ref);
+      up(fb->weights, d_wt);
+      const bool need_ref = cfg.policy_kl > 0.0 && !fb->ref_logp;
+      if (!fb->old_logp || need_ref) {
+        // the policy that the fit starts from took the actions, or is the reference
+        d_logp.alloc(N);
+        d_stats.alloc(2 * (size_t)N);
+        stats.kernel_launches += launch_logprobs(fb_rows, d_logp.p, d_stats.p, st);
+      }
+    } else {
+      up(fb->reference, d_ref);
+      plan.build(fb->winners, fb->losers, fb->pair_weights, fb->n_pairs, N);
+      if (fb->actions) {
+        d_logp.alloc(N);
+        d_stats.alloc(2 * (size_t)N);
+        d_gl.alloc(N);
+        d_hl.alloc(N);
+      }
+    }
+    mark("feedback uploaded");
+  }
+  // the round's derivatives from the raw scores; returns the launches
+  auto feedback_derivatives = [&]() {
+    const ScoreDerivatives out = {d_G.p, d_H.p, 1, N};
+    if (cfg.objective == OBJECTIVE_POLICY) {
+      const double* start = d_logp.p;
+      const PolicyTerms t = {d_adv.p, d_old.p ? d_old.p : start,
+                             cfg.policy_kl > 0.0 ? (d_ref.p ? d_ref.p : start) : nullptr, d_wt.p,
+                             cfg.policy_clip_low, cfg.policy_clip_high, cfg.policy_kl, nullptr, nullptr};
+      return launch_policy(fb_rows, t, out, st);
+    }
+    int n = 0;
+    PreferenceTerms t = {d_raw.p, d_ref.p, SCORE_F64, cfg.preference_beta, cfg.preference_label_smoothing,
+                         cfg.preference_loss, nullptr, d_G.p, d_H.p};
+    if (K == 1) return launch_preference(plan, t, st);
+    n += launch_logprobs(fb_rows, d_logp.p, d_stats.p, st);
+    t.scores = d_logp.p;
+    t.grad = d_gl.p;
+    t.hess = d_hl.p;
+    n += launch_preference(plan, t, st);
+    return n + launch_logprobs_grad(fb_rows, d_stats.p, d_gl.p, d_hl.p, out, st);
+  };
   DevBuf<int> d_missing, d_ncats, d_feats;
   d_missing.alloc(F);
   d_ncats.alloc(F);
@@ -401,8 +475,10 @@ void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
   d_pairs0.alloc((size_t)N * pair_bytes);
   d_pairs1.alloc((size_t)N * pair_bytes);
   DevBuf<float> d_g, d_h;
-  d_g.alloc(N);
-  d_h.alloc(N);
+  if (!fb) {
+    d_g.alloc(N);
+    d_h.alloc(N);
+  }
   // FIXED-mode |g|, |h| partials: one per 1024 global rows.  Across devices
   // every rank gathers all ranks' partials (P per rank, the last rank's tail
   // zero-padded) so all reduce the same global pairwise tree.
@@ -621,7 +697,7 @@ void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
   } ieg{iter_ev};
   for (auto& e : iter_ev) MTB_CUDA(cudaEventCreateWithFlags(&e, cudaEventDisableTiming));
 
-  model.objective = cfg.objective;
+  model.objective = !fb ? cfg.objective : K > 1 ? (int)OBJECTIVE_MULTICLASS : (int)OBJECTIVE_L2;
   model.num_class = K;
   model.n_features = F;
   model.learning_rate = cfg.learning_rate;
@@ -742,7 +818,11 @@ void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
   mark_round();
   std::vector<size_t> round_trees;  // trees after each round
   for (int it = 0; it < cfg.num_iterations; ++it) {
-    if (K > 1) {
+    if (fb) {
+      timer.begin(&stats.grad_ms);
+      launches += feedback_derivatives();
+      timer.end();
+    } else if (K > 1) {
       k_softmax<<<grid256, 256, 0, st>>>(d_raw.p, d_prob.p, N, K);
       launches++;
     }
@@ -756,7 +836,12 @@ void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
         MTB_CUDA(cudaMemsetAsync(d_pg.p, 0, sizeof(double) * P_rank, st));
         MTB_CUDA(cudaMemsetAsync(d_ph.p, 0, sizeof(double) * P_rank, st));
       }
-      if (K == 1)
+      const float* g32 = fb ? d_G.p + (size_t)k * N : d_g.p;  // this class's derivatives
+      const float* h32 = fb ? d_H.p + (size_t)k * N : d_h.p;
+      if (fb)
+        k_grad_given<<<(unsigned)grid1024, 1024, 0, st>>>(g32, d_H.p + (size_t)k * N, N, mode, d_pg.p, d_ph.p,
+                                                          d_sc.p);
+      else if (K == 1)
         k_grad<<<(unsigned)std::min<long long>(grid1024, 2ll * n_sm), 1024, 0, st>>>(
             d_raw.p, d_y.p, d_g.p, d_h.p, N, cfg.objective, mode, d_pg.p, d_ph.p, d_sc.p);
       else
@@ -801,13 +886,13 @@ void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
       uint64_t gs = mt_quant_stream(cfg.quant_seed, it, k, 0);
       uint64_t hs = mt_quant_stream(cfg.quant_seed, it, k, 1);
       if (mode == MODE_QUANT)
-        k_quantize<MODE_QUANT><<<grid256, 256, 0, st>>>(d_g.p, d_h.p, N, in.row_offset, d_sc.p, const_h, gs, hs,
+        k_quantize<MODE_QUANT><<<grid256, 256, 0, st>>>(g32, h32, N, in.row_offset, d_sc.p, const_h, gs, hs,
                                                          d_rows0.p, d_pairs0.p);
       else if (wide)
-        k_quantize<MODE_FIXED, true><<<grid256, 256, 0, st>>>(d_g.p, d_h.p, N, in.row_offset, d_sc.p, const_h, gs, hs,
+        k_quantize<MODE_FIXED, true><<<grid256, 256, 0, st>>>(g32, h32, N, in.row_offset, d_sc.p, const_h, gs, hs,
                                                                d_rows0.p, d_pairs0.p);
       else
-        k_quantize<MODE_FIXED><<<grid256, 256, 0, st>>>(d_g.p, d_h.p, N, in.row_offset, d_sc.p, const_h, gs, hs,
+        k_quantize<MODE_FIXED><<<grid256, 256, 0, st>>>(g32, h32, N, in.row_offset, d_sc.p, const_h, gs, hs,
                                                          d_rows0.p, d_pairs0.p);
       launches += 2;
       timer.end();
@@ -917,10 +1002,15 @@ void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
       launches += 3;
       MTB_CUDA(cudaGetLastError());
       MTB_CUDA(cudaMemcpyAsync(&hdr, &d_ts.p->hdr, sizeof(TreeHeader), cudaMemcpyDeviceToHost, st));
+      RoundScales sc_host;
+      if (fb) MTB_CUDA(cudaMemcpyAsync(&sc_host, d_sc.p, sizeof(RoundScales), cudaMemcpyDeviceToHost, st));
       MTB_CUDA(cudaMemcpyAsync(nodes_host.data(), d_ts.p->nodes, sizeof(HostNode) * M, cudaMemcpyDeviceToHost, st));
       host_sync();
       timer.collect();
       hist_timer.collect();
+      // a log ratio beyond float32's range (e^88) makes a derivative infinite
+      if (fb && !(std::isfinite(sc_host.g_total) && std::isfinite(sc_host.h_total)))
+        throw std::runtime_error("the objective's derivatives are not finite: its log probabilities or scores lie too far apart");
       if (hdr.error || !hdr.done) throw std::runtime_error("device trainer reported an internal error");
       stats.iterations += hdr.iterations;
       stats.expansions += (hdr.n_pool - 1) / 2;

@@ -14,6 +14,25 @@ struct Unsupported : std::runtime_error {
 
 struct BinMapper;
 
+// What the objectives preference and policy learn from, in place of labels.
+// Host arrays, checked by the caller; per-row ones have n_rows values, and
+// null ones the meaning given here.
+struct Feedback {
+  const int32_t* actions = nullptr;  // class each row took (null: one score per row); policy: -1 takes no part
+  const double* initial = nullptr;   // [n_rows][num_class] raw scores to start from (null: 0)
+  // policy
+  const double* advantages = nullptr;
+  const double* old_logp = nullptr;  // null: under the initial scores
+  const double* ref_logp = nullptr;  // null: under the initial scores
+  const double* weights = nullptr;   // null: 1
+  // preference: rows winners[p] preferred to rows losers[p]
+  const int64_t* winners = nullptr;
+  const int64_t* losers = nullptr;
+  const float* pair_weights = nullptr;  // null: 1
+  int64_t n_pairs = 0;
+  const double* reference = nullptr;  // a reference model's scores or log probabilities (null: 0)
+};
+
 struct BinnedInput {
   const uint8_t* bins_fm;   // feature-major bins[f * n_rows + r], host memory
   long long n_rows;
@@ -32,6 +51,8 @@ struct BinnedInput {
   // + r] (host memory) binned on the device with `mapper`.
   const double* dense_fm = nullptr;
   const BinMapper* mapper = nullptr;
+  // Set for the objectives that learn from feedback; labels is null then.
+  const Feedback* feedback = nullptr;
 };
 
 // Trains on the current (or configured) CUDA device; fills model.trees,
