@@ -15,6 +15,7 @@ is 0 or every score is -inf; an action of n_classes or more gives NaN there.
 torch is imported by the first call on device scores.
 """
 import ctypes
+import threading
 
 import numpy as np
 
@@ -24,68 +25,81 @@ from ._capi import Model, MojoTreesError, _Err, _ptr, lib, params_string
 PREFERENCE_LOSSES = {"logistic": 0, "squared": 1}
 
 _types = None
+_local = threading.local()
 
 
 def _torch_types():
-    """{score dtype: (C code, per-row dtype, derivatives' dtype)}, and torch."""
+    """{score dtype: (C code, per-row dtype, derivatives' dtype)}, torch, and
+    the function that gives a device's current stream as an integer."""
     global _types
     if _types is None:
         import torch
+        # without the Stream object that torch.cuda.current_stream makes, where this torch has it
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
         _types = ({torch.float64: (0, torch.float64, torch.float32), torch.float32: (1, torch.float32, torch.float32),
                    torch.float16: (2, torch.float32, torch.float16), torch.bfloat16: (3, torch.float32, torch.bfloat16)},
-                  torch)
+                  torch, stream)
     return _types
+
+
+def _err():
+    """This thread's error object."""
+    e = getattr(_local, "err", None)
+    if e is None:
+        e = _local.err = _Err()
+    return e
 
 
 def _invalid(message):
     return MojoTreesError(_capi.ERROR_INVALID_ARGUMENT, message)
 
 
-def _vector(name, t, n, dtype, device, shape=None):
-    """The address of a contiguous tensor of n values (shape: its shape instead)."""
+def _vector(name, t, shape, dtype, device):
+    """The address of a contiguous tensor (None: none)."""
     if t is None:
         return None
-    shape = (n,) if shape is None else shape
-    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
-        raise _invalid(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}, got "
+    if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise _invalid(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, got "
                        f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
 def _rows(scores, actions):
     """The arguments that describe scores and actions, and what follows from them."""
-    types, torch = _torch_types()
+    types, torch, stream = _torch_types()
+    dev = scores.device
     if scores.dtype not in types:
         raise _invalid(f"scores must be float64, float32, float16 or bfloat16, got {scores.dtype}")
-    if scores.dim() != 2 or scores.device.type != "cuda":
-        raise _invalid(f"scores must be [n_rows, n_classes] on a CUDA device, got {tuple(scores.shape)} on {scores.device}")
+    if scores.dim() != 2 or dev.type != "cuda":
+        raise _invalid(f"scores must be [n_rows, n_classes] on a CUDA device, got {tuple(scores.shape)} on {dev}")
     n, k = scores.shape
-    stride = scores.stride(0) if n > 1 else k
-    if (k > 1 and scores.stride(1) != 1) or stride < k:
+    stride, inner = scores.stride()
+    if n <= 1:
+        stride = k
+    if (k > 1 and inner != 1) or stride < k:
         raise _invalid("scores must hold a row's classes next to each other and rows that do not overlap")
-    if actions.dtype not in (torch.int32, torch.int64):
+    if actions.dtype is torch.int32:
+        width = 4
+    elif actions.dtype is torch.int64:
+        width = 8
+    else:
         raise _invalid(f"actions must be int32 or int64, got {actions.dtype}")
     code, row, out = types[scores.dtype]
-    a = _vector("actions", actions, n, actions.dtype, scores.device)
-    head = (scores.data_ptr(), code, n, k, stride, a, 4 if actions.dtype == torch.int32 else 8)
-    return torch, head, row, out
-
-
-def _stream(torch, device):
-    return torch.cuda.current_stream(device).cuda_stream
+    head = (scores.data_ptr(), code, n, k, stride, _vector("actions", actions, (n,), actions.dtype, dev), width)
+    return torch, head, row, out, dev, stream(dev.index)
 
 
 def action_logprobs(scores, actions):
     """log softmax(scores)[actions] of [n_rows, n_classes] scores, and the row
     statistics its gradient needs: (logp [n_rows], stats [n_rows, 2]), float64
     for float64 scores and else float32."""
-    torch, head, row, _ = _rows(scores, actions)
+    torch, head, row, _, dev, stream = _rows(scores, actions)
     n = head[2]
-    logp = torch.empty(n, dtype=row, device=scores.device)
-    stats = torch.empty((n, 2), dtype=row, device=scores.device)
-    e = _Err()
-    e.check(lib().mojotrees_b200_action_logprobs(*head, logp.data_ptr(), stats.data_ptr(),
-                                                 _stream(torch, scores.device), e.h))
+    logp = torch.empty(n, dtype=row, device=dev)
+    stats = torch.empty((n, 2), dtype=row, device=dev)
+    e = _err()
+    e.check(lib().mojotrees_b200_action_logprobs(*head, logp.data_ptr(), stats.data_ptr(), stream, e.h))
     return logp, stats
 
 
@@ -94,17 +108,16 @@ def action_logprobs_grad(scores, actions, stats, grad_logp, hess_logp=None):
     to action_logprobs' log probabilities (float32 [n_rows]): (grad, hess), hess
     None without hess_logp.  float32 for float64 and float32 scores, else the
     scores' type."""
-    torch, head, row, out = _rows(scores, actions)
-    n, k, dev = head[2], head[3], scores.device
-    st = _vector("stats", stats, n, row, dev, (n, 2))
-    g = _vector("grad_logp", grad_logp, n, torch.float32, dev)
-    h = _vector("hess_logp", hess_logp, n, torch.float32, dev)
+    torch, head, row, out, dev, stream = _rows(scores, actions)
+    n, k = head[2], head[3]
+    st = _vector("stats", stats, (n, 2), row, dev)
+    g = _vector("grad_logp", grad_logp, (n,), torch.float32, dev)
+    h = _vector("hess_logp", hess_logp, (n,), torch.float32, dev)
     grad = torch.empty((n, k), dtype=out, device=dev)
     hess = None if hess_logp is None else torch.empty((n, k), dtype=out, device=dev)
-    e = _Err()
+    e = _err()
     e.check(lib().mojotrees_b200_action_logprobs_grad(*head, st, g, h, grad.data_ptr(),
-                                                      None if hess is None else hess.data_ptr(), k,
-                                                      _stream(torch, dev), e.h))
+                                                      None if hess is None else hess.data_ptr(), k, stream, e.h))
     return grad, hess
 
 
@@ -115,20 +128,21 @@ def policy_loss(scores, actions, advantages, old_logp, ref_logp=None, weights=No
     r = exp(logp - old_logp), t = ref_logp - logp.  Per-row tensors are float64
     for float64 scores and else float32.  Returns (loss, logp, grad, hess); the
     derivatives with respect to the scores are None where not asked for."""
-    torch, head, row, out = _rows(scores, actions)
-    n, k, dev = head[2], head[3], scores.device
+    torch, head, row, out, dev, stream = _rows(scores, actions)
+    n, k = shape = head[2], head[3]
     if hess and not grad:
         raise _invalid("hess needs grad")
-    rows = [_vector(name, t, n, row, dev) for name, t in (("advantages", advantages), ("old_logp", old_logp),
-                                                          ("ref_logp", ref_logp), ("weights", weights))]
+    per_row = (n,)
+    rows = (_vector("advantages", advantages, per_row, row, dev), _vector("old_logp", old_logp, per_row, row, dev),
+            _vector("ref_logp", ref_logp, per_row, row, dev), _vector("weights", weights, per_row, row, dev))
     loss = torch.empty(n, dtype=row, device=dev)
     logp = torch.empty(n, dtype=row, device=dev)
-    dg = torch.empty((n, k), dtype=out, device=dev) if grad else None
-    dh = torch.empty((n, k), dtype=out, device=dev) if hess else None
-    e = _Err()
+    dg = torch.empty(shape, dtype=out, device=dev) if grad else None
+    dh = torch.empty(shape, dtype=out, device=dev) if hess else None
+    e = _err()
     e.check(lib().mojotrees_b200_policy_loss(*head, *rows, clip_low, clip_high, kl_coef, loss.data_ptr(),
                                              logp.data_ptr(), None if dg is None else dg.data_ptr(),
-                                             None if dh is None else dh.data_ptr(), k, _stream(torch, dev), e.h))
+                                             None if dh is None else dh.data_ptr(), k, stream, e.h))
     return loss, logp, dg, dh
 
 
@@ -159,7 +173,7 @@ class PreferencePlan:
         self.h = h.value
 
     def __del__(self):
-        if getattr(self, "h", None) and _capi._lib is not None:
+        if getattr(self, "h", None) and _capi is not None and _capi._lib is not None:
             _capi._lib.mojotrees_b200_preference_plan_free(self.h)
             self.h = None
 
@@ -171,21 +185,22 @@ def preference_loss(plan, scores, reference=None, beta=1.0, label_smoothing=0.0,
     smoothing; "squared": (u - 1 / (2 beta))^2, for a pair's difference u of
     score - reference.  Returns (loss [n_pairs], grad [n_items], hess
     [n_items]); the derivatives are float32."""
-    types, torch = _torch_types()
-    if scores.dtype not in (torch.float64, torch.float32) or scores.device.type != "cuda":
-        raise _invalid(f"scores must be float64 or float32 on a CUDA device, got {scores.dtype} on {scores.device}")
+    types, torch, stream = _torch_types()
+    dtype, dev = scores.dtype, scores.device
+    if dtype not in (torch.float64, torch.float32) or dev.type != "cuda":
+        raise _invalid(f"scores must be float64 or float32 on a CUDA device, got {dtype} on {dev}")
     if loss not in PREFERENCE_LOSSES:
         raise _invalid(f"loss must be one of {', '.join(PREFERENCE_LOSSES)}, got {loss!r}")
-    dev = scores.device
-    s = _vector("scores", scores, plan.n_items, scores.dtype, dev)
-    r = _vector("reference", reference, plan.n_items, scores.dtype, dev)
-    out = torch.empty(plan.n_pairs, dtype=scores.dtype, device=dev)
-    grad = torch.empty(plan.n_items, dtype=torch.float32, device=dev)
-    hess = torch.empty(plan.n_items, dtype=torch.float32, device=dev)
-    e = _Err()
-    e.check(lib().mojotrees_b200_preference_loss(plan.h, s, r, types[scores.dtype][0], beta, label_smoothing,
+    items = (plan.n_items,)
+    s = _vector("scores", scores, items, dtype, dev)
+    r = _vector("reference", reference, items, dtype, dev)
+    out = torch.empty(plan.n_pairs, dtype=dtype, device=dev)
+    grad = torch.empty(items, dtype=torch.float32, device=dev)
+    hess = torch.empty(items, dtype=torch.float32, device=dev)
+    e = _err()
+    e.check(lib().mojotrees_b200_preference_loss(plan.h, s, r, types[dtype][0], beta, label_smoothing,
                                                  PREFERENCE_LOSSES[loss], out.data_ptr(), grad.data_ptr(),
-                                                 hess.data_ptr(), _stream(torch, dev), e.h))
+                                                 hess.data_ptr(), stream(dev.index), e.h))
     return out, grad, hess
 
 

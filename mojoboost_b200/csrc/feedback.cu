@@ -21,6 +21,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 #include <memory>
 #include <stdexcept>
 #include <string>
@@ -741,9 +742,13 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
 inline bool on16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
 int multiprocessors() {
+  constexpr int kMostDevices = 64;
+  static std::atomic<int> known[kMostDevices];
   int dev = 0, n = 0;
   MTB_CUDA_FB(cudaGetDevice(&dev));
+  if (dev < kMostDevices && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
   MTB_CUDA_FB(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < kMostDevices) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
@@ -1354,43 +1359,62 @@ void by_type(int type, F&& f) {
 // Paired preference loss
 // ---------------------------------------------------------------------------
 
-// With u = (s_w - s_l) - (ref_w - ref_l):
-//   logistic  L = (1 - e) softplus(-beta u) + e softplus(beta u)
-//             L' = beta (e sig(beta u) - (1 - e) sig(-beta u))
-//             L'' = beta^2 sig(beta u) sig(-beta u)
+// With u = (s_w - s_l) - (ref_w - ref_l) and x = beta u:
+//   logistic  L = (1 - e) softplus(-x) + e softplus(x)
+//             L' = beta (e sig(x) - (1 - e) sig(-x))
+//             L'' = beta^2 sig(x) sig(-x)
 //   squared   L = (u - 1 / (2 beta))^2
-// in float64 throughout: u is the difference of log probabilities of whole
-// answers, tens or hundreds each.
 //
 // An item's derivatives are a sum over its pairs, which the plan lists item by
 // item: no atomics, and the same bits at every call.  Each pair's terms are
-// computed for both of its items (a dozen float64 operations on top of what
-// each loads) rather than once and stored, which would take memory that calls
-// share; the winner's side also writes the pair's loss.  What bounds it is
-// the other item's score and reference: a sector of L2 each per entry.
+// computed for both of its items (a hundred instructions) rather than once and
+// stored, which would take memory that calls share; the winner's side also
+// writes the pair's loss.  What bounds it is the other item's score and
+// reference, a sector of L2 each per entry, and the terms' arithmetic.
 struct PairMath {
   double beta, smoothing, target;  // target: 1 / (2 beta)
   int kind;
 };
 
+template <typename T>
 struct PairTerms {
-  double g, h, loss;
+  T g, h, loss;
 };
 
-__device__ __forceinline__ PairTerms pair_terms(const PairMath& pm, double u, const TableMath& math) {
+// float64 scores: float64 throughout.  float32 scores: u is as good as exact
+// (see Lean), and what follows is float32 arithmetic of a few steps' error.
+__device__ __forceinline__ double pair_exp(double x, const TableMath& math) { return math.exp(x); }
+__device__ __forceinline__ float pair_exp(float x, const TableMath&) { return expf(x); }
+__device__ __forceinline__ double pair_inverse(double x) { return TableMath::inverse(x); }
+__device__ __forceinline__ float pair_inverse(float x) { return __frcp_rn(x); }
+__device__ __forceinline__ double pair_log1p(double x, const TableMath& math) { return math.log1p(x); }
+__device__ __forceinline__ float pair_log1p(float x, const TableMath&) { return log1pf(x); }
+__device__ __forceinline__ double flip(double x, int by) {  // x, negated where by is negative
+  return __hiloint2double(__double2hiint(x) ^ (by & 0x80000000), __double2loint(x));
+}
+__device__ __forceinline__ float flip(float x, int by) { return __uint_as_float(__float_as_uint(x) ^ (by & 0x80000000u)); }
+
+template <typename T>
+__device__ __forceinline__ PairTerms<T> pair_terms(const PairMath& pm, T u, bool want_loss, const TableMath& math) {
+  PairTerms<T> t;
   if (pm.kind == PREFERENCE_SQUARED) {
-    const double d = u - pm.target;
-    return {2.0 * d, 2.0, d * d};
+    const T d = u - (T)pm.target;
+    return {(T)2 * d, (T)2, d * d};
   }
-  const double x = pm.beta * u, e = math.exp(-fabs(x)), big = TableMath::inverse(1.0 + e), small = e * big;
-  const double up = x >= 0.0 ? big : small, down = x >= 0.0 ? small : big, soft = math.log1p(e);
-  PairTerms t = {-pm.beta * (1.0 - pm.smoothing) * down, pm.beta * pm.beta * big * small,
-                 (1.0 - pm.smoothing) * (soft + fmax(-x, 0.0))};
-  if (pm.smoothing > 0.0) {  // an infinite x times 0 would be NaN
-    t.g += pm.beta * pm.smoothing * up;
-    t.loss += pm.smoothing * (soft + fmax(x, 0.0));
+  const T beta = (T)pm.beta, x = beta * u, e = pair_exp(-fabs(x), math), r = pair_inverse((T)1 + e), er = e * r;
+  const T down = x >= (T)0 ? er : r;  // sig(-x)
+  const T keep = (T)(1.0 - pm.smoothing);
+  t.g = -(beta * keep) * down;
+  t.h = beta * beta * er * r;
+  t.loss = (T)0;
+  if (want_loss) {
+    const T soft = pair_log1p(e, math);
+    t.loss = keep * (soft + (x < (T)0 ? -x : (T)0));
+    if (pm.smoothing > 0.0) t.loss += (T)pm.smoothing * (soft + (x > (T)0 ? x : (T)0));
+    if (x != x) t.loss = x;
   }
-  if (x != x) t.loss = x;
+  // apart, since an infinite x times a smoothing of 0 would be NaN
+  if (pm.smoothing > 0.0) t.g += beta * (T)pm.smoothing * (x >= (T)0 ? r : er);
   return t;
 }
 
@@ -1407,30 +1431,63 @@ struct PreferenceArgs {
   float *grad, *hess;
 };
 
+// An item's distance to its reference.  The difference of two float32 log
+// probabilities of whole answers loses what the pair's difference needs, so it
+// is kept with its rounding error (O. Moller, "Quasi double-precision in
+// floating point addition", BIT 5, 1965).
 template <typename T>
-__device__ __forceinline__ double lean(const PreferenceArgs<T>& A, int i) {
-  return A.ref ? (double)A.s[i] - (double)A.ref[i] : (double)A.s[i];
+struct Lean;
+template <>
+struct Lean<double> {
+  double v;
+  __device__ __forceinline__ Lean(double s, double r) : v(s - r) {}
+  __device__ __forceinline__ double minus(const Lean& o) const { return v - o.v; }
+};
+template <>
+struct Lean<float> {
+  float v, err;
+  __device__ __forceinline__ Lean(float s, float r) {
+    v = s - r;
+    const float b = v - s;
+    err = (s - (v - b)) - (r + b);
+  }
+  __device__ __forceinline__ float minus(const Lean& o) const {
+    const float d = v - o.v, b = d - v;
+    const float low = ((v - (d - b)) - (o.v + b)) + (err - o.err);
+    return low == low ? d + low : d;  // infinities have no error terms
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ Lean<T> lean(const PreferenceArgs<T>& A, int i) {
+  return Lean<T>(A.s[i], A.ref ? A.ref[i] : (T)0);
 }
 
-// One entry of item i's list; `own` is the item's own distance to its reference.
+// One entry of an item's list; `own` is the item's own distance to its reference.
 template <typename T>
-__device__ __forceinline__ void add_entry(const PreferenceArgs<T>& A, int2 entry, double w, double own, double other,
-                                          const TableMath& math, double* g, double* h) {
-  const bool lost = entry.x < 0;
-  const PairTerms t = pair_terms(A.pm, lost ? other - own : own - other, math);
-  *g += lost ? -(w * t.g) : w * t.g;
-  *h += w * t.h;
-  if (!lost && A.loss) A.loss[entry.y] = (T)(w * t.loss);
+__device__ __forceinline__ void add_entry(const PreferenceArgs<T>& A, int2 entry, T w, const Lean<T>& own,
+                                          const Lean<T>& other, const TableMath& math, double* g, double* h) {
+  const PairTerms<T> t = pair_terms<T>(A.pm, flip(own.minus(other), entry.x), A.loss != nullptr, math);
+  *g += (double)flip(w * t.g, entry.x);
+  *h += (double)(w * t.h);
+  if (A.loss && entry.x >= 0) A.loss[entry.y] = w * t.loss;
 }
 
 constexpr int kPairThreads = 256;
-// Items of more pairs than a warp takes in this many steps have a block, or
-// from kHuge pairs a cluster of 8, to themselves: a warp's steps are one
-// after the other, about 0.5 us each with four loads in flight.
+// Items of more pairs than a warp takes in this many steps have a block to
+// themselves, or from kHuge pairs a cluster of 8: a warp's steps are one after
+// the other, and a long item in a warp would be the last to end.
 constexpr int kWarpSteps = 16;
 constexpr int kLong = 32 * kWarpSteps;
 constexpr int kHuge = 16384;
 constexpr int kPairCluster = 8;
+constexpr int kLongThreads = 512;
+
+// The launches for huge, long and other items write apart from one another,
+// so each lets the next begin at once; each ends only when the one before it
+// has, so that the last one's end is the call's.
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // G lanes an item.
 template <typename T, int G>
@@ -1447,15 +1504,20 @@ __global__ void __launch_bounds__(kPairThreads) k_preference_items(const Prefere
     const int e0 = A.offsets[i], e1 = A.offsets[i + 1];
     const bool skip = at >= A.n_items || e1 - e0 > kLong;
     double g = 0.0, h = 0.0;
-    if (!skip && e0 < e1) {
-      const double own = lean(A, i);
-      for (int e = e0 + l; e < e1; e += 2 * G) {  // two entries' loads in flight
-        const bool two = e + G < e1;
-        const int2 a = A.entries[e], b = two ? A.entries[e + G] : a;
-        const double wa = A.entry_w ? (double)A.entry_w[e] : 1.0, wb = two && A.entry_w ? (double)A.entry_w[e + G] : 1.0;
-        const double la = lean(A, a.x & 0x7fffffff), lb = two ? lean(A, b.x & 0x7fffffff) : 0.0;
-        add_entry(A, a, wa, own, la, math, &g, &h);
-        if (two) add_entry(A, b, wb, own, lb, math, &g, &h);
+    if (!skip && e0 + l < e1) {
+      const Lean<T> own = lean(A, i);
+      int2 c = A.entries[e0 + l];
+      Lean<T> other = lean(A, c.x & 0x7fffffff);
+      T w = A.entry_w ? (T)A.entry_w[e0 + l] : (T)1;
+      for (int e = e0 + l; e < e1; e += G) {  // the next entry's loads while this one is computed
+        const bool more = e + G < e1;
+        const int2 cn = more ? A.entries[e + G] : c;
+        const Lean<T> on = more ? lean(A, cn.x & 0x7fffffff) : other;
+        const T wn = more && A.entry_w ? (T)A.entry_w[e + G] : w;
+        add_entry(A, c, w, own, other, math, &g, &h);
+        c = cn;
+        other = on;
+        w = wn;
       }
     }
 #pragma unroll
@@ -1468,33 +1530,36 @@ __global__ void __launch_bounds__(kPairThreads) k_preference_items(const Prefere
       A.hess[i] = (float)h;
     }
   }
+  wait_for_previous();
 }
 
 // A block or cluster an item of the list.
 template <typename T>
-__global__ void __launch_bounds__(kPairThreads) k_preference_long(const PreferenceArgs<T> A, const int* __restrict__ items) {
+__global__ void __launch_bounds__(kLongThreads) k_preference_long(const PreferenceArgs<T> A, const int* __restrict__ items) {
   namespace cg = cooperative_groups;
   __shared__ MathTables tables;
-  __shared__ double sm[2][kPairThreads / 32], sum[2];
+  __shared__ double sm[2][kLongThreads / 32], sum[2];
+  let_next_begin();
   const TableMath math(tables);
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int i = items[blockIdx.x / blocks], e1 = A.offsets[i + 1], step = blocks * kPairThreads;
-  const double own = lean(A, i);
+  const int i = items[blockIdx.x / blocks], e1 = A.offsets[i + 1], step = blocks * kLongThreads;
+  const Lean<T> own = lean(A, i);
   double g = 0.0, h = 0.0;
-  for (int e = A.offsets[i] + rank * kPairThreads + threadIdx.x; e < e1; e += 4 * step) {
+  for (int e = A.offsets[i] + rank * kLongThreads + threadIdx.x; e < e1; e += 4 * step) {
     int2 c[4];
-    double other[4], w[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) c[q] = e1 - e > q * step ? A.entries[e + q * step] : make_int2(i, -1);
+    T w[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      other[q] = lean(A, c[q].x & 0x7fffffff);
-      w[q] = A.entry_w && c[q].y >= 0 ? (double)A.entry_w[e + q * step] : 1.0;
+      const bool there = e1 - e > q * step;
+      c[q] = there ? A.entries[e + q * step] : make_int2(i, -1);
+      w[q] = there && A.entry_w ? (T)A.entry_w[e + q * step] : (T)1;
     }
+    const Lean<T> o[4] = {lean(A, c[0].x & 0x7fffffff), lean(A, c[1].x & 0x7fffffff), lean(A, c[2].x & 0x7fffffff),
+                          lean(A, c[3].x & 0x7fffffff)};
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      if (c[q].y >= 0) add_entry(A, c[q], w[q], own, other[q], math, &g, &h);
+      if (c[q].y >= 0) add_entry(A, c[q], w[q], own, o[q], math, &g, &h);
   }
   for (int k = 16; k > 0; k >>= 1) {
     g += __shfl_xor_sync(0xffffffffu, g, k);
@@ -1507,7 +1572,7 @@ __global__ void __launch_bounds__(kPairThreads) k_preference_long(const Preferen
   __syncthreads();
   if (threadIdx.x < 2) {
     double t = 0.0;
-    for (int k = 0; k < kPairThreads / 32; ++k) t += sm[threadIdx.x][k];
+    for (int k = 0; k < kLongThreads / 32; ++k) t += sm[threadIdx.x][k];
     sum[threadIdx.x] = t;
   }
   if (blocks > 1) cluster.sync();
@@ -1517,30 +1582,38 @@ __global__ void __launch_bounds__(kPairThreads) k_preference_long(const Preferen
     (threadIdx.x ? A.hess : A.grad)[i] = (float)t;
   }
   if (blocks > 1) cluster.sync();  // until the first block has read the sums
+  wait_for_previous();
 }
 
-template <typename T>
-void launch_preference_long(const PreferenceArgs<T>& A, const int* items, long long n, int blocks, cudaStream_t st) {
-  if (n == 0) return;
+// after: this call's launch before this one, which it need not wait for.
+template <typename K, typename... Args>
+void launch_pairs(K kernel, unsigned grid, int threads, int blocks, bool after, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3((unsigned)(n * blocks));
-  lc.blockDim = dim3(kPairThreads);
+  lc.gridDim = dim3(grid);
+  lc.blockDim = dim3(threads);
   lc.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = blocks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
   lc.attrs = attr;
-  lc.numAttrs = blocks > 1 ? 1 : 0;
-  MTB_CUDA_FB(cudaLaunchKernelEx(&lc, k_preference_long<T>, A, items));
+  lc.numAttrs = 0;
+  if (blocks > 1) {
+    cudaLaunchAttribute& a = attr[lc.numAttrs++];
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = blocks;
+    a.val.clusterDim.y = a.val.clusterDim.z = 1;
+  }
+  if (after) {
+    cudaLaunchAttribute& a = attr[lc.numAttrs++];
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+  }
+  MTB_CUDA_FB(cudaLaunchKernelEx(&lc, kernel, args...));
 }
 
 template <typename T, int G>
-void launch_preference_items(const PreferenceArgs<T>& A, cudaStream_t st) {
+void launch_preference_items(const PreferenceArgs<T>& A, bool after, cudaStream_t st) {
   const long long blocks = ((long long)A.n_items * G + kPairThreads - 1) / kPairThreads;
   const unsigned grid = (unsigned)std::min<long long>(blocks, 16ll * multiprocessors());
-  k_preference_items<T, G><<<grid, kPairThreads, 0, st>>>(A);
-  MTB_CUDA_FB(cudaGetLastError());
+  launch_pairs(k_preference_items<T, G>, grid, kPairThreads, 1, after, st, A);
 }
 
 template <typename T>
@@ -1560,14 +1633,18 @@ void launch_preference_t(const PreferencePlan& plan, const PreferenceTerms& t, c
   A.grad = t.grad;
   A.hess = t.hess;
   // long items first: they take longest
-  launch_preference_long(A, plan.huge_items, plan.n_huge, kPairCluster, st);
-  launch_preference_long(A, plan.long_items, plan.n_long, 1, st);
-  // lanes for half of the mean number of pairs, so that most items take two steps
+  const bool huge = plan.n_huge > 0, any = huge || plan.n_long > 0;
+  if (huge)
+    launch_pairs(k_preference_long<T>, (unsigned)plan.n_huge * kPairCluster, kLongThreads, kPairCluster, false, st, A,
+                 (const int*)plan.huge_items);
+  if (plan.n_long > 0)
+    launch_pairs(k_preference_long<T>, (unsigned)plan.n_long, kLongThreads, 1, huge, st, A, (const int*)plan.long_items);
+  // about as many lanes as half of the mean number of pairs
   const long long mean = plan.n_entries / plan.n_items;
-  if (mean < 4) launch_preference_items<T, 1>(A, st);
-  else if (mean < 16) launch_preference_items<T, 4>(A, st);
-  else if (mean < 48) launch_preference_items<T, 16>(A, st);
-  else launch_preference_items<T, 32>(A, st);
+  if (mean < 4) launch_preference_items<T, 1>(A, any, st);
+  else if (mean < 16) launch_preference_items<T, 4>(A, any, st);
+  else if (mean < 48) launch_preference_items<T, 16>(A, any, st);
+  else launch_preference_items<T, 32>(A, any, st);
 }
 
 }  // namespace

@@ -482,21 +482,28 @@ def test_preference_loss(mtlib, n, P_, how, dtype):
         rd = None if ref is None else ref.double().cpu().numpy()
         L, g, h = fu.pairs_loss(sd, rd, i, j, w, beta, eps, loss)
         unit = 2.0 ** -53 if dtype == "float64" else fu.U32
-        # float64 arithmetic of values up to |u| ~ 100: a difference's rounding (2^-53 * 160) times the slope, and a
-        # few operations' own
-        slope = np.abs(g) + h * 1e-12
-        _close(got[0], L, np.abs(L) * (2 * unit + 2.0 ** -49) + slope * 160 * 2.0 ** -52, "loss")
-        G, H, A = np.zeros(n), np.zeros(n), np.zeros(n)
+        # Each term in the scores' arithmetic, with half a step `unit`.  The pair's difference u: a rounding of each
+        # item's distance to its reference (up to 60 here) and of their difference in float64; in float32 that
+        # distance keeps its rounding error, which leaves one rounding of u itself.  Then x = beta u, exp within 2 + |x|
+        # steps, 1 + e, its inverse, three products; the loss a log1p within 2 steps and a sum.
+        u = np.abs(sd - (0 if rd is None else rd))
+        u = (u[i] + u[j]) if P_ else np.zeros(0)
+        x = beta * u
+        # The plain form rounds alike in float64: beside a float64 kernel its error counts too.
+        sides = 2 if dtype == "float64" else 1
+        du = sides * (u + (1 / (2 * beta) if loss == "squared" else 0)) * 2 * unit  # absolute
+        term = sides * 2 * (14 + 4 * x) * unit  # relative, a full step being 2 unit
+        _close(got[0], L, np.abs(L) * (term + 2 * unit) + (np.abs(g) + h * du) * du + 2.0 ** -126, "loss")
+        G, H, E, A, B = (np.zeros(n) for _ in range(5))
         np.add.at(G, i, g)
         np.add.at(G, j, -g)
-        for v, at in ((h, H), (np.abs(g) + h * 160, A)):
+        for v, at in ((h, H), (np.abs(g), A), (np.abs(g) * term + h * du * 1.1, E), (h * (term + 2 * beta * du), B)):
             np.add.at(at, i, v)
             np.add.at(at, j, v)
         degree = np.bincount(np.concatenate([i, j]), minlength=n)[:n]
-        # each term's rounding, and a float64 sum of `degree` terms in any order (both here and there)
-        tol = A * (2.0 ** -48 + 2 * degree * 2.0 ** -53)
-        _close(got[1], G, np.abs(G) * fu.U32 * 1.01 + tol + TINY["float32"], "grad")
-        _close(got[2], H, H * (fu.U32 * 1.01 + 2.0 ** -44 + 2 * degree * 2.0 ** -53) + TINY["float32"], "hess")
+        lane = 2 * degree * 2.0 ** -53  # sums in float64, in any order, both here and there
+        _close(got[1], G, np.abs(G) * fu.U32 * 1.01 + E + A * lane + 2.0 ** -126, "grad")
+        _close(got[2], H, H * (fu.U32 * 1.01 + lane) + B + 2.0 ** -126, "hess")
         again = mtlib.preference_loss(plan, s, reference=ref, beta=beta, label_smoothing=eps, loss=loss)
         for u, v in zip(got, again):
             assert torch.equal(u, v)
