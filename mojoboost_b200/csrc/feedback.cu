@@ -322,8 +322,9 @@ struct MathTables {
 
 struct TableMath {
   MathTables* t;
-  // The whole block calls it.
-  __device__ __forceinline__ explicit TableMath(MathTables& tables) : t(&tables) {
+  // The whole block calls it; used: whether any of the tables is.
+  __device__ __forceinline__ explicit TableMath(MathTables& tables, bool used = true) : t(&tables) {
+    if (!used) return;
     for (int j = threadIdx.x; j < 65; j += blockDim.x) t->two[j] = j < 64 ? exp2(j / 64.0) : 0.0;
     for (int j = threadIdx.x; j < 64; j += blockDim.x) {
       t->inv_c[j] = 64.0 / (64 + j);
@@ -1424,7 +1425,7 @@ struct PreferenceArgs {
   const int2* entries;
   const float* entry_w;
   const int* zero_pairs;
-  int n_zero, n_items;
+  int n_zero, n_items, long_from;
   const T *s, *ref;
   PairMath pm;
   T* loss;
@@ -1474,14 +1475,28 @@ __device__ __forceinline__ void add_entry(const PreferenceArgs<T>& A, int2 entry
 }
 
 constexpr int kPairThreads = 256;
-// Items of more pairs than a warp takes in this many steps have a block to
-// themselves, or from kHuge pairs a cluster of 8: a warp's steps are one after
-// the other, and a long item in a warp would be the last to end.
-constexpr int kWarpSteps = 16;
-constexpr int kLong = 32 * kWarpSteps;
-constexpr int kHuge = 16384;
+constexpr int kLongThreads = 128;
+constexpr int kHugeThreads = 512;
 constexpr int kPairCluster = 8;
-constexpr int kLongThreads = 512;
+
+// Lanes an item, by the mean number of an item's pairs: about eight steps of a
+// lane, so that an item's own loads, sums of lanes and stores are shared by
+// few instructions (all pairs in groups of 64, float64: 53 us with 32 lanes,
+// 41 us with 8).
+int pair_lanes(long long mean) { return mean < 8 ? 1 : mean < 32 ? 4 : mean < 128 ? 8 : 32; }
+
+}  // namespace
+
+// Items of more pairs than their lanes take in 24 steps have a block to
+// themselves, or from 2048 pairs a cluster of 8: a lane's steps are one after
+// the other, and a long item in a warp would be the last to end.
+int PreferencePlan::long_from(long long n_entries, long long n_items) {
+  return 24 * pair_lanes(n_entries / std::max(1ll, n_items)) + 1;
+}
+
+namespace {
+
+constexpr int kHuge = 2048;
 
 // The launches for huge, long and other items write apart from one another,
 // so each lets the next begin at once; each ends only when the one before it
@@ -1493,7 +1508,7 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 template <typename T, int G>
 __global__ void __launch_bounds__(kPairThreads) k_preference_items(const PreferenceArgs<T> A) {
   __shared__ MathTables tables;
-  const TableMath math(tables);
+  const TableMath math(tables, sizeof(T) == 8);
   const long long thread = (long long)blockIdx.x * kPairThreads + threadIdx.x;
   const long long threads = (long long)gridDim.x * kPairThreads;
   if (A.loss)
@@ -1502,7 +1517,7 @@ __global__ void __launch_bounds__(kPairThreads) k_preference_items(const Prefere
   for (long long at = thread / G; at < (A.n_items + 31) / 32 * 32ll; at += threads / G) {  // whole warps
     const int i = (int)min(at, (long long)A.n_items - 1);
     const int e0 = A.offsets[i], e1 = A.offsets[i + 1];
-    const bool skip = at >= A.n_items || e1 - e0 > kLong;
+    const bool skip = at >= A.n_items || e1 - e0 >= A.long_from;
     double g = 0.0, h = 0.0;
     if (!skip && e0 + l < e1) {
       const Lean<T> own = lean(A, i);
@@ -1534,52 +1549,56 @@ __global__ void __launch_bounds__(kPairThreads) k_preference_items(const Prefere
 }
 
 // A block or cluster an item of the list.
-template <typename T>
-__global__ void __launch_bounds__(kLongThreads) k_preference_long(const PreferenceArgs<T> A, const int* __restrict__ items) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_preference_long(const PreferenceArgs<T> A, const int* __restrict__ items,
+                                                             const int n) {
   namespace cg = cooperative_groups;
   __shared__ MathTables tables;
-  __shared__ double sm[2][kLongThreads / 32], sum[2];
+  __shared__ double sm[2][2][THREADS / 32], sum[2][2];  // by the parity of the item
   let_next_begin();
-  const TableMath math(tables);
+  const TableMath math(tables, sizeof(T) == 8);
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int i = items[blockIdx.x / blocks], e1 = A.offsets[i + 1], step = blocks * kLongThreads;
-  const Lean<T> own = lean(A, i);
-  double g = 0.0, h = 0.0;
-  for (int e = A.offsets[i] + rank * kLongThreads + threadIdx.x; e < e1; e += 4 * step) {
-    int2 c[4];
-    T w[4];
+  int parity = 0;
+  for (int at = blockIdx.x / blocks; at < n; at += gridDim.x / blocks, parity ^= 1) {
+    const int i = items[at], e1 = A.offsets[i + 1], step = blocks * THREADS;
+    const Lean<T> own = lean(A, i);
+    double g = 0.0, h = 0.0;
+    for (int e = A.offsets[i] + rank * THREADS + threadIdx.x; e < e1; e += 4 * step) {
+      int2 c[4];
+      T w[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const bool there = e1 - e > q * step;
-      c[q] = there ? A.entries[e + q * step] : make_int2(i, -1);
-      w[q] = there && A.entry_w ? (T)A.entry_w[e + q * step] : (T)1;
+      for (int q = 0; q < 4; ++q) {
+        const bool there = e1 - e > q * step;
+        c[q] = there ? A.entries[e + q * step] : make_int2(i, -1);
+        w[q] = there && A.entry_w ? (T)A.entry_w[e + q * step] : (T)1;
+      }
+      const Lean<T> o[4] = {lean(A, c[0].x & 0x7fffffff), lean(A, c[1].x & 0x7fffffff), lean(A, c[2].x & 0x7fffffff),
+                            lean(A, c[3].x & 0x7fffffff)};
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (c[q].y >= 0) add_entry(A, c[q], w[q], own, o[q], math, &g, &h);
     }
-    const Lean<T> o[4] = {lean(A, c[0].x & 0x7fffffff), lean(A, c[1].x & 0x7fffffff), lean(A, c[2].x & 0x7fffffff),
-                          lean(A, c[3].x & 0x7fffffff)};
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (c[q].y >= 0) add_entry(A, c[q], w[q], own, o[q], math, &g, &h);
-  }
-  for (int k = 16; k > 0; k >>= 1) {
-    g += __shfl_xor_sync(0xffffffffu, g, k);
-    h += __shfl_xor_sync(0xffffffffu, h, k);
-  }
-  if ((threadIdx.x & 31) == 0) {
-    sm[0][threadIdx.x >> 5] = g;
-    sm[1][threadIdx.x >> 5] = h;
-  }
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    double t = 0.0;
-    for (int k = 0; k < kLongThreads / 32; ++k) t += sm[threadIdx.x][k];
-    sum[threadIdx.x] = t;
-  }
-  if (blocks > 1) cluster.sync();
-  if (rank == 0 && threadIdx.x < 2 && A.grad) {
-    double t = 0.0;
-    for (int k = 0; k < blocks; ++k) t += *cluster.map_shared_rank(&sum[threadIdx.x], k);
-    (threadIdx.x ? A.hess : A.grad)[i] = (float)t;
+    for (int k = 16; k > 0; k >>= 1) {
+      g += __shfl_xor_sync(0xffffffffu, g, k);
+      h += __shfl_xor_sync(0xffffffffu, h, k);
+    }
+    if ((threadIdx.x & 31) == 0) {
+      sm[parity][0][threadIdx.x >> 5] = g;
+      sm[parity][1][threadIdx.x >> 5] = h;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      double t = 0.0;
+      for (int k = 0; k < THREADS / 32; ++k) t += sm[parity][threadIdx.x][k];
+      sum[parity][threadIdx.x] = t;
+    }
+    if (blocks > 1) cluster.sync();
+    if (rank == 0 && threadIdx.x < 2 && A.grad) {
+      double t = 0.0;
+      for (int k = 0; k < blocks; ++k) t += *cluster.map_shared_rank(&sum[parity][threadIdx.x], k);
+      (threadIdx.x ? A.hess : A.grad)[i] = (float)t;
+    }
   }
   if (blocks > 1) cluster.sync();  // until the first block has read the sums
   wait_for_previous();
@@ -1626,6 +1645,7 @@ void launch_preference_t(const PreferencePlan& plan, const PreferenceTerms& t, c
   A.zero_pairs = plan.zero_pairs;
   A.n_zero = (int)plan.n_zero;
   A.n_items = (int)plan.n_items;
+  A.long_from = PreferencePlan::long_from(plan.n_entries, plan.n_items);
   A.s = static_cast<const T*>(t.scores);
   A.ref = static_cast<const T*>(t.reference);
   A.pm = {t.beta, t.smoothing, 1.0 / (2.0 * t.beta), t.kind};
@@ -1635,16 +1655,19 @@ void launch_preference_t(const PreferencePlan& plan, const PreferenceTerms& t, c
   // long items first: they take longest
   const bool huge = plan.n_huge > 0, any = huge || plan.n_long > 0;
   if (huge)
-    launch_pairs(k_preference_long<T>, (unsigned)plan.n_huge * kPairCluster, kLongThreads, kPairCluster, false, st, A,
-                 (const int*)plan.huge_items);
+    launch_pairs(k_preference_long<T, kHugeThreads>,
+                 (unsigned)std::min<long long>(plan.n_huge, multiprocessors() / 4) * kPairCluster, kHugeThreads,
+                 kPairCluster, false, st, A, (const int*)plan.huge_items, (int)plan.n_huge);
   if (plan.n_long > 0)
-    launch_pairs(k_preference_long<T>, (unsigned)plan.n_long, kLongThreads, 1, huge, st, A, (const int*)plan.long_items);
-  // about as many lanes as half of the mean number of pairs
-  const long long mean = plan.n_entries / plan.n_items;
-  if (mean < 4) launch_preference_items<T, 1>(A, any, st);
-  else if (mean < 16) launch_preference_items<T, 4>(A, any, st);
-  else if (mean < 48) launch_preference_items<T, 16>(A, any, st);
-  else launch_preference_items<T, 32>(A, any, st);
+    launch_pairs(k_preference_long<T, kLongThreads>,
+                 (unsigned)std::min<long long>(plan.n_long, 8ll * multiprocessors()), kLongThreads, 1, huge, st, A,
+                 (const int*)plan.long_items, (int)plan.n_long);
+  switch (pair_lanes(plan.n_entries / plan.n_items)) {
+    case 1: launch_preference_items<T, 1>(A, any, st); break;
+    case 4: launch_preference_items<T, 4>(A, any, st); break;
+    case 8: launch_preference_items<T, 8>(A, any, st); break;
+    default: launch_preference_items<T, 32>(A, any, st);
+  }
 }
 
 }  // namespace
@@ -1792,10 +1815,11 @@ void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const 
   }
   off[ni] = (int)total;
   std::vector<int> lng, huge;
+  const int from = long_from(total, ni);
   for (long long i = 0; i < ni; ++i) {
     const int d = off[i + 1] - off[i];
-    if (d > kHuge) huge.push_back((int)i);
-    else if (d > kLong) lng.push_back((int)i);
+    if (d < from) continue;
+    (d >= std::max(kHuge, from) ? huge : lng).push_back((int)i);
   }
   // one allocation, each array on 256 bytes
   MTB_CUDA_FB(cudaGetDevice(&device));
