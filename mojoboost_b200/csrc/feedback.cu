@@ -421,12 +421,12 @@ __device__ __forceinline__ void bulk_out(void* global, const void* shared, int b
                : "memory");
 }
 
-// Starts the copy of `rows` rows of K elements, row_stride apart, into shared
-// memory; rows_wait ends it.  The whole warp calls both.  vec: the rows are
+// Starts the copy of `rows` rows, row_stride apart, into shared memory (`at`
+// walks over their elements); rows_wait ends it.  The whole warp calls both.  vec: the rows are
 // one piece of global memory that starts on 16 bytes, copied whole, or row by
 // row where they lie apart in shared memory.
 template <typename E>
-__device__ __forceinline__ void rows_in(const E* global, unsigned char* tile, TileRows R, int rows, int K,
+__device__ __forceinline__ void rows_in(const E* global, unsigned char* tile, TileRows R, int rows, RowWalk at,
                                         long long row_stride, bool vec, unsigned long long* barrier) {
   const int lane = threadIdx.x & 31;
   if (vec) {
@@ -440,10 +440,9 @@ __device__ __forceinline__ void rows_in(const E* global, unsigned char* tile, Ti
     } else {
       if (lane == 0 && bytes) bulk_in(tile, global, bytes, barrier);
       const int j = bytes / (int)sizeof(E) + lane;  // fewer than 16 bytes are left
-      if (j < rows * K) reinterpret_cast<E*>(tile)[j] = global[j];
+      if (j < rows * at.width) reinterpret_cast<E*>(tile)[j] = global[j];
     }
   } else {
-    RowWalk at(lane, K);
     while (at.row < rows) {  // four loads in flight
       E x[4];
       E* to[4];
@@ -478,8 +477,8 @@ __device__ __forceinline__ bool rows_wait(bool vec, unsigned long long* barrier,
 // Rows from shared memory to global memory, elements row_stride and
 // class_stride apart; vec as above.  The whole warp calls it, after writing
 // the rows; out_wait before they are overwritten.
-template <typename E>
-__device__ __forceinline__ void rows_out(E* global, const unsigned char* tile, TileRows R, int rows, int K,
+template <int ROWS, typename E>
+__device__ __forceinline__ void rows_out(E* global, const unsigned char* tile, TileRows R, int rows, RowWalk at,
                                          long long row_stride, long long class_stride, bool vec) {
   const int lane = threadIdx.x & 31;
   if (vec) {
@@ -489,14 +488,16 @@ __device__ __forceinline__ void rows_out(E* global, const unsigned char* tile, T
     } else {
       if (lane == 0 && bytes) bulk_out(global, tile, bytes);
       const int j = bytes / (int)sizeof(E) + lane;
-      if (j < rows * K) global[j] = reinterpret_cast<const E*>(tile)[j];
+      if (j < rows * at.width) global[j] = reinterpret_cast<const E*>(tile)[j];
     }
   } else if (class_stride == 1) {
-    for (RowWalk at(lane, K); at.row < rows; at.next())
+    for (; at.row < rows; at.next())
       global[at.row * row_stride + at.col] = reinterpret_cast<const E*>(tile + at.row * R.stride)[at.col];
   } else {  // classes apart: rows next to each other
-    for (RowWalk at(lane, rows); at.row < K; at.next())
-      global[at.col * row_stride + at.row * class_stride] = reinterpret_cast<const E*>(tile + at.col * R.stride)[at.row];
+    const int row = lane % ROWS;
+    if (row < rows)
+      for (int k = lane / ROWS; k < at.width; k += 32 / ROWS)
+        global[row * row_stride + k * class_stride] = reinterpret_cast<const E*>(tile + row * R.stride)[k];
   }
 }
 
@@ -557,6 +558,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
   unsigned char* tile = small_smem + (threadIdx.x >> 5) * (2 * lay.tile);
   int other = lay.tile;  // from this batch's tile to the next one's
   const TileRows in_rows(K * (int)sizeof(T)), out_rows(K * (int)sizeof(Out));
+  const RowWalk walk(lane, K);
   const long long step = (long long)gridDim.x * (kSmallThreads / 32) * kRows;
   long long base = ((long long)blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5)) * kRows;
   auto rows_at = [&](long long b) { return (int)max(0ll, min((long long)kRows, A.in.n - b)); };
@@ -569,7 +571,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
   __syncwarp();
   RowValues next = load_row<OP>(A, base + i, i < rows_at(base));
   if (base < A.in.n)
-    rows_in(A.in.scores + base * A.in.stride, tile, in_rows, rows_at(base), K, A.in.stride, lay.vec_in, barrier);
+    rows_in(A.in.scores + base * A.in.stride, tile, in_rows, rows_at(base), walk, A.in.stride, lay.vec_in, barrier);
   unsigned turn = 0;  // bit 0: the tile's barrier, bit 1: its phase
   for (; base < A.in.n; base += step, tile += other, other = -other, turn = (turn + 1) & 3) {
     const int rows = rows_at(base);
@@ -650,7 +652,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
     out_wait();
     __syncwarp();
     if (base + step < A.in.n)
-      rows_in(A.in.scores + (base + step) * A.in.stride, tile + other, in_rows, rows_at(base + step), K, A.in.stride,
+      rows_in(A.in.scores + (base + step) * A.in.stride, tile + other, in_rows, rows_at(base + step), walk, A.in.stride,
               lay.vec_in, barrier + (turn + 1 & 1));
 
     if (OP == ROW_LOGPROBS) {
@@ -731,9 +733,9 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     const long long to = base * A.out.row_stride;
-    rows_out(A.out.grad + to, tile, out_rows, rows, K, A.out.row_stride, A.out.class_stride, lay.vec_out);
+    rows_out<kRows>(A.out.grad + to, tile, out_rows, rows, walk, A.out.row_stride, A.out.class_stride, lay.vec_out);
     if (want_h)
-      rows_out(A.out.hess + to, tile_h, out_rows, rows, K, A.out.row_stride, A.out.class_stride, lay.vec_out);
+      rows_out<kRows>(A.out.hess + to, tile_h, out_rows, rows, walk, A.out.row_stride, A.out.class_stride, lay.vec_out);
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     __syncwarp();
   }
