@@ -74,7 +74,7 @@ def sum_error(K, p, d, f64):
     """Bound of the relative error of a row's sum: each term's own, and the
     additions of n positive terms one after the other in the scores'
     arithmetic, which change the sum by at most (n - 1) half steps.  Rows of up
-    to 128 classes: at most 16 terms in a lane, then 3 sums of lanes; longer
+    to 128 (float64: 512) classes: at most 16 terms in a lane, then 5 sums of lanes; longer
     rows: ceil(K / 256) in a thread, and float64 across threads."""
     terms = (p * exp_error(d, f64)).sum(1)
     return terms + (min(K, 16) + K // 256 + 4) * (2.0 ** -53 if f64 else U32)
