@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
   using Row = typename Types<T>::Row;
   constexpr int N = Vec<T>::N, kWarps = THREADS / 32;
   __shared__ LargeShared<THREADS> S;
-  const TableMath math(S.tables);
+  const TableMath math(S.tables, OP != ROW_BACK);
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -520,7 +520,8 @@ void launch_large_h(const RowArgs<T>& A, int blocks, int per, cudaStream_t st) {
   else if (per > 1024) launch_large_t<T, OP, HESS, 512, 4>(A, blocks, per, st);
   else if (per > 512) launch_large_t<T, OP, HESS, 256, 4>(A, blocks, per, st);
   else if (per > 128) launch_large_t<T, OP, HESS, 128, 4>(A, blocks, per, st);
-  else launch_large_t<T, OP, HESS, 32, 4>(A, blocks, per, st);
+  else if (per > 32) launch_large_t<T, OP, HESS, 32, 4>(A, blocks, per, st);
+  else launch_large_t<T, OP, HESS, 32, 1>(A, blocks, per, st);
 }
 
 // False when a row does not fit a cluster's registers, or its derivatives are
