@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <math.h>
 
+#include <algorithm>
 #include <atomic>
 #include <stdexcept>
 #include <string>
@@ -144,6 +145,24 @@ int multiprocessors() {
   MTB_CUDA_FB(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
   if (dev < kMostDevices) known[dev].store(n, std::memory_order_relaxed);
   return n;
+}
+
+// Blocks of a kernel that an SM holds at once, for the grids of kernels whose
+// blocks loop: each block's start (tables, the first rows' way from memory)
+// is paid once.  The registers are asked for once per kernel.
+template <typename K>
+int resident_blocks(K kernel, int threads, size_t dynamic_smem, std::atomic<int>& known) {
+  int packed = known.load(std::memory_order_relaxed);  // registers a thread, and static shared memory in 16 bytes
+  if (packed == 0) {
+    cudaFuncAttributes a;
+    MTB_CUDA_FB(cudaFuncGetAttributes(&a, kernel));
+    packed = a.numRegs | (int)((a.sharedSizeBytes + 15) / 16) << 8;
+    known.store(packed, std::memory_order_relaxed);
+  }
+  const int warps = threads / 32, regs = ((packed & 255) + 7) / 8 * 8 * 32 * warps;
+  const size_t smem = dynamic_smem + 16 * (size_t)(packed >> 8) + 1024;
+  const int by_smem = (int)(228 * 1024 / smem);
+  return std::max(1, std::min(std::min(65536 / regs, by_smem), std::min(64 / warps, 32)));
 }
 
 }  // namespace

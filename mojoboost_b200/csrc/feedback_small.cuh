@@ -404,8 +404,10 @@ void launch_small_t(const RowArgs<T>& A, cudaStream_t st) {
   lay.vec_out = on16(A.out.grad) && on16(A.out.hess) && A.out.row_stride == K && A.out.class_stride == 1 &&
                 rows * out.bytes % 16 == 0;
   const long long blocks = (A.in.n + rows * warps - 1) / (rows * warps);
-  const unsigned grid = (unsigned)std::min<long long>(blocks, 16ll * multiprocessors());
-  k_feedback_small<T, OP, L, P><<<grid, kSmallThreads, (size_t)lay.tile * 2 * warps, st>>>(A, lay);
+  const size_t smem = (size_t)lay.tile * 2 * warps;
+  static std::atomic<int> known{0};
+  const long long most = (long long)multiprocessors() * resident_blocks(k_feedback_small<T, OP, L, P>, kSmallThreads, smem, known);
+  k_feedback_small<T, OP, L, P><<<(unsigned)std::min(blocks, most), kSmallThreads, smem, st>>>(A, lay);
 }
 
 // Few classes fit one lane; a class too many in P costs a float64 exponential
