@@ -218,6 +218,33 @@ def _policy_rows(seed, n, f64, logp, with_ref, with_w):
     return adv, old, ref, w
 
 
+def _check_policy(got, z, a, adv, old, ref, w, low, high, kl, dtype):
+    """policy_loss's four outputs against the plain form on float64 scores z."""
+    n, f64 = len(z), dtype == "float64"
+    wide = [None if v is None else v.astype(np.float64) for v in (adv, old, ref, w)]
+    logp, stats, p, left, part = fu.softmax_rows(z, a, wide[3])
+    loss, g, h, part2 = fu.policy_rows(logp, part, *wide, low, high, kl)
+    e_l, e_p, e_left = _row_bounds(z, p, stats, logp, f64)
+    unit = 2.0 ** -53 if f64 else fu.U32
+    l = np.where(part2, logp, 0.0)
+    ww = np.where(part2, 1.0 if w is None else wide[3], 0.0)
+    ra = np.abs(np.exp(l - wide[1]) * wide[0])
+    et = np.exp(wide[2] - l) if ref is not None else np.zeros(n)
+    # a rounded step of the float64 scalars: exp of a sum of a few units
+    step = 2.0 ** -50 * (1 + np.abs(l) + np.abs(wide[1]))
+    e_g = ww * ((ra + kl * et) * (e_l * 1.01 + step))
+    _close(got[1], logp, e_l, "logp")
+    _close(got[0], loss, (np.abs(g) + e_g) * e_l + ww * (ra + kl * (et + 1 + np.abs(l) + np.abs(wide[2] if ref is not None else 0))) * step
+           + np.abs(loss) * unit * 2 + TINY["float32"], "loss")
+    G, H, q = fu.to_scores(p, left, a, part2, g, h)
+    tol_q = np.where(q > 0, np.maximum(e_left[:, None], e_p), e_p)
+    half, tiny = HALF_STEP[dtype], TINY[dtype]
+    eg, unit_c = e_g[:, None] * 1.01, 4 * unit
+    _close(got[2], G, (np.abs(q) * eg + np.abs(G) * (tol_q + half + unit_c)) * 1.01 + tiny, "grad")
+    if got[3] is not None:
+        _close(got[3], H, ((q * q + p * left) * 2 * eg + H * (2 * tol_q + e_p + e_left[:, None] + half + unit_c)) * 1.02 + tiny, "hess")
+
+
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,K", SIZES)
@@ -235,27 +262,7 @@ def test_policy_loss(mtlib, n, K, dtype):
         if n == 0:
             assert got[2].shape == (0, K)
             continue
-        wide = [None if v is None else v.astype(np.float64) for v in (adv, old, ref, w)]
-        logp, stats, p, left, part = fu.softmax_rows(z, a, wide[3])
-        loss, g, h, part2 = fu.policy_rows(logp, part, *wide, low, high, kl)
-        e_l, e_p, e_left = _row_bounds(z, p, stats, logp, f64)
-        unit = 2.0 ** -53 if f64 else fu.U32
-        l = np.where(part2, logp, 0.0)
-        ww = np.where(part2, 1.0 if w is None else wide[3], 0.0)
-        ra = np.abs(np.exp(l - wide[1]) * wide[0])
-        et = np.exp(wide[2] - l) if ref is not None else np.zeros(n)
-        # a rounded step of the float64 scalars: exp of a sum of a few units
-        step = 2.0 ** -50 * (1 + np.abs(l) + np.abs(wide[1]))
-        e_g = ww * ((ra + kl * et) * (e_l * 1.01 + step))
-        _close(got[1], logp, e_l, "logp")
-        _close(got[0], loss, (np.abs(g) + e_g) * e_l + ww * (ra + kl * (et + 1 + np.abs(l) + np.abs(wide[2] if ref is not None else 0))) * step
-               + np.abs(loss) * unit * 2 + TINY["float32"], "loss")
-        G, H, q = fu.to_scores(p, left, a, part2, g, h)
-        tol_q = np.where(q > 0, np.maximum(e_left[:, None], e_p), e_p)
-        half, tiny = HALF_STEP[dtype], TINY[dtype]
-        eg, unit_c = e_g[:, None] * 1.01, 4 * unit
-        _close(got[2], G, (np.abs(q) * eg + np.abs(G) * (tol_q + half + unit_c)) * 1.01 + tiny, "grad")
-        _close(got[3], H, ((q * q + p * left) * 2 * eg + H * (2 * tol_q + e_p + e_left[:, None] + half + unit_c)) * 1.02 + tiny, "hess")
+        _check_policy(got, z, a, adv, old, ref, w, low, high, kl, dtype)
         alone = mtlib.policy_loss(x, a_t, args[0], args[1], ref_logp=args[2], weights=args[3], clip_low=low,
                                   clip_high=high, kl_coef=kl, grad=False)
         assert alone[2] is None and alone[3] is None
@@ -572,3 +579,128 @@ def test_preference_through_class_scores(mtlib):
     size = g.abs().double()[:, None].expand(n, K)
     assert ((G.double() - y.grad).abs() <= 2.1 * fu.U32 * size + 1e-12).all()
     assert (H >= 0).all()
+
+
+# --------------------------------------------- calls that the ones above leave out
+
+@gpu
+@pytest.mark.parametrize("dtype,n,K,out_stride", [
+    ("float64", 70, 10, 13), ("float64", 33, 200, 203), ("float32", 65, 7, 8), ("float32", 9, 300, 304), ("float32", 5, 5000, 5001),
+    ("bfloat16", 40, 50, 57), ("bfloat16", 9, 1000, 1003), ("float16", 7, 4096, 4104), ("float16", 3, 20001, 20011)])
+def test_strided_derivatives_leave_the_rest_alone(mtlib, dtype, n, K, out_stride):
+    """Derivatives written at a row stride of their own: the same values, and
+    what lies between the rows and behind the last keeps its bits."""
+    import torch
+    x, z, a_t, a = _inputs(K, n, K, dtype, mask=True)
+    row = torch.float64 if dtype == "float64" else torch.float32
+    adv = torch.randn(n, device="cuda", dtype=row)
+    old = torch.full((n,), -2.0, device="cuda", dtype=row)
+    loss, logp, want_g, want_h = mtlib.policy_loss(x, a_t, adv, old, hess=True)
+    got = [torch.full((n + 2, out_stride), 7.0, dtype=want_g.dtype, device="cuda") for _ in range(2)]
+    out_loss = torch.full((n + 5,), 7.0, dtype=row, device="cuda")
+    lib = mtlib.lib()
+    e = lib.mojotrees_error_create()
+    kind = DTYPES.index(dtype)
+    rc = lib.mojotrees_b200_policy_loss(x.data_ptr(), kind, n, K, x.stride(0), a_t.data_ptr(), 4, adv.data_ptr(), old.data_ptr(),
+                                        None, None, 0.2, 0.2, 0.0, out_loss.data_ptr(), None, got[0].data_ptr(), got[1].data_ptr(),
+                                        out_stride, torch.cuda.current_stream().cuda_stream, e)
+    assert rc == 0, lib.mojotrees_error_message(e)
+    lib.mojotrees_error_free(e)
+    assert torch.equal(out_loss[:n], loss) and (out_loss[n:] == 7).all()
+    for u, want in zip(got, (want_g, want_h)):
+        assert torch.equal(u[:n, :K], want)
+        assert (u[:n, K:] == 7).all() and (u[n:] == 7).all()
+
+
+@gpu
+def test_first_call_inside_a_capture():
+    """A process whose first calls are captured into a graph, items of many
+    pairs among them; the graph is replayed twice without a wait between."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import numpy as np, torch
+import mojoboost_b200 as mb
+rng = np.random.default_rng(0)
+n = 3000
+i = np.concatenate([np.zeros(40000, int), np.ones(3000, int), rng.integers(2, n, 20000)])
+j = 2 + rng.integers(0, n - 3, i.size); j += j == i
+plan = mb.PreferencePlan(i, j, n)
+s = torch.randn(n, dtype=torch.float64, device="cuda")
+x = torch.randn(300, 1000, device="cuda").half(); a = torch.randint(0, 1000, (300,), device="cuda")
+y = torch.randn(300, 9, dtype=torch.float64, device="cuda"); b = torch.randint(0, 9, (300,), device="cuda", dtype=torch.int32)
+adv = torch.randn(300, device="cuda"); old = torch.full((300,), -7.0, device="cuda")
+torch.cuda.synchronize()
+def run():
+    l, st = mb.action_logprobs(y, b)
+    return [l, *mb.policy_loss(x, a, adv, old)[:3], *mb.preference_loss(plan, s), mb.action_logprobs_grad(y, b, st, adv, adv.abs())[0]]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = run()
+for seed in range(3):
+    s.normal_(); y.normal_(); x.normal_()
+    g.replay(); g.replay()
+    torch.cuda.synchronize()
+    for u, v in zip(out, run()):
+        assert torch.equal(u, v)
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
+@gpu
+@pytest.mark.parametrize("n,K,dtype", [(66_000, 32_769, "bfloat16"), (270_000_000, 8, "float16")])
+def test_offsets_beyond_32_bits(mtlib, n, K, dtype):
+    """Scores of more than 2^31 elements: the last rows as in a call of their own."""
+    import torch
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    x = torch.zeros((n, K), dtype=getattr(torch, dtype), device="cuda")
+    x[-40:] = torch.randn((40, K), device="cuda").to(x.dtype)
+    a = torch.zeros(n, dtype=torch.int32, device="cuda")
+    a[-40:] = torch.randint(0, K, (40,), device="cuda", dtype=torch.int32)
+    adv, old = torch.ones(n, device="cuda"), torch.full((n,), -math.log(K), device="cuda")
+    loss, logp, grad, _ = mtlib.policy_loss(x, a, adv, old)
+    l2, stats = mtlib.action_logprobs(x, a)
+    back, _ = mtlib.action_logprobs_grad(x, a, stats, adv)
+    t = slice(n - 40, n)
+    z, at = x[t].double().cpu().numpy(), a[t].cpu().numpy()
+    rows = [v[t].cpu().numpy() for v in (adv, old)]
+    _check_policy((loss[t], logp[t], grad[t], None), z, at, *rows, None, None, 0.2, 0.2, 0.0, dtype)
+    want_l, want_s, p, left, part = fu.softmax_rows(z, at)
+    e_l, e_p, e_left = _row_bounds(z, p, want_s, want_l, False)
+    _close(l2[t], want_l, e_l, "logp")
+    G, _, q = fu.to_scores(p, left, at, part, rows[0].astype(np.float64), np.zeros(40))
+    tol_q = np.where(q > 0, np.maximum(e_left[:, None], e_p), e_p)
+    _close(back[t], G, np.abs(G) * (tol_q + HALF_STEP[dtype]) * 1.01 + TINY[dtype], "grad")
+    assert (logp[:-40] + math.log(K)).abs().max() < 1e-5
+    del grad, back
+    torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("n,P_", [(1500, 200_000), (40_000, 30_000)])
+def test_preference_loss_alone_and_derivatives_alone(mtlib, n, P_):
+    """The C entry's optional outputs: the loss without derivatives, and the
+    derivatives without the loss (as a fit takes them)."""
+    import torch
+    i, j = _pairs(n, n, P_, "any")
+    i[: P_ // 4], j[: P_ // 4] = 0, 1 + np.arange(P_ // 4) % (n - 1)  # an item of many pairs
+    w = np.random.default_rng(1).random(P_).astype(np.float32)
+    w[::7] = 0
+    plan = mtlib.PreferencePlan(i, j, n, weights=w)
+    s = torch.randn(n, dtype=torch.float64, device="cuda")
+    want = mtlib.preference_loss(plan, s)
+    loss = torch.full_like(want[0], 7)
+    g, h = torch.full_like(want[1], 7), torch.full_like(want[2], 7)
+    lib = mtlib.lib()
+    e = lib.mojotrees_error_create()
+    st = torch.cuda.current_stream().cuda_stream
+    assert lib.mojotrees_b200_preference_loss(plan.h, s.data_ptr(), None, 0, 1.0, 0.0, 0, loss.data_ptr(), None, None, st, e) == 0
+    assert lib.mojotrees_b200_preference_loss(plan.h, s.data_ptr(), None, 0, 1.0, 0.0, 0, None, g.data_ptr(), h.data_ptr(), st, e) == 0
+    assert lib.mojotrees_b200_preference_loss(plan.h, s.data_ptr(), None, 0, 1.0, 0.0, 0, None, None, h.data_ptr(), st, e) == -1
+    lib.mojotrees_error_free(e)
+    assert torch.equal(loss, want[0]) and torch.equal(g, want[1]) and torch.equal(h, want[2])
