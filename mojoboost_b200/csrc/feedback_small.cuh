@@ -191,6 +191,10 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
   using Row = typename Types<T>::Row;
   using Out = typename Types<T>::Out;
   constexpr int kRows = 32 / L;
+  // How many of a lane's classes every row of this variant has (launch_small):
+  // no guards for them.
+  constexpr int kSure = L > 1 ? P / 2 : sizeof(T) == 2 ? 1 : sizeof(T) == 4 ? (P == 4 ? 1 : P / 2 + 1) : P == 16 ? 13 : P - 1;
+  auto has = [&](int e, int l, int K) { return e < kSure || l + e * L < K; };
   // In float64 a sum that holds the 1 of the largest class gives the others'
   // to 2^-43 of it unless it is below 2^-10, far beyond what the float32
   // derivatives keep; the statistics keep it whole.
@@ -238,7 +242,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
     C v[P];
     int top = -1;  // a class of this lane at the maximum
 #pragma unroll
-    for (int e = 0; e < P; ++e) v[e] = l + e * L < K ? (C)widen(z[l + e * L]) : (C)-INFINITY;
+    for (int e = 0; e < P; ++e) v[e] = has(e, l, K) ? (C)widen(z[l + e * L]) : (C)-INFINITY;
     if (OP != ROW_BACK) {
       C mx = v[0];
 #pragma unroll
@@ -292,8 +296,10 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
 #pragma unroll
       for (int e = 0; e < P; ++e) v[e] = math.exp(v[e] - m);
       const bool exact = kExact || rest < kNearOne;
+      if (kExact || __any_sync(0xffffffffu, exact)) {
 #pragma unroll
-      for (int e = 0; e < P; ++e) top = v[e] == (C)1 && exact ? l + e * L : top;
+        for (int e = 0; e < P; ++e) top = v[e] == (C)1 && exact ? l + e * L : top;
+      }
     }
     // the next rows into the other tile, whose derivatives are on their way by now
     out_wait();
@@ -352,12 +358,12 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
       const C down = -g * inv, ag = fabs(g), bend = h - ag;
 #pragma unroll
       for (int e = 0; e < P; ++e)
-        if (l + e * L < K) narrow(v[e] * down, to_g[l + e * L]);
+        if (has(e, l, K)) narrow(v[e] * down, to_g[l + e * L]);
       if (want_h) {
 #pragma unroll
         for (int e = 0; e < P; ++e) {
           const C p = v[e] * inv;
-          if (l + e * L < K) narrow(p * fma(p, bend, ag), to_h[l + e * L]);
+          if (has(e, l, K)) narrow(p * fma(p, bend, ag), to_h[l + e * L]);
         }
       }
       // a class with more than half of the probability is alone at the
