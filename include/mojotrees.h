@@ -395,8 +395,8 @@ int32_t mojotrees_b200_policy_loss(const void *scores, int32_t score_type, int64
  * of calls: item winners[p] was preferred to losers[p] (both in
  * [0, n_items), different), with weights[p] >= 0 (NULL: 1); host arrays,
  * copied.  gpu_device_id -1: the current device.  The plan is not changed by
- * calls that use it, which may overlap; free it when none is running and no
- * graph holds one. */
+ * calls that use it, which may overlap; free it when no graph holds one
+ * (freeing waits for the device's work).  Neither may run during a capture. */
 typedef struct MojoTreesPreferencePlan MojoTreesPreferencePlan;
 int32_t mojotrees_b200_preference_plan_create(const int64_t *winners, const int64_t *losers, const float *weights,
                                               int64_t n_pairs, int64_t n_items, int32_t gpu_device_id,

@@ -4,6 +4,7 @@
 // points (feedback.cu) and the trainer.
 #pragma once
 #include <cuda_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #include <vector>
@@ -70,6 +71,7 @@ struct PreferencePlan {
   int* huge_items = nullptr;
   long long n_zero = 0, n_long = 0, n_huge = 0;
   void* memory = nullptr;
+  size_t memory_bytes = 0;
   PreferencePlan() = default;
   PreferencePlan(const PreferencePlan&) = delete;
   PreferencePlan& operator=(const PreferencePlan&) = delete;

@@ -1,6 +1,7 @@
 // The paired preference loss with its gradient and hessian, and the plan of
 // its pairs.
 #include <cooperative_groups.h>
+#include <string.h>
 
 #include <algorithm>
 #include <cmath>
@@ -10,6 +11,7 @@
 
 #include "feedback.h"
 #include "feedback_math.cuh"
+#include "trainer.h"
 
 namespace mtb {
 namespace {
@@ -331,7 +333,15 @@ void launch_preference_t(const PreferencePlan& plan, const PreferenceTerms& t, c
 
 }  // namespace
 
-PreferencePlan::~PreferencePlan() { cudaFree(memory); }
+// The memory comes from the fits' cache: allocating and freeing took 0.6 ms a
+// plan, more than the loss of most batches.
+PreferencePlan::~PreferencePlan() {
+  if (!memory) return;
+  int before = -1;
+  const bool known = cudaGetDevice(&before) == cudaSuccess;
+  if (cudaSetDevice(device) == cudaSuccess) give_device_memory(memory, memory_bytes);
+  if (known) cudaSetDevice(before);
+}
 
 void PreferencePlan::check(const int64_t* winners, const int64_t* losers, const float* weights, long long np,
                            long long ni) {
@@ -388,7 +398,8 @@ void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const 
   start[kRanges] = total;
   for (int t = 0; t < parts; ++t) zero_at[t + 1] = zero_at[t] + zeros[t];
   std::unique_ptr<Entry[]> sorted(new Entry[std::max(1ll, total)]);
-  std::vector<int> zero((size_t)zero_at[parts]), off((size_t)ni + 1);
+  std::vector<int> zero((size_t)zero_at[parts]);
+  std::unique_ptr<int[]> off(new int[(size_t)ni + 1]);
   std::unique_ptr<int2[]> ent(new int2[std::max(1ll, total)]);
   std::unique_ptr<float[]> ew(new float[weights ? std::max(1ll, total) : 1]);
 #pragma omp parallel for schedule(static, 1) if (parts > 1)
@@ -406,6 +417,8 @@ void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const 
       sorted[c[b / range]++] = {b, make_int2(a | (int)0x80000000, (int)p), w};
     }
   }
+  const int from = long_from(total, ni);
+  std::vector<int> lng_of[kRanges], huge_of[kRanges];
 #pragma omp parallel for schedule(dynamic, 1) if (parts > 1)
   for (int q = 0; q < kRanges; ++q) {
     const long long i0 = std::min(ni, q * range), i1 = std::min(ni, i0 + range);
@@ -418,6 +431,7 @@ void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const 
       const int n = at[i - i0 + 1];
       at[i - i0] = sum;
       sum += n;
+      if (n >= from) (n >= std::max(kHuge, from) ? huge_of : lng_of)[q].push_back((int)i);
     }
     for (long long e = start[q]; e < start[q + 1]; ++e) {
       const int to = at[sorted[e].item - i0]++;
@@ -427,11 +441,9 @@ void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const 
   }
   off[ni] = (int)total;
   std::vector<int> lng, huge;
-  const int from = long_from(total, ni);
-  for (long long i = 0; i < ni; ++i) {
-    const int d = off[i + 1] - off[i];
-    if (d < from) continue;
-    (d >= std::max(kHuge, from) ? huge : lng).push_back((int)i);
+  for (int q = 0; q < kRanges; ++q) {
+    lng.insert(lng.end(), lng_of[q].begin(), lng_of[q].end());
+    huge.insert(huge.end(), huge_of[q].begin(), huge_of[q].end());
   }
   // one allocation, each array on 256 bytes
   MTB_CUDA_FB(cudaGetDevice(&device));
@@ -446,13 +458,21 @@ void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const 
     bytes += (n + 255) / 256 * 256;
     return copies.back().at;
   };
-  const size_t at_off = add(off.data(), 4 * off.size()), at_ent = add(ent.get(), 8 * (size_t)total),
+  const size_t at_off = add(off.get(), 4 * ((size_t)ni + 1)), at_ent = add(ent.get(), 8 * (size_t)total),
                at_w = add(ew.get(), weights ? 4 * (size_t)total : 0), at_zero = add(zero.data(), 4 * zero.size()),
                at_long = add(lng.data(), 4 * lng.size()), at_huge = add(huge.data(), 4 * huge.size());
-  MTB_CUDA_FB(cudaMalloc(&memory, bytes));
+  memory_bytes = bytes;
+  memory = take_device_memory(&memory_bytes);
   char* base = static_cast<char*>(memory);
-  for (const Copy& c : copies)
-    if (c.n) MTB_CUDA_FB(cudaMemcpy(base + c.at, c.from, c.n, cudaMemcpyHostToDevice));
+  if (bytes <= 1 << 20) {  // a copy costs more than its bytes
+    std::vector<char> all(bytes);
+    for (const Copy& c : copies)
+      if (c.n) memcpy(&all[c.at], c.from, c.n);
+    MTB_CUDA_FB(cudaMemcpy(base, all.data(), bytes, cudaMemcpyHostToDevice));
+  } else {
+    for (const Copy& c : copies)
+      if (c.n) MTB_CUDA_FB(cudaMemcpy(base + c.at, c.from, c.n, cudaMemcpyHostToDevice));
+  }
   n_items = ni;
   n_pairs = np;
   n_entries = total;

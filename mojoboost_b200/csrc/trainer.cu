@@ -198,6 +198,13 @@ struct EventTimer {
 
 }  // namespace
 
+void* take_device_memory(size_t* bytes) {
+  *bytes = (*bytes + (2u << 20) - 1) & ~(size_t)((2u << 20) - 1);
+  return DeviceCache::get().take(*bytes);
+}
+
+void give_device_memory(void* p, size_t bytes) { DeviceCache::get().give(p, bytes); }
+
 void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
   const long long N = in.n_rows;
   const int F = in.n_features;

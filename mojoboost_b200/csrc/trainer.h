@@ -1,5 +1,7 @@
 // GPU trainer entry point (host side).
 #pragma once
+#include <stddef.h>
+
 #include <stdexcept>
 #include <string>
 
@@ -58,6 +60,12 @@ struct BinnedInput {
 // Trains on the current (or configured) CUDA device; fills model.trees,
 // base_scores and stats.  Throws Unsupported or std::runtime_error.
 void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model);
+
+// Device memory of the per-process cache that fits take theirs from, on the
+// current device: `bytes` is rounded up to what the block holds.  Returning a
+// block, on the device it came from, waits for the device's work.
+void* take_device_memory(size_t* bytes);
+void give_device_memory(void* p, size_t bytes);
 
 // Number of CUDA devices visible (0 when the driver or a device is absent).
 int cuda_device_count();
