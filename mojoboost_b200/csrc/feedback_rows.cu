@@ -26,7 +26,9 @@ namespace {
 
 // ---------------------------------------------------------------------------
 // Any rows: float64 scores of more than 512 classes, and rows that a cluster's
-// registers do not hold
+// registers do not hold (float32 of more than 262000).  Three passes, the
+// later ones out of L2: 8192 x 32768 bfloat16 took 690 us this way, 242 in
+// registers.
 // ---------------------------------------------------------------------------
 
 constexpr int kRowThreads = 256;

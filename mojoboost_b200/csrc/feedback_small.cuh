@@ -16,6 +16,16 @@ namespace {
 // in one piece per warp.  With L = 1 (up to 16 classes) no lane waits for
 // another.  A row's float64 scalars, a logarithm, two exponentials and a
 // quotient, cost as much as ten classes; every lane of a row computes them.
+//
+// Measured, policy loss with gradient and hessian of 4M x 10 float64 (816 MB,
+// 125 us at the copy rate): 189 us.  Bound is the issue of instructions, 62%
+// of the slots with a quarter of the warps an SM could hold: about 1050 for 32
+// rows, a third of them float64.  A block per row took 20.2 ms; rows spread
+// over four lanes' registers 396 us; a branch per class 309 us, and classes
+// fixed at compile time with the next rows' copy in flight 224 us, since a
+// lane's exponentials then overlap; bulk copies and the branch-free functions
+// of TableMath 195 us.  Fewer registers for five or six blocks an SM instead
+// of four cost 10 and 13%.
 // ---------------------------------------------------------------------------
 
 constexpr int kSmallThreads = 128;
