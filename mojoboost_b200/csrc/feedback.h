@@ -14,8 +14,7 @@ namespace mtb {
 enum ScoreType : int { SCORE_F64 = 0, SCORE_F32 = 1, SCORE_F16 = 2, SCORE_BF16 = 3 };
 enum PreferenceKind : int { PREFERENCE_LOGISTIC = 0, PREFERENCE_SQUARED = 1 };
 
-// Most classes of a row: bounds how many terms a thread of the row kernels adds
-// in float32 (see border_slack in feedback_rows.cuh).
+// Most classes of a row: what a cluster's registers hold in float32.
 constexpr long long kMaxClasses = 1 << 18;
 
 // Scores [n][K] (rows `stride` elements apart, classes next to each other)

@@ -524,20 +524,18 @@ void launch_large_h(const RowArgs<T>& A, int blocks, int per, cudaStream_t st) {
   else launch_large_t<T, OP, HESS, 32, 1>(A, blocks, per, st);
 }
 
-// False when a row does not fit a cluster's registers, or its derivatives are
-// not next to each other.
+// Derivatives next to each other (class_stride 1), as every caller with such
+// scores has them.
 template <typename T, int OP>
-bool launch_large(const RowArgs<T>& A, cudaStream_t st) {
+void launch_large(const RowArgs<T>& A, cudaStream_t st) {
   const int vecs = A.in.K / Vec<T>::N;  // or one fewer, where a row does not start on 16 bytes
-  if (OP != ROW_LOGPROBS && A.out.grad && A.out.class_stride != 1) return false;
+  static_assert(kMaxClasses / 4 <= 8 * 8192, "a cluster's registers hold the longest float32 row");
   int blocks = 1;
   while (blocks < 8 && (vecs > 8192 * blocks || (vecs > 512 * blocks && A.in.n * blocks * 2 <= multiprocessors()))) blocks *= 2;
   const int per = (vecs + blocks - 1) / blocks;
-  if (per > 8192) return false;
   if constexpr (OP == ROW_LOGPROBS) launch_large_h<T, OP, false>(A, blocks, per, st);
   else if (A.out.hess) launch_large_h<T, OP, true>(A, blocks, per, st);
   else launch_large_h<T, OP, false>(A, blocks, per, st);
-  return true;
 }
 
 }  // namespace

@@ -25,30 +25,19 @@ namespace mtb {
 namespace {
 
 // ---------------------------------------------------------------------------
-// Any rows: float64 scores of more than 512 classes, and rows that a cluster's
-// registers do not hold (float32 of more than 262000).  Three passes, the
-// later ones out of L2: 8192 x 32768 bfloat16 took 690 us this way, 242 in
-// registers.
+// float64 scores of more than 512 classes: a trained model has 64 at most, so
+// these rows stay with the simplest kernel.  Three passes, the later ones out
+// of L2 (2000 x 2000, log probabilities: 21 us).
 // ---------------------------------------------------------------------------
 
 constexpr int kRowThreads = 256;
 
-// Derivatives at class k from e = exp(z_k - m) and the row's sum.  e is 1 for
-// a class at the maximum (or one so near to it that its term of the sum is 1).
-template <typename C>
-__device__ __forceinline__ void derivative(C e, C inv_total, C rest_share, bool taken, C g, C h, bool want_h, C* grad,
-                                           C* hess) {
-  const C p = e * inv_total;
-  const C left = e == (C)1 ? rest_share : (C)1 - p;  // 1 - p
-  const C q = taken ? left : -p;
-  *grad = g * q;
-  if (want_h) *hess = h * q * q + fabs(g) * p * left;
-}
-
 __device__ __forceinline__ double add_f64(double a, double b) { return a + b; }
 
-template <typename V, typename F>
-__device__ __forceinline__ V block_reduce(V v, V* sm, F f) {
+__device__ __forceinline__ double max_f64(double a, double b) { return (b > a || b != b) ? b : a; }  // NaN when either is
+
+template <typename F>
+__device__ __forceinline__ double block_reduce(double v, double* sm, F f) {
   for (int k = 16; k > 0; k >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, k));
   __syncthreads();
   if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
@@ -60,95 +49,77 @@ __device__ __forceinline__ V block_reduce(V v, V* sm, F f) {
 
 // One block per row: the maximum, the sum, the derivatives, each a pass over
 // the row.
-template <typename T, int OP>
-__global__ void __launch_bounds__(kRowThreads) k_feedback_rows(const RowArgs<T> A) {
-  using C = typename Types<T>::C;
-  using Row = typename Types<T>::Row;
-  __shared__ C sm_c[kRowThreads / 32];
-  __shared__ double sm_d[kRowThreads / 32];
+template <int OP>
+__global__ void __launch_bounds__(kRowThreads) k_feedback_rows(const RowArgs<double> A) {
+  __shared__ double sm[kRowThreads / 32];
   const int K = A.in.K;
   for (long long r = blockIdx.x; r < A.in.n; r += gridDim.x) {
-    const T* z = A.in.scores + r * A.in.stride;
+    const double* z = A.in.scores + r * A.in.stride;
     const long long a = A.in.action(r);
     const bool bad = a >= K;
     bool part = a >= 0;
-    if (OP == ROW_POLICY && A.pol.weights) part = part && A.pol.weights[r] != (Row)0;
-    C m = 0;
-    double rest = -1.0;
+    if (OP == ROW_POLICY && A.pol.weights) part = part && A.pol.weights[r] != 0.0;
+    double m = 0.0, rest = -1.0;
     if (OP == ROW_BACK) {
       m = A.stats[2 * r];
-      rest = (double)A.stats[2 * r + 1];
+      rest = A.stats[2 * r + 1];
       part = part && rest != -1.0;
     } else if (part && !bad) {
-      C mx = -INFINITY;
-      for (int k = threadIdx.x; k < K; k += kRowThreads) mx = max_nan<C>(mx, widen(z[k]));
-      mx = block_reduce(mx, sm_c, max_nan<C>);
-      if (mx == (C)-INFINITY) {
+      double mx = -INFINITY;
+      for (int k = threadIdx.x; k < K; k += kRowThreads) mx = max_f64(mx, z[k]);
+      mx = block_reduce(mx, sm, max_f64);
+      if (mx == -INFINITY) {
         part = false;
       } else {
         m = mx;
-        C s = 0;
-        int ties = 0;
+        double s = 0.0, ties = 0.0;
         for (int k = threadIdx.x; k < K; k += kRowThreads) {
-          const C e = exp_c((C)widen(z[k]) - m);
-          if (e != (C)1) s += e;
-          else ++ties;
+          const double e = exp(z[k] - m);
+          if (e != 1.0) s += e;
+          else ties += 1.0;
         }
-        const double others = block_reduce((double)s, sm_d, add_f64);
-        rest = others + (block_reduce((double)ties, sm_d, add_f64) - 1.0);
+        s = block_reduce(s, sm, add_f64);
+        rest = s + (block_reduce(ties, sm, add_f64) - 1.0);
       }
     }
     RowDerivative row = {0.0, 0.0};
-    if (OP == ROW_LOGPROBS) {
-      if (threadIdx.x == 0) {
-        const double l = part ? (bad ? (double)NAN : (double)widen(z[a]) - (double)m - log1p(rest)) : 0.0;
-        A.logp[r] = (Row)l;
-        A.stats[2 * r] = part && bad ? (Row)NAN : (Row)m;
-        A.stats[2 * r + 1] = part ? (bad ? (Row)NAN : (Row)rest) : (Row)-1;
+    double l = 0.0, loss = 0.0;
+    if (OP == ROW_BACK) {
+      if (part) row = {(double)A.grad_logp[r], A.hess_logp ? (double)A.hess_logp[r] : 0.0};
+    } else if (part && bad) {
+      l = loss = NAN;
+    } else if (part) {
+      l = z[a] - m - log1p(rest);
+      if (OP == ROW_POLICY) {
+        part = z[a] != -INFINITY;  // the class taken is masked
+        if (part)
+          row = policy_terms(A.pol, l, A.pol.advantages[r], A.pol.old_logp[r], A.pol.ref_logp ? A.pol.ref_logp[r] : 0.0,
+                             A.pol.weights ? A.pol.weights[r] : 1.0, &loss, [](double d) { return exp(d); });
       }
-      __syncthreads();
-      continue;
-    } else if (OP == ROW_BACK) {
-      row = {part ? (double)A.grad_logp[r] : 0.0, part && A.hess_logp ? (double)A.hess_logp[r] : 0.0};
-    } else {
-      double l = 0.0, loss = 0.0;
-      if (part && bad) {
-        l = loss = row.g = row.h = NAN;
-      } else if (part) {
-        const double za = (double)widen(z[a]);
-        l = za - (double)m - log1p(rest);
-        if (za == -INFINITY) {
-          part = false;
-        } else {
-          const double adv = (double)A.pol.advantages[r], old = (double)A.pol.old_logp[r];
-          if (sizeof(C) == 4 && near_border(A.pol, l - old, adv, border_slack(kMaxClasses / kRowThreads + 16, 12.5))) {
-            double s = 0.0;
-            for (int k = threadIdx.x; k < K; k += kRowThreads) s += exp((double)widen(z[k]) - (double)m);
-            l = za - (double)m - log(block_reduce(s, sm_d, add_f64));
-          }
-          row = policy_terms(A.pol, l, adv, old, A.pol.ref_logp ? (double)A.pol.ref_logp[r] : 0.0,
-                             A.pol.weights ? (double)A.pol.weights[r] : 1.0, &loss,
-                             [](double d) { return exp(d); });
+    }
+    if (OP == ROW_LOGPROBS && threadIdx.x == 0) {
+      A.logp[r] = l;
+      A.stats[2 * r] = part && bad ? NAN : m;
+      A.stats[2 * r + 1] = part && bad ? NAN : part ? rest : -1.0;
+    }
+    if (OP == ROW_POLICY && threadIdx.x == 0) {
+      if (A.pol.loss) A.pol.loss[r] = loss;
+      if (A.pol.logp) A.pol.logp[r] = l;
+    }
+    if (OP != ROW_LOGPROBS && A.out.grad) {
+      float* gp = A.out.grad + r * A.out.row_stride;
+      float* hp = A.out.hess ? A.out.hess + r * A.out.row_stride : nullptr;
+      const double inv = 1.0 / (1.0 + rest), share = rest / (1.0 + rest);
+      for (int k = threadIdx.x; k < K; k += kRowThreads) {
+        double g = part && bad ? NAN : 0.0, h = g;
+        if (part && !bad) {
+          const double e = exp(z[k] - m), p = e * inv, left = e == 1.0 ? share : 1.0 - p, q = k == a ? left : -p;
+          g = row.g * q;
+          h = row.h * q * q + fabs(row.g) * p * left;
         }
+        gp[k * A.out.class_stride] = (float)g;
+        if (hp) hp[k * A.out.class_stride] = (float)h;
       }
-      if (threadIdx.x == 0) {
-        if (A.pol.loss) A.pol.loss[r] = (Row)loss;
-        if (A.pol.logp) A.pol.logp[r] = (Row)l;
-      }
-    }
-    if (OP == ROW_POLICY && !A.out.grad) {
-      __syncthreads();
-      continue;
-    }
-    auto* gp = A.out.grad + r * A.out.row_stride;
-    auto* hp = A.out.hess ? A.out.hess + r * A.out.row_stride : nullptr;
-    const C g = (C)row.g, h = (C)row.h, inv = (C)(1.0 / (1.0 + rest)), left = (C)(rest / (1.0 + rest));
-    for (int k = threadIdx.x; k < K; k += kRowThreads) {
-      C dg = 0, dh = 0;
-      if (part && bad) dg = dh = (C)NAN;
-      else if (part) derivative<C>(exp_c((C)widen(z[k]) - m), inv, left, k == a, g, h, hp != nullptr, &dg, &dh);
-      narrow(dg, gp[k * A.out.class_stride]);
-      if (hp) narrow(dh, hp[k * A.out.class_stride]);
     }
     __syncthreads();
   }
@@ -162,11 +133,12 @@ void launch_rows_t(const RowArgs<T>& A, cudaStream_t st) {
     MTB_CUDA_FB(cudaGetLastError());
     return;
   }
-  if constexpr (sizeof(T) <= 4)
-    if (launch_large<T, OP>(A, st)) return;
-  const unsigned grid = (unsigned)std::min<long long>(A.in.n, 1 << 20);
-  k_feedback_rows<T, OP><<<grid, kRowThreads, 0, st>>>(A);
-  MTB_CUDA_FB(cudaGetLastError());
+  if constexpr (sizeof(T) == 8) {
+    k_feedback_rows<OP><<<(unsigned)std::min<long long>(A.in.n, 1 << 20), kRowThreads, 0, st>>>(A);
+    MTB_CUDA_FB(cudaGetLastError());
+  } else {
+    launch_large<T, OP>(A, st);
+  }
 }
 
 template <typename T>

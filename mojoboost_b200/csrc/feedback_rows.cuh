@@ -36,15 +36,6 @@ __device__ __forceinline__ void narrow(double v, float& o) { o = (float)v; }
 __device__ __forceinline__ void narrow(float v, __half& o) { o = __float2half_rn(v); }
 __device__ __forceinline__ void narrow(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 
-__device__ __forceinline__ double exp_c(double d) { return exp(d); }
-__device__ __forceinline__ float exp_c(float d) { return __expf(d); }
-
-// The larger of two values, NaN when either is.
-template <typename C>
-__device__ __forceinline__ C max_nan(C a, C b) {
-  return (b > a || b != b) ? b : a;
-}
-
 template <typename T>
 struct RowPointers {
   const T* scores;
