@@ -409,7 +409,8 @@ void mojotrees_b200_preference_plan_free(MojoTreesPreferencePlan *plan);
  * u = (score - reference of the winner) - (score - reference of the loser):
  *   MOJOTREES_B200_PREFERENCE_LOGISTIC  -(1 - s) log sigmoid(beta u)
  *                                       - s log sigmoid(-beta u), s = label_smoothing
- *   MOJOTREES_B200_PREFERENCE_SQUARED   (u - 1 / (2 beta))^2
+ *   MOJOTREES_B200_PREFERENCE_SQUARED   (u - 1 / (2 beta))^2, which has no use
+ *                                       for label_smoothing
  * times its weight.  out_loss (scores' type [n_pairs], may be NULL) receives
  * each pair's; out_grad and out_hess (float [n_items], may both be NULL) the
  * sums over an item's pairs of the first and second derivative with respect
@@ -434,8 +435,8 @@ int32_t mojotrees_b200_preference_loss(const MojoTreesPreferencePlan *plan, cons
  * fits do not cover these objectives.
  *
  * Preference: row winners[p] was preferred to row losers[p].  Parameters
- * preference_beta (1), preference_label_smoothing (0), preference_loss
- * (logistic, squared).  With num_class > 1 a row stands for the class that
+ * preference_beta (1), preference_loss (logistic, squared) and, for the
+ * logistic loss, preference_label_smoothing (0).  With num_class > 1 a row stands for the class that
  * actions (int32 [n_rows]) says it took, and its score is that class's log
  * probability; else actions is NULL.  reference: a reference model's score or
  * log probability per row (double [n_rows], NULL: 0).

@@ -182,7 +182,7 @@ def preference_loss(plan, scores, reference=None, beta=1.0, label_smoothing=0.0,
     """Paired preference loss of the items' scores (raw scores or log
     probabilities of whole answers, float64 or float32 [n_items]) relative to
     a reference model's.  loss "logistic": -log sigmoid(beta u), with label
-    smoothing; "squared": (u - 1 / (2 beta))^2, for a pair's difference u of
+    smoothing; "squared": (u - 1 / (2 beta))^2, without; for a pair's difference u of
     score - reference.  Returns (loss [n_pairs], grad [n_items], hess
     [n_items]); the derivatives are float32."""
     types, torch, stream = _torch_types()

@@ -289,8 +289,6 @@ TrainConfig parse_config(const char* params, bool need_training) {
     if (c.objective == mtb::OBJECTIVE_MULTICLASS && c.num_class < 2)
       throw InvalidArgument("multiclass needs num_class >= 2");
     if (c.objective < mtb::OBJECTIVE_MULTICLASS) c.num_class = 1;
-    if (c.preference_loss == 1 && c.preference_label_smoothing > 0.0)
-      throw InvalidArgument("preference_label_smoothing needs preference_loss=logistic");
   }
   return c;
 }

@@ -216,7 +216,6 @@ int32_t mojotrees_b200_preference_loss(const MojoTreesPreferencePlan* plan, cons
     require(beta > 0.0 && std::isfinite(beta), "beta must be positive");
     require(label_smoothing >= 0.0 && label_smoothing <= 0.5, "label_smoothing must be in [0, 0.5]");
     require(loss_kind == mtb::PREFERENCE_LOGISTIC || loss_kind == mtb::PREFERENCE_SQUARED, "unknown preference loss");
-    require(loss_kind == mtb::PREFERENCE_LOGISTIC || label_smoothing == 0.0, "label_smoothing needs the logistic loss");
     const mtb::PreferencePlan& p = plan->plan;
     require(p.n_items == 0 || scores, "null pointer argument");
     require(!out_grad == !out_hess, "out_grad and out_hess go together");

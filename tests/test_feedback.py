@@ -438,7 +438,7 @@ def test_mixed_and_host_arrays_are_refused(mtlib):
     plan = mtlib.PreferencePlan([0], [1], 4)
     for f in (lambda: mtlib.preference_loss(plan, one[:3]), lambda: mtlib.preference_loss(plan, one.half()),
               lambda: mtlib.preference_loss(plan, one, beta=0.0), lambda: mtlib.preference_loss(plan, one, label_smoothing=0.6),
-              lambda: mtlib.preference_loss(plan, one, loss="squared", label_smoothing=0.1), lambda: mtlib.preference_loss(plan, one, loss="x"),
+              lambda: mtlib.preference_loss(plan, one, label_smoothing=-0.1), lambda: mtlib.preference_loss(plan, one, loss="x"),
               lambda: mtlib.preference_loss(plan, one, reference=one.double()), lambda: mtlib.preference_loss(plan, one.cpu())):
         with pytest.raises(mtlib.MojoTreesError) as e:
             f()
@@ -476,7 +476,7 @@ def test_preference_loss(mtlib, n, P_, how, dtype):
     i, j = _pairs(n + P_, n, P_, how) if P_ else (np.zeros(0, np.int64), np.zeros(0, np.int64))
     rng = np.random.default_rng(P_)
     for loss, beta, eps, with_ref, with_w in (("logistic", 0.5, 0.0, True, False), ("logistic", 2.0, 0.1, False, True),
-                                              ("squared", 0.1, 0.0, True, True)):
+                                              ("squared", 0.1, 0.0, True, True), ("squared", 0.3, 0.1, False, False)):
         w = rng.random(P_).astype(np.float32) if with_w else None
         if with_w:
             w[rng.random(P_) < 0.2] = 0

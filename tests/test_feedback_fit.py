@@ -63,7 +63,7 @@ def _preference(mtlib, **kw):
     (dict(initial_scores=np.zeros((4, 2))), -1, "initial_scores"), (dict(initial_scores=np.zeros(3)), -1, "initial_scores"),
     (dict(params={"preference_beta": 0}), -1, "preference_beta"), (dict(params={"preference_label_smoothing": 0.7}), -1, "smoothing"),
     (dict(params={"preference_loss": "hinge"}), -1, "preference_loss"),
-    (dict(params={"preference_loss": "squared", "preference_label_smoothing": 0.1}), -1, "smoothing"),
+    (dict(params={"preference_loss": "squared", "preference_label_smoothing": -0.1}), -1, "smoothing"),
     (dict(params={"objective": "regression"}), -1, "objective=preference"),
 ])
 def test_preference_fit_refusals(mtlib, kw, code, needle):
