@@ -468,14 +468,20 @@ void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const 
   memory_bytes = bytes;
   memory = take_device_memory(&memory_bytes);
   char* base = static_cast<char*>(memory);
+  // A copy from pageable memory may return before it has arrived, and the
+  // streams that will read the plan need not be ordered behind this one: the
+  // copies are waited for.
+  const cudaStream_t st = cudaStreamPerThread;
   if (bytes <= 1 << 20) {  // a copy costs more than its bytes
     std::vector<char> all(bytes);
     for (const Copy& c : copies)
       if (c.n) memcpy(&all[c.at], c.from, c.n);
-    MTB_CUDA_FB(cudaMemcpy(base, all.data(), bytes, cudaMemcpyHostToDevice));
+    MTB_CUDA_FB(cudaMemcpyAsync(base, all.data(), bytes, cudaMemcpyHostToDevice, st));
+    MTB_CUDA_FB(cudaStreamSynchronize(st));
   } else {
     for (const Copy& c : copies)
-      if (c.n) MTB_CUDA_FB(cudaMemcpy(base + c.at, c.from, c.n, cudaMemcpyHostToDevice));
+      if (c.n) MTB_CUDA_FB(cudaMemcpyAsync(base + c.at, c.from, c.n, cudaMemcpyHostToDevice, st));
+    MTB_CUDA_FB(cudaStreamSynchronize(st));
   }
   n_items = ni;
   n_pairs = np;
