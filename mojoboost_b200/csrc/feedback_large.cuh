@@ -145,7 +145,20 @@ constexpr double kLn2 = 0.6931471805599453;
 // c of the comment above, negated.
 __device__ __forceinline__ float exponent_offset(float m) { return -__fmul_rn(m, kLog2e); }
 
-enum RowState : int { ROW_EMPTY = 0, ROW_DONE = 1, ROW_SLOW = 2, ROW_NEAR = 3 };
+// Up to 2^24, c is within 1 of log2(e) m.  Far beyond, `shift` would leave
+// float32's exponents, and c itself at the type's end.  A warp that lies
+// farther than kFarWarp leaves its sum out (0, with its maximum): it matters
+// only to a row whose own maximum is farther than kFarRow, as a warp of masked
+// classes is e^-8000000 of any other row.  Such rows are left to far_rows, which
+// takes their exponentials of z - m.  float16 holds no such score.
+constexpr float kFarWarp = 0x1p24f, kFarRow = 0x1p23f;
+
+template <typename T>
+__device__ __forceinline__ bool is_far(float m) {
+  return !std::is_same<T, __half>::value && fabsf(m) > kFarRow;
+}
+
+enum RowState : int { ROW_EMPTY = 0, ROW_DONE = 1, ROW_SLOW = 2, ROW_NEAR = 3, ROW_FAR = 4 };
 
 template <int THREADS>
 struct LargeShared {
@@ -178,6 +191,89 @@ __device__ __forceinline__ Part add_parts(Part p, int n) {
   return p;
 }
 
+// A far row's derivatives; 0 without `live`.
+template <typename T, bool HESS>
+__device__ __noinline__ void far_derivatives(const RowArgs<T>& A, long long r, float m, float g, float h, float inv,
+                                             float share, bool live) {
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const T* z = A.in.scores + r * A.in.stride;
+  const long long a = A.in.action(r), to = r * A.out.row_stride;
+  for (int k = cluster.thread_rank(); k < A.in.K; k += cluster.num_threads()) {
+    const float f = widen(z[k]), p = exp2_approx((f - m) * kLog2e) * inv, left = f == m ? share : 1.0f - p;
+    const float q = k == a ? left : -p;
+    narrow(live ? g * q : 0.0f, A.out.grad[to + k]);
+    if (HESS) narrow(live ? h * q * q + fabsf(g) * p * left : 0.0f, A.out.hess[to + k]);
+  }
+}
+
+// The far rows among this block's or cluster's, after all others: their
+// elements are read again, and summed in float64.  Apart from the loop over
+// rows, which has no registers left for it: called in there it took 2 to 10%
+// more time for other rows, called behind it 1 to 3%, inlined there -3 to 4%.
+template <typename T, int OP, bool HESS, int THREADS>
+__device__ __forceinline__ void far_rows(const RowArgs<T>& A, LargeShared<THREADS>& S, const TableMath math) {
+  namespace cg = cooperative_groups;
+  using Row = typename Types<T>::Row;
+  constexpr int kWarps = THREADS / 32;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = A.in.K;
+  // Every block of the cluster sums what every block has: no joins between blocks.
+  for (long long r = blockIdx.x / blocks; r < A.in.n; r += gridDim.x / blocks) {
+    const T* z = A.in.scores + r * A.in.stride;
+    const long long a = A.in.action(r);
+    if (a < 0 || a >= K || (OP == ROW_POLICY && A.pol.weights && A.pol.weights[r] == (Row)0)) continue;
+    float m = -INFINITY;
+    for (int k = threadIdx.x; k < K; k += THREADS) m = max_nan32(m, widen(z[k]));
+    for (int k = 16; k > 0; k >>= 1) m = max_nan32(m, __shfl_xor_sync(0xffffffffu, m, k));
+    __syncthreads();
+    if (lane == 0) S.warp[0][warp].m = m;
+    __syncthreads();
+    for (int i = 0; i < kWarps; ++i) m = max_nan32(m, S.warp[0][i].m);
+    if (!is_far<T>(m) || m == -INFINITY) continue;
+    double sum = 0.0;  // less the terms at the maximum
+    int ones = 0;
+    for (int k = threadIdx.x; k < K; k += THREADS) {
+      const double d = (double)widen(z[k]) - (double)m;  // NaN at a maximum of infinity
+      if (d == 0.0) ++ones;
+      else sum += math.exp(d);
+    }
+    const Part p = add_parts({sum, m, 0.0f, ones}, 32);
+    if (lane == 0) S.slow[0][warp] = p;
+    __syncthreads();
+    sum = 0.0;
+    ones = -1;
+    for (int i = 0; i < kWarps; ++i) {
+      sum += S.slow[0][i].sum;
+      ones += S.slow[0][i].ones;
+    }
+    const double rest = sum + (double)ones, za = (double)widen(z[a]), lp = za - (double)m - math.log1p(rest);
+    if (OP == ROW_LOGPROBS) {
+      if (rank == 0 && threadIdx.x == 0) {
+        A.logp[r] = (Row)lp;
+        A.stats[2 * r] = m;
+        A.stats[2 * r + 1] = (Row)rest;
+      }
+      continue;
+    }
+    double loss = 0.0;
+    RowDerivative d = {0.0, 0.0};
+    const bool live = za != -INFINITY;
+    if (live)
+      d = policy_terms(A.pol, lp, (double)A.pol.advantages[r], (double)A.pol.old_logp[r],
+                       A.pol.ref_logp ? (double)A.pol.ref_logp[r] : 0.0, A.pol.weights ? (double)A.pol.weights[r] : 1.0,
+                       &loss, math);
+    if (rank == 0 && threadIdx.x == 0) {
+      if (A.pol.loss) A.pol.loss[r] = (Row)loss;
+      if (A.pol.logp) A.pol.logp[r] = (Row)lp;
+    }
+    if (!A.out.grad) continue;
+    const double inv64 = TableMath::inverse(1.0 + rest);
+    const float g = (float)d.g, h = (float)d.h, inv = (float)inv64, share = (float)(rest * inv64);
+    far_derivatives<T, HESS>(A, r, m, g, h, inv, share, live);
+  }
+}
+
 // A vector's elements one by one, for derivatives whose vectors do not start
 // on 16 bytes where the scores' do.
 template <typename T>
@@ -188,7 +284,8 @@ __device__ __noinline__ void store_elements(T* to, Vec<T> v) {
 
 // per: whole vectors of a row that a block takes at most.
 template <typename T, int OP, bool HESS, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(const RowArgs<T> A, const int per) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(const __grid_constant__ RowArgs<T> A,
+                                                                             const int per) {
   namespace cg = cooperative_groups;
   using Row = typename Types<T>::Row;
   constexpr int N = Vec<T>::N, kWarps = THREADS / 32;
@@ -201,6 +298,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
   const Pair scale = Pair::of(kLog2e, kLog2e);
   const long long clusters = gridDim.x / blocks;
   int parity = 0;
+  bool far = false;
   for (long long r = blockIdx.x / blocks; r < A.in.n; r += clusters) {
     // The row's whole vectors of 16 bytes are divided among the blocks.  The
     // up to 2 (N - 1) elements before and behind them lie with the first
@@ -227,6 +325,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
         g = A.grad_logp[r];
         if (HESS) h = A.hess_logp[r];
         const float inv_total = __frcp_rn(1.0f + rest);
+        if (is_far<T>(m)) {
+          far_derivatives<T, HESS>(A, r, m, g, h, inv_total, rest * inv_total, true);
+          continue;
+        }
         inv = inv_total * exp2_approx(-fmaf(m, kLog2e, exponent_offset(m)));
         share = rest * inv_total;
       }
@@ -305,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
       }
       for (int k = 16; k > 0; k >>= 1) wm = max_nan32(wm, __shfl_xor_sync(0xffffffffu, wm, k));
       Part p = {0.0, wm, 0.0f, 0};
-      if (wm != -INFINITY) {
+      if (!(fabsf(wm) > kFarWarp)) {
         const float c = exponent_offset(wm);
         const Pair offset = Pair::of(c, c);
         Pair sum = Pair::of(exp2_approx(fmaf(ze, kLog2e, c)), 0.0f);
@@ -335,9 +437,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
       }
       if (warp == 0) {
         const double rest = all.sum - 1.0;
-        if (all.m == -INFINITY || rest < 1.0) {
+        if (all.m == -INFINITY || rest < 1.0 || is_far<T>(all.m)) {
           if (lane == 0) {
-            S.state = all.m == -INFINITY ? ROW_EMPTY : ROW_SLOW;
+            S.state = all.m == -INFINITY ? ROW_EMPTY : is_far<T>(all.m) ? ROW_FAR : ROW_SLOW;
             S.m = all.m;
             if (OP == ROW_POLICY && rank == 0 && S.state == ROW_EMPTY) {
               if (A.pol.loss) A.pol.loss[r] = 0.0f;
@@ -349,6 +451,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
         }
       }
       __syncthreads();
+      if (!std::is_same<T, __half>::value && S.state == ROW_FAR) {
+        far = true;
+        continue;
+      }
       if (S.state == ROW_SLOW) {
         // One class has more than half, and its 1 took the last bits of the
         // others: the sum without the terms at the maximum, of the warps that
@@ -493,6 +599,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_feedback_large(cons
       narrow(g * q, to_g[taken]);
       if (HESS) narrow(q * (h * q + ag * p), to_h[taken]);
     }
+  }
+  if constexpr (!std::is_same<T, __half>::value && OP != ROW_BACK) {
+    if (far) far_rows<T, OP, HESS, THREADS>(A, S, math);
   }
   if (blocks > 1) cluster.sync();  // the others may still read this block's parts
 }

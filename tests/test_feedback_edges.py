@@ -1,10 +1,13 @@
 """Losses from feedback where they can go wrong: plans used at once, masks of
 finite values, log ratios at the end of float64's range, and the like, against
 plain float64 forms (feedback_util)."""
+import math
+
 import numpy as np
 import pytest
 
 import feedback_util as fu
+from test_feedback import DTYPES, HALF_STEP, TINY, _close
 
 gpu = pytest.mark.gpu
 
@@ -45,3 +48,199 @@ def test_plan_is_there_for_any_stream(mtlib, n, P, turns):
         degree = np.bincount(np.concatenate([i, j]), minlength=n)
         tol = np.abs(G) * fu.U32 * 1.01 + degree * (term + degree * 2.0 ** -52)
         assert (np.abs(grad.cpu().numpy() - G) <= tol).all(), turn
+
+
+# ------------------------------------------------------------------- masks
+
+def _bounds(z, a, f64):
+    """(logp, stats, p, left, part) of float64 scores z, and error bounds from
+    the kernels' arithmetic: of a log probability (absolute), each p, the
+    others' sum and the largest class's complement (relative).
+
+    A lane adds at most 16 terms (up to 128 classes, float64 512) or 33 (a
+    lane's 8 vectors of 16 bytes in pairs, and an element at the row's edge),
+    then 5 sums of lanes; warps are joined in float64.  float64 rows of more
+    than 512 classes: ceil(K / 256) in a thread.  An exponential's own error is
+    fu.exp_error; a row's statistics and scalars round up to 10 times on the way
+    to a gradient."""
+    logp, stats, p, left, part = fu.softmax_rows(z, a)
+    K = z.shape[1]
+    unit = 2.0 ** -53 if f64 else fu.U32
+    adds = 16 if K <= (512 if f64 else 128) else -(-K // 256) if f64 else 33
+    with np.errstate(invalid="ignore"):
+        d = np.where(np.isfinite(z), z - stats[:, :1], -np.inf)
+    e_exp = np.where(p > 0, fu.exp_error(d, f64), 0.0)
+    e_sum = (p * e_exp).sum(1) + (adds + 5) * unit
+    others = p.copy()
+    others[np.arange(len(z)), z.argmax(1)] = 0.0
+    total = others.sum(1)
+    e_rest = np.where(total > 0, (others * e_exp).sum(1) / np.where(total > 0, total, 1.0), 0.0) + (adds + 5) * unit
+    e_rest = 2 * e_rest + 2 * unit  # the sum less 1, where it is 1 and more
+    e_l = e_sum + np.where(np.isfinite(logp), np.abs(logp), 0.0) * (2 * unit) + 2.0 ** -52
+    e_p = e_exp + e_sum[:, None] + 10 * unit
+    return logp, stats, p, left, part, e_l, e_p, e_rest, e_rest + 10 * unit + (2.0 ** -42 if f64 else 0.0)
+
+
+def _check_logprobs(mtlib, x, a_t, z, a, dtype):
+    """action_logprobs and its way back on scores x (z in float64) within _bounds."""
+    import torch
+    f64 = dtype == "float64"
+    n, K = z.shape
+    logp, stats, p, left, part, e_l, e_p, e_rest, e_left = _bounds(z, a, f64)
+    got_l, got_s = mtlib.action_logprobs(x, a_t)
+    _close(got_l, logp, e_l, "logp")
+    _close(got_s[:, 0], stats[:, 0], 0.0, "maximum")
+    _close(got_s[:, 1], stats[:, 1], np.abs(stats[:, 1]) * e_rest + TINY[dtype] * K, "sum less 1")
+    rng = np.random.default_rng(K)
+    g, h = rng.normal(size=n).astype(np.float32), rng.random(n).astype(np.float32)
+    got_g, got_h = mtlib.action_logprobs_grad(x, a_t, got_s, torch.from_numpy(g).cuda(), torch.from_numpy(h).cuda())
+    G, H, q = fu.to_scores(p, left, a, part, g.astype(np.float64), h.astype(np.float64))
+    tol_q = np.where(q > 0, np.maximum(e_left[:, None], e_p), e_p)
+    # 1 - p of the largest class by the others' share, of the rest within p's error of a value of at least a half
+    tol_h = 2 * tol_q + e_p + e_left[:, None]
+    half, tiny = HALF_STEP[dtype], TINY[dtype] * 4
+    _close(got_g, G, np.abs(G) * (tol_q + half) * 1.01 + tiny, "grad")
+    _close(got_h, H, H * (tol_h + half) * 1.01 + tiny, "hess")
+
+
+def _check_policy(got, z, a, adv, old, ref, low, high, kl, dtype):
+    """policy_loss's four outputs within _bounds: with e the bound of l, the
+    loss is off by |dloss/dl| e and a few roundings of its float64 terms, and
+    dloss/dl by its own derivative times e (away from the clip range's ends)."""
+    n, f64 = len(z), dtype == "float64"
+    logp, stats, p, left, part, e_l, e_p, e_rest, e_left = _bounds(z, a, f64)
+    loss, g, h, part = fu.policy_rows(logp, part, adv.astype(np.float64), old.astype(np.float64),
+                                      None if ref is None else ref.astype(np.float64), None, low, high, kl)
+    unit = 2.0 ** -53 if f64 else fu.U32
+    l = np.where(part, logp, 0.0)
+    ra = np.abs(np.exp(l - old) * adv)
+    et = np.zeros(n) if ref is None else np.exp(ref - l)
+    far = 0.0 if ref is None else 1 + np.abs(ref - l)
+    step = 2.0 ** -50 * (1 + np.abs(l) + np.abs(old))
+    e_g = np.where(part, (ra + kl * et) * (e_l * 1.01 + step), 0.0)
+    _close(got[1], logp, e_l, "logp")
+    _close(got[0], loss, np.where(part, (np.abs(g) + e_g) * e_l + (ra + kl * (et + far)) * step, 0.0) + np.abs(loss) * 2 * unit
+           + TINY["float32"], "loss")
+    G, H, q = fu.to_scores(p, left, a, part, g, h)
+    tol_q = np.where(q > 0, np.maximum(e_left[:, None], e_p), e_p)
+    tol_h = 2 * tol_q + e_p + e_left[:, None]
+    half, tiny, e_g = HALF_STEP[dtype], TINY[dtype] * 4, e_g[:, None]
+    _close(got[2], G, (np.abs(q) * e_g + np.abs(G) * (tol_q + half)) * 1.01 + tiny, "grad")
+    _close(got[3], H, ((q * q + p * left) * 2 * e_g + H * (tol_h + half)) * 1.01 + tiny, "hess")
+
+
+MASKS = ["-inf", -1e4, -1e7, -1e9, -1e10, -1e12, -1e20, -1e30, "lowest"]
+
+
+def _masked_rows(seed, K, dtype, mask):
+    """Rows with masked classes: none, single ones, all but three next to one
+    another, all but one, all but the first or last, all; the class taken
+    allowed but in one row."""
+    import torch
+    rng = np.random.default_rng(seed)
+    t = getattr(torch, dtype)
+    low = -math.inf if mask == "-inf" else torch.finfo(t).min if mask == "lowest" else max(mask, torch.finfo(t).min)
+    allowed = [np.ones(K, bool), rng.random(K) < 0.7, np.zeros(K, bool), np.zeros(K, bool), np.zeros(K, bool), np.zeros(K, bool),
+               np.zeros(K, bool), rng.random(K) < 0.5]
+    at = int(rng.integers(0, K - 3))
+    allowed[2][at:at + 3] = True
+    allowed[3][at] = True
+    allowed[4][0] = allowed[5][K - 1] = True
+    z = rng.normal(size=(len(allowed), K)) * 2
+    a = np.zeros(len(allowed), np.int64)
+    for r, ok in enumerate(allowed):
+        z[r, ~ok] = low
+        a[r] = rng.choice(np.flatnonzero(ok)) if ok.any() else 1
+    a[7] = np.flatnonzero(~allowed[7])[0]
+    x = torch.from_numpy(z).to(t).cuda()
+    return x, x.double().cpu().numpy(), torch.from_numpy(a).cuda(), a
+
+
+WIDTHS = [5, 64, 128, 129, 300, 600, 1025, 5000, 20_001, 50_001, 131_072]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K", WIDTHS)
+def test_masks_of_any_value(mtlib, K, dtype):
+    """A mask is as good as -inf from where its probability is 0 on, and a row
+    that holds nothing else is uniform (of -inf: takes no part)."""
+    import torch
+    t = torch.float64 if dtype == "float64" else torch.float32
+    for mask in MASKS:
+        x, z, a_t, a = _masked_rows(K, K, dtype, mask)
+        _check_logprobs(mtlib, x, a_t, z, a, dtype)
+        rng = np.random.default_rng(1)
+        logp = fu.softmax_rows(z, a)[0]
+        near = np.where(np.isfinite(logp), logp, -1.0)
+        near = np.maximum(near, -80)  # the masked class that a row took: a ratio of 0
+        adv = rng.normal(size=len(z))
+        old, ref = near + 0.2 * rng.normal(size=len(z)), near + 0.3 * rng.normal(size=len(z))
+        rows = [torch.from_numpy(v).to(t).cuda() for v in (adv, old, ref)]
+        back = [v.cpu().numpy() for v in rows]
+        for n, kl in ((len(z), 0.0), (7, 0.3)):  # exp(ref - l) of a masked class that was taken has no end
+            got = mtlib.policy_loss(x[:n], a_t[:n], rows[0][:n], rows[1][:n], ref_logp=rows[2][:n], kl_coef=kl, clip_high=0.3, hess=True)
+            _check_policy(got, z[:n], a[:n], back[0][:n], back[1][:n], back[2][:n] if kl else None, 0.2, 0.3, kl, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float64", "float32", "bfloat16"])
+@pytest.mark.parametrize("K", WIDTHS)
+def test_scores_of_any_size(mtlib, K, dtype):
+    """Rows that lie far from 0 as a whole, on both sides of where the kernels
+    take the maximum out first, and up to the ends of the type."""
+    import torch
+    t = getattr(torch, dtype)
+    rng = np.random.default_rng(K)
+    far = [0.0, 1e3, 2.0 ** 22, 2.0 ** 23 - 4, 2.0 ** 23 + 4, 2.0 ** 24 - 8, 2.0 ** 24 + 8, 2.0 ** 26, 1e9, 1e10, 1e20, 1e30]
+    far = far + [-v for v in far[1:]] + [torch.finfo(t).max, torch.finfo(t).min]
+    z = rng.normal(size=(len(far), K)) * 3
+    for r, v in enumerate(far):
+        at = np.float64(torch.tensor(v, dtype=t))
+        step = abs(at) * torch.finfo(t).eps if v else 1.0  # a class now and then is a step or two below
+        if step > 1e30:  # the type's ends: the row's other classes are at 0
+            z[r] = np.where(rng.random(K) < 0.5, at, 0.0) if v > 0 else at
+            z[r, 0] = at
+        else:
+            z[r] = np.where(rng.random(K) < 0.5, at, at - max(step, 1.0) * rng.integers(1, 3, size=K))
+    x = torch.from_numpy(z).to(t).cuda()
+    z = x.double().cpu().numpy()
+    a = z.argmax(1)
+    a[::2] = rng.integers(0, K, size=len(a[::2]))
+    a_t = torch.from_numpy(a).cuda()
+    _check_logprobs(mtlib, x, a_t, z, a, dtype)
+    row = torch.float64 if dtype == "float64" else torch.float32
+    logp = fu.softmax_rows(z, a)[0]
+    rows = [torch.from_numpy(v).to(row).cuda() for v in (rng.normal(size=len(z)), np.maximum(logp, -80) + 0.2 * rng.normal(size=len(z)))]
+    back = [v.cpu().numpy() for v in rows]
+    got = mtlib.policy_loss(x, a_t, *rows, clip_high=0.3, hess=True)
+    _check_policy(got, z, a, *back, None, 0.2, 0.3, 0.0, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,K", [("float32", 129), ("float32", 40_000), ("bfloat16", 200), ("bfloat16", 131_072)])
+def test_clip_border_of_far_rows(mtlib, dtype, K):
+    """As test_clip_border_is_decided_in_float64, for rows at 1e12 whose
+    classes lie apart by more than an exponential tells, so that 1 to 64 of them
+    share the probability."""
+    import torch
+    n = 64
+    rng = np.random.default_rng(K)
+    top = float(torch.tensor(1e12, dtype=getattr(torch, dtype)))
+    z = np.full((n, K), 0.0)
+    for r in range(n):
+        z[r, rng.permutation(K)[:r + 1]] = top
+    a = z.argmax(1)
+    x = torch.from_numpy(z).to(getattr(torch, dtype)).cuda()
+    adv = np.where(np.arange(n) % 2 == 0, 1.0, -1.0)
+    logp = -np.log(np.arange(n) + 1.0)
+    end = np.where(adv > 0, math.log1p(0.3), math.log1p(-0.2))
+    old = (logp - end - rng.choice([-1, 1], size=n) * 10.0 ** rng.uniform(-9, -6, size=n)).astype(np.float32)
+    d = logp - old.astype(np.float64)
+    clear = np.abs(d - end) > 1e-12
+    t = [torch.from_numpy(v.astype(np.float32)).cuda() for v in (adv, old)]
+    grad = mtlib.policy_loss(x, torch.from_numpy(a).cuda(), *t, clip_low=0.2, clip_high=0.3)[2]
+    moved = (grad != 0).any(1).cpu().numpy()
+    active = np.where(adv > 0, d <= end, d >= end)
+    active[0] = False  # one class has it all: a gradient of 0 either way
+    np.testing.assert_array_equal(moved[clear], active[clear])
