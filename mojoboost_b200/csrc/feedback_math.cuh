@@ -88,10 +88,10 @@ struct TableMath {
     }
     __syncthreads();
   }
-  // exp(d), d <= 709.78: d = (n / 64) ln 2 + r, exp(d) = 2^(n / 64) (1 + r +
-  // ... + r^5 / 120), |r| <= ln 2 / 128, truncation below 2^-54.  NaN stays;
-  // below -708 (3e-308) the value is 0.
-  __device__ __forceinline__ double exp(double d) const {
+  // exp(d) / 2^less, d <= 709 + less: d = (n / 64) ln 2 + r, exp(d) = 2^(n / 64)
+  // (1 + r + ... + r^5 / 120), |r| <= ln 2 / 128, truncation below 2^-54.  NaN
+  // stays; below -708 (3e-308) the value is 0.
+  __device__ __forceinline__ double exp(double d, int less = 0) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
     const bool none = d < -708.0;
     d = __hiloint2double(none ? 0 : __double2hiint(d), __double2loint(d));
@@ -105,11 +105,16 @@ struct TableMath {
     q = fma(q, r, 0.5);
     q = fma(q, r * r, r);
     const double two_n = t->two[none ? 64 : n & 63];
-    const double scaled = __hiloint2double(__double2hiint(two_n) + (n >> 6 << 20), __double2loint(two_n));
+    const double scaled = __hiloint2double(__double2hiint(two_n) + ((n >> 6) - less << 20), __double2loint(two_n));
     return fma(scaled, q, scaled);
   }
   __device__ __forceinline__ float exp(float d) const { return __expf(d); }
-  __device__ __forceinline__ double operator()(double d) const { return d > 709.78 ? INFINITY : exp(d); }
+  // exp(d) for any d: the last binade by its half, whose scale still has an exponent.
+  __device__ __forceinline__ double operator()(double d) const {
+    const int less = d > 709.0 ? 1 : 0;
+    const double e = exp(d, less);
+    return d > 709.79 ? INFINITY : less ? e + e : e;
+  }
   // log(1 + x), 0 <= x < 2^1000: 1 + x = 2^e c (1 + f), c the multiple of 1/64
   // next to its significand, |f| <= 1 / 128; f - f^2 / 2 + ... - f^8 / 8,
   // truncation below 2^-59.  Next to 1, f is x itself.

@@ -244,3 +244,44 @@ def test_clip_border_of_far_rows(mtlib, dtype, K):
     active = np.where(adv > 0, d <= end, d >= end)
     active[0] = False  # one class has it all: a gradient of 0 either way
     np.testing.assert_array_equal(moved[clear], active[clear])
+
+
+# ------------------------------------------------------- the end of float64's range
+
+FAR_RATIOS = [-800.0, -708.5, -707.5, 600.0, 708.9, 709.1, 709.7, 709.77, 709.7773, 709.779, 709.78, 709.781, 709.7827, 709.783, 709.79, 710.0, 1e4]
+
+
+@gpu
+@pytest.mark.parametrize("K", [3, 40, 600])
+@pytest.mark.parametrize("end", ["ratio", "reference"])
+def test_log_ratios_up_to_the_end_of_float64(mtlib, K, end):
+    """e^d of a log ratio or of the reference's distance is right up to
+    float64's largest and infinite beyond; a clipped row keeps its finite loss."""
+    import torch
+    rng = np.random.default_rng(K)
+    d = np.repeat(FAR_RATIOS, 2)
+    n = len(d)
+    x, a = rng.normal(size=(n, K)), rng.integers(0, K, size=n)
+    logp = fu.softmax_rows(x, a)[0]
+    adv, old, ref, kl = np.where(np.arange(n) % 2 == 0, -1e-300, 1e-300), logp - d, None, 0.0
+    if end == "reference":
+        adv, old, ref, kl = np.zeros(n), logp.copy(), logp + d, 1e-300
+    t = [None if v is None else torch.from_numpy(v).cuda() for v in (x, a, adv, old, ref)]
+    got = mtlib.policy_loss(t[0], t[1], t[2], t[3], ref_logp=t[4], clip_low=0.2, clip_high=0.3, kl_coef=kl, hess=True)
+    with np.errstate(over="ignore"):
+        loss, g, h, part = fu.policy_rows(logp, np.ones(n, bool), adv, old, ref, None, 0.2, 0.3, kl)
+        # where the oracle's own d decides between finite and infinite
+        clear = np.isfinite(np.exp(np.abs(d) + 1e-9)) | ~np.isfinite(np.exp(np.abs(d) - 1e-9))
+    step = 2.0 ** -50 * (1 + np.abs(logp) + np.abs(logp - d))
+    have = got[0].cpu().numpy()
+    assert not np.isnan(have).any() and not any(v.isnan().any() for v in got[1:3])
+    fine = clear & np.isfinite(loss)
+    np.testing.assert_array_equal(have[clear & ~fine], loss[clear & ~fine])
+    # exp is 0 below -708: off by at most e^-708 there
+    tol = np.abs(loss) * step + (np.abs(adv) + kl) * (np.exp(-708) + 2.0 ** -52 * (1 + np.abs(d)))
+    assert (np.abs(have[fine] - loss[fine]) <= tol[fine]).all()
+    grad = got[2].double().cpu().numpy()[np.arange(n), a]
+    q = 1 - np.exp(logp)
+    small = fine & (np.abs(g) < 1e38)
+    tol = np.abs(g) * q * (fu.U32 * 1.01 + step + 2.0 ** -40) + 2.0 ** -149
+    assert (np.abs(grad[small] - (g * q)[small]) <= tol[small]).all()
