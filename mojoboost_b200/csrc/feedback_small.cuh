@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_feedback_small(const RowArgs<
     const C inv = (C)inv_total, share = (C)(rest * inv_total), g = (C)row.g, h = (C)row.h;
     if (part && !bad) {
       // every class as one that was not taken, and with 1 - p as it comes
-      const C down = -g * inv, ag = fabs(g), bend = h - ag;
+      const C down = -g * inv, ag = fabs(g), bend = ag < (C)INFINITY ? h - ag : (C)0;
 #pragma unroll
       for (int e = 0; e < P; ++e)
         if (has(e, l, K)) narrow(v[e] * down, to_g[l + e * L]);

@@ -285,3 +285,26 @@ def test_log_ratios_up_to_the_end_of_float64(mtlib, K, end):
     small = fine & (np.abs(g) < 1e38)
     tol = np.abs(g) * q * (fu.U32 * 1.01 + step + 2.0 ** -40) + 2.0 ** -149
     assert (np.abs(grad[small] - (g * q)[small]) <= tol[small]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K", [3, 10, 40, 128, 300, 600, 5000])
+def test_infinite_derivatives(mtlib, K, dtype):
+    """A ratio beyond the derivatives' type: the row's gradient and hessian are
+    infinite, with the gradient's signs, and not NaN; other rows are theirs."""
+    import torch
+    t = torch.float64 if dtype == "float64" else torch.float32
+    rng = np.random.default_rng(K)
+    x = torch.from_numpy(rng.normal(size=(4, K))).to(getattr(torch, dtype)).cuda()
+    a = torch.tensor([0, 1, 2, K - 1], device="cuda")
+    logp, _ = mtlib.action_logprobs(x, a)
+    # minus an advantage of 1: every class has probability, and the ratio is e^150 or 1
+    old = logp - torch.tensor([150.0, 0.0, 150.0, 0.0], device="cuda", dtype=t)
+    loss, _, G, H = mtlib.policy_loss(x, a, -torch.ones(4, device="cuda", dtype=t), old, hess=True)
+    taken = torch.zeros(4, K, dtype=torch.bool, device="cuda").scatter_(1, a[:, None], True)
+    for r in (0, 2):
+        assert (H[r] == math.inf).all()
+        assert torch.equal(G[r], torch.where(taken[r], math.inf, -math.inf).to(G.dtype))
+    assert torch.isfinite(G[1::2]).all() and torch.isfinite(H[1::2]).all()
+    assert torch.isfinite(loss[1::2]).all() and (loss[::2] > 1e38).all()
