@@ -43,7 +43,8 @@ struct PairTerms {
 };
 
 // float64 scores: float64 throughout.  float32 scores: u is as good as exact
-// (see Lean), and what follows is float32 arithmetic of a few steps' error.
+// (see Lean), the squared loss's distance to its target is rounded once, and
+// what follows is float32 arithmetic of a few steps' error.
 __device__ __forceinline__ double pair_exp(double x, const TableMath& math) { return math.exp(x); }
 __device__ __forceinline__ float pair_exp(float x, const TableMath&) { return expf(x); }
 __device__ __forceinline__ double pair_inverse(double x) { return TableMath::inverse(x); }
@@ -55,14 +56,30 @@ __device__ __forceinline__ double flip(double x, int by) {  // x, negated where 
 }
 __device__ __forceinline__ float flip(float x, int by) { return __uint_as_float(__float_as_uint(x) ^ (by & 0x80000000u)); }
 
+// A pair's difference: hi + low, low being what float32 scores' hi leaves out.
 template <typename T>
-__device__ __forceinline__ PairTerms<T> pair_terms(const PairMath& pm, T u, bool want_loss, const TableMath& math) {
+struct Difference {
+  T hi, low;
+  __device__ __forceinline__ T value() const { return hi + low; }
+  __device__ __forceinline__ T less(double target) const { return (T)((double)hi - target + (double)low); }
+};
+template <>
+struct Difference<double> {
+  double hi;
+  __device__ __forceinline__ double value() const { return hi; }
+  __device__ __forceinline__ double less(double target) const { return hi - target; }
+};
+__device__ __forceinline__ Difference<double> flip(Difference<double> d, int by) { return {flip(d.hi, by)}; }
+__device__ __forceinline__ Difference<float> flip(Difference<float> d, int by) { return {flip(d.hi, by), flip(d.low, by)}; }
+
+template <typename T>
+__device__ __forceinline__ PairTerms<T> pair_terms(const PairMath& pm, Difference<T> u, bool want_loss, const TableMath& math) {
   PairTerms<T> t;
   if (pm.kind == PREFERENCE_SQUARED) {
-    const T d = u - (T)pm.target;
+    const T d = u.less(pm.target);
     return {(T)2 * d, (T)2, d * d};
   }
-  const T beta = (T)pm.beta, x = beta * u, e = pair_exp(-fabs(x), math), r = pair_inverse((T)1 + e), er = e * r;
+  const T beta = (T)pm.beta, x = beta * u.value(), e = pair_exp(-fabs(x), math), r = pair_inverse((T)1 + e), er = e * r;
   const T down = x >= (T)0 ? er : r;  // sig(-x)
   const T keep = (T)(1.0 - pm.smoothing);
   t.g = -(beta * keep) * down;
@@ -102,7 +119,7 @@ template <>
 struct Lean<double> {
   double v;
   __device__ __forceinline__ Lean(double s, double r) : v(s - r) {}
-  __device__ __forceinline__ double minus(const Lean& o) const { return v - o.v; }
+  __device__ __forceinline__ Difference<double> minus(const Lean& o) const { return {v - o.v}; }
 };
 template <>
 struct Lean<float> {
@@ -112,10 +129,10 @@ struct Lean<float> {
     const float b = v - s;
     err = (s - (v - b)) - (r + b);
   }
-  __device__ __forceinline__ float minus(const Lean& o) const {
+  __device__ __forceinline__ Difference<float> minus(const Lean& o) const {
     const float d = v - o.v, b = d - v;
     const float low = ((v - (d - b)) - (o.v + b)) + (err - o.err);
-    return low == low ? d + low : d;  // infinities have no error terms
+    return {d, low == low ? low : 0.0f};  // infinities have no error terms
   }
 };
 

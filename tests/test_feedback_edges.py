@@ -308,3 +308,35 @@ def test_infinite_derivatives(mtlib, K, dtype):
         assert torch.equal(G[r], torch.where(taken[r], math.inf, -math.inf).to(G.dtype))
     assert torch.isfinite(G[1::2]).all() and torch.isfinite(H[1::2]).all()
     assert torch.isfinite(loss[1::2]).all() and (loss[::2] > 1e38).all()
+
+
+# ------------------------------------------------------------------- pairs
+
+@gpu
+@pytest.mark.parametrize("beta", [0.1, 0.37, 3.0])
+@pytest.mark.parametrize("size", [1.0, 40.0, 900.0])
+def test_squared_loss_next_to_its_target(mtlib, beta, size):
+    """float32 scores and references whose difference is next to 1 / (2 beta):
+    u is known to its parts' rounding errors (2^-46 of the items' distances to
+    their references), u - 1 / (2 beta) is rounded once, and its square and
+    double once more each; float32 holds the results."""
+    import torch
+    rng = np.random.default_rng(int(size))
+    P = 4000
+    target = 1 / (2 * beta)
+    ref = (rng.normal(size=2 * P) * size - size).astype(np.float32)
+    s = (ref + rng.normal(size=2 * P)).astype(np.float32)
+    i, j = np.arange(P), P + np.arange(P)
+    lean = s.astype(np.float64) - ref
+    s[:P] = (target + lean[j] + ref[:P]).astype(np.float32)
+    step = np.abs(np.spacing(s[:P])).astype(np.float64)
+    s[:P] = (s[:P] + step * rng.integers(-3, 4, size=P)).astype(np.float32)
+    lean = s.astype(np.float64) - ref
+    plan = mtlib.PreferencePlan(i, j, 2 * P)
+    got = mtlib.preference_loss(plan, torch.from_numpy(s).cuda(), reference=torch.from_numpy(ref).cuda(), beta=beta, loss="squared")
+    d = (lean[i] - lean[j]) - target
+    off = 2.0 ** -46 * (np.abs(lean[i]) + np.abs(lean[j])) + 2.0 ** -52 * target
+    e = np.abs(d) * fu.U32 + off
+    _close(got[0], d * d, 2 * np.abs(d) * e + e * e + d * d * 2 * fu.U32 + 2.0 ** -126, "loss")
+    _close(got[1][:P], 2 * d, 2 * e + 2.0 ** -126, "grad of the winners")
+    assert torch.equal(got[1][P:], -got[1][:P]) and (got[2] == 2).all()
