@@ -79,8 +79,6 @@ struct PreferencePlan {
   // with itself, or a weight that is negative or not finite.
   static void check(const int64_t* winners, const int64_t* losers, const float* weights, long long n_pairs,
                     long long n_items);
-  // From how many pairs on an item is long.
-  static int long_from(long long n_entries, long long n_items);
   // Host arrays that passed check().  Allocates on the current device and
   // waits for the copies.
   void build(const int64_t* winners, const int64_t* losers, const float* weights, long long n_pairs,

@@ -11,6 +11,7 @@
 
 #include "feedback.h"
 #include "feedback_math.cuh"
+#include "feedback_plan.h"
 #include "trainer.h"
 
 namespace mtb {
@@ -155,25 +156,6 @@ constexpr int kPairThreads = 256;
 constexpr int kLongThreads = 128;
 constexpr int kHugeThreads = 512;
 constexpr int kPairCluster = 8;
-
-// Lanes an item, by the mean number of an item's pairs: about eight steps of a
-// lane, so that an item's own loads, sums of lanes and stores are shared by
-// few instructions (all pairs in groups of 64, float64: 53 us with 32 lanes,
-// 41 us with 8).
-int pair_lanes(long long mean) { return mean < 8 ? 1 : mean < 32 ? 4 : mean < 128 ? 8 : 32; }
-
-}  // namespace
-
-// Items of more pairs than their lanes take in 24 steps have a block to
-// themselves, or from 2048 pairs a cluster of 8: a lane's steps are one after
-// the other, and a long item in a warp would be the last to end.
-int PreferencePlan::long_from(long long n_entries, long long n_items) {
-  return 24 * pair_lanes(n_entries / std::max(1ll, n_items)) + 1;
-}
-
-namespace {
-
-constexpr int kHuge = 2048;
 
 // The launches for huge, long and other items write apart from one another,
 // so each lets the next begin at once; each ends only when the one before it
@@ -327,7 +309,7 @@ void launch_preference_t(const PreferencePlan& plan, const PreferenceTerms& t, c
   A.zero_pairs = plan.zero_pairs;
   A.n_zero = (int)plan.n_zero;
   A.n_items = (int)plan.n_items;
-  A.long_from = PreferencePlan::long_from(plan.n_entries, plan.n_items);
+  A.long_from = pairs_long_from(plan.n_entries, plan.n_items);
   A.s = static_cast<const T*>(t.scores);
   A.ref = static_cast<const T*>(t.reference);
   A.pm = {t.beta, t.smoothing, 1.0 / (2.0 * t.beta), t.kind};
@@ -379,93 +361,9 @@ void PreferencePlan::check(const int64_t* winners, const int64_t* losers, const 
   if (fault == 1) throw std::invalid_argument("pair weights must be finite and non-negative");
 }
 
-// Two passes of a counting sort, both in the pairs' order and on all host
-// threads: pairs into ranges of items, then each range's by item, within a
-// core's cache.
 void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const float* weights, long long np,
                            long long ni) {
-  struct Entry {
-    int item;
-    int2 e;
-    float w;
-  };
-  constexpr int kRanges = 256, kMostThreads = 64;
-  const int parts = (int)std::min<long long>(kMostThreads, 1 + np / 16384);
-  const long long range = std::max<long long>(1, (ni + kRanges - 1) / kRanges);
-  std::vector<long long> count((size_t)parts * kRanges, 0), zeros(parts, 0);
-  auto slice = [&](int t) { return np * t / parts; };
-#pragma omp parallel for schedule(static, 1) if (parts > 1)
-  for (int t = 0; t < parts; ++t) {
-    long long* c = &count[(size_t)t * kRanges];
-    for (long long p = slice(t); p < slice(t + 1); ++p) {
-      if (weights && weights[p] == 0.0f) {
-        ++zeros[t];
-        continue;
-      }
-      ++c[winners[p] / range];
-      ++c[losers[p] / range];
-    }
-  }
-  std::vector<long long> start(kRanges + 1, 0), zero_at(parts + 1, 0);
-  long long total = 0;
-  for (int q = 0; q < kRanges; ++q) {
-    start[q] = total;
-    for (int t = 0; t < parts; ++t) {
-      const long long c = count[(size_t)t * kRanges + q];
-      count[(size_t)t * kRanges + q] = total;
-      total += c;
-    }
-  }
-  start[kRanges] = total;
-  for (int t = 0; t < parts; ++t) zero_at[t + 1] = zero_at[t] + zeros[t];
-  std::unique_ptr<Entry[]> sorted(new Entry[std::max(1ll, total)]);
-  std::vector<int> zero((size_t)zero_at[parts]);
-  std::unique_ptr<int[]> off(new int[(size_t)ni + 1]);
-  std::unique_ptr<int2[]> ent(new int2[std::max(1ll, total)]);
-  std::unique_ptr<float[]> ew(new float[weights ? std::max(1ll, total) : 1]);
-#pragma omp parallel for schedule(static, 1) if (parts > 1)
-  for (int t = 0; t < parts; ++t) {
-    long long* c = &count[(size_t)t * kRanges];
-    long long z = zero_at[t];
-    for (long long p = slice(t); p < slice(t + 1); ++p) {
-      const int a = (int)winners[p], b = (int)losers[p];
-      const float w = weights ? weights[p] : 1.0f;
-      if (w == 0.0f) {
-        zero[z++] = (int)p;
-        continue;
-      }
-      sorted[c[a / range]++] = {a, make_int2(b, (int)p), w};
-      sorted[c[b / range]++] = {b, make_int2(a | (int)0x80000000, (int)p), w};
-    }
-  }
-  const int from = long_from(total, ni);
-  std::vector<int> lng_of[kRanges], huge_of[kRanges];
-#pragma omp parallel for schedule(dynamic, 1) if (parts > 1)
-  for (int q = 0; q < kRanges; ++q) {
-    const long long i0 = std::min(ni, q * range), i1 = std::min(ni, i0 + range);
-    if (i0 >= i1) continue;
-    std::vector<int> at((size_t)(i1 - i0) + 1, 0);
-    for (long long e = start[q]; e < start[q + 1]; ++e) ++at[sorted[e].item - i0 + 1];
-    int sum = (int)start[q];
-    for (long long i = i0; i < i1; ++i) {
-      off[i] = sum;
-      const int n = at[i - i0 + 1];
-      at[i - i0] = sum;
-      sum += n;
-      if (n >= from) (n >= std::max(kHuge, from) ? huge_of : lng_of)[q].push_back((int)i);
-    }
-    for (long long e = start[q]; e < start[q + 1]; ++e) {
-      const int to = at[sorted[e].item - i0]++;
-      ent[to] = sorted[e].e;
-      if (weights) ew[to] = sorted[e].w;
-    }
-  }
-  off[ni] = (int)total;
-  std::vector<int> lng, huge;
-  for (int q = 0; q < kRanges; ++q) {
-    lng.insert(lng.end(), lng_of[q].begin(), lng_of[q].end());
-    huge.insert(huge.end(), huge_of[q].begin(), huge_of[q].end());
-  }
+  const SortedPairs s = sort_pairs(winners, losers, weights, np, ni);
   // one allocation, each array on 256 bytes
   MTB_CUDA_FB(cudaGetDevice(&device));
   size_t bytes = 0;
@@ -479,9 +377,11 @@ void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const 
     bytes += (n + 255) / 256 * 256;
     return copies.back().at;
   };
-  const size_t at_off = add(off.get(), 4 * ((size_t)ni + 1)), at_ent = add(ent.get(), 8 * (size_t)total),
-               at_w = add(ew.get(), weights ? 4 * (size_t)total : 0), at_zero = add(zero.data(), 4 * zero.size()),
-               at_long = add(lng.data(), 4 * lng.size()), at_huge = add(huge.data(), 4 * huge.size());
+  const size_t at_off = add(s.offsets.get(), 4 * ((size_t)ni + 1)), at_ent = add(s.entries.get(), 8 * (size_t)s.n_entries),
+               at_w = add(s.weights.get(), weights ? 4 * (size_t)s.n_entries : 0),
+               at_zero = add(s.zero_pairs.get(), 4 * (size_t)s.n_zero),
+               at_long = add(s.long_items.get(), 4 * (size_t)s.n_long),
+               at_huge = add(s.huge_items.get(), 4 * (size_t)s.n_huge);
   memory_bytes = bytes;
   memory = take_device_memory(&memory_bytes);
   char* base = static_cast<char*>(memory);
@@ -502,10 +402,10 @@ void PreferencePlan::build(const int64_t* winners, const int64_t* losers, const 
   }
   n_items = ni;
   n_pairs = np;
-  n_entries = total;
-  n_zero = (long long)zero.size();
-  n_long = (long long)lng.size();
-  n_huge = (long long)huge.size();
+  n_entries = s.n_entries;
+  n_zero = s.n_zero;
+  n_long = s.n_long;
+  n_huge = s.n_huge;
   offsets = reinterpret_cast<int*>(base + at_off);
   entries = reinterpret_cast<int2*>(base + at_ent);
   entry_w = weights ? reinterpret_cast<float*>(base + at_w) : nullptr;
