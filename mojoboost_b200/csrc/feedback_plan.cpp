@@ -77,9 +77,13 @@ SortedPairs sort_pairs(const int64_t* winners, const int64_t* losers, const floa
     if (i0 >= i1) continue;
     // the range's offsets count its items' entries, then say where each item's
     // next entry goes, and are put back at the end
-    int* at = &s.offsets[i0];
+    int* const at = &s.offsets[i0];
+    int2* const entries = s.entries.get();
+    float* const entry_w = s.weights.get();
+    const Entry* const first = &sorted[start[q]];
+    const Entry* const last = first + (start[q + 1] - start[q]);
     std::fill(at, at + (i1 - i0), 0);
-    for (long long e = start[q]; e < start[q + 1]; ++e) ++at[sorted[e].item - i0];
+    for (const Entry* e = first; e < last; ++e) ++at[e->item - i0];
     int sum = (int)start[q];
     for (long long i = 0; i < i1 - i0; ++i) {
       const int n = at[i];
@@ -87,10 +91,10 @@ SortedPairs sort_pairs(const int64_t* winners, const int64_t* losers, const floa
       sum += n;
       if (n >= from) ++(n >= huge_from ? n_huge : n_long)[q];
     }
-    for (long long e = start[q]; e < start[q + 1]; ++e) {
-      const int to = at[sorted[e].item - i0]++;
-      s.entries[to] = sorted[e].e;
-      if (weights) s.weights[to] = sorted[e].w;
+    for (const Entry* e = first; e < last; ++e) {
+      const int to = at[e->item - i0]++;
+      entries[to] = e->e;
+      if (entry_w) entry_w[to] = e->w;
     }
     for (long long i = i1 - i0 - 1; i > 0; --i) at[i] = at[i - 1];
     at[0] = (int)start[q];
