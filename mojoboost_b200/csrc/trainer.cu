@@ -72,7 +72,9 @@ class DeviceCache {
     static DeviceCache c;
     return c;
   }
-  void* take(size_t bytes) {
+  // `bytes` becomes the size of the block that is handed out, which is what it
+  // is given back with.
+  void* take(size_t& bytes) {
     int dev = 0;
     MTB_CUDA(cudaGetDevice(&dev));
     {
@@ -84,8 +86,10 @@ class DeviceCache {
         it = m.erase(it);
         held_[dev] -= sz;
         cudaPointerAttributes a;
-        if (cudaPointerGetAttributes(&a, p) == cudaSuccess && a.type == cudaMemoryTypeDevice && a.device == dev)
+        if (cudaPointerGetAttributes(&a, p) == cudaSuccess && a.type == cudaMemoryTypeDevice && a.device == dev) {
+          bytes = sz;
           return p;
+        }
         cudaGetLastError();  // a block from a context that no longer exists: dropped
       }
     }

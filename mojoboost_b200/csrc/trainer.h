@@ -62,8 +62,9 @@ struct BinnedInput {
 void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model);
 
 // Device memory of the per-process cache that fits take theirs from, on the
-// current device: `bytes` is rounded up to what the block holds.  Returning a
-// block, on the device it came from, waits for the device's work.
+// current device: `bytes` becomes the size of the block, 2 MB at least, which
+// it is returned with.  Returning a block, on the device it came from, waits
+// for the device's work.
 void* take_device_memory(size_t* bytes);
 void give_device_memory(void* p, size_t bytes);
 

@@ -50,6 +50,31 @@ def test_plan_is_there_for_any_stream(mtlib, n, P, turns):
         assert (np.abs(grad.cpu().numpy() - G) <= tol).all(), turn
 
 
+@gpu
+def test_recycled_memory_keeps_its_size():
+    """A plan that takes a somewhat larger block of recycled memory gives all
+    of it back: the next plan of the larger size needs no new memory."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import numpy as np, torch
+import mojoboost_b200 as mb
+def plan(pairs):  # 16 bytes a pair: 9 and 8 units of 2 MB
+    i = np.arange(pairs) % 999
+    mb.PreferencePlan(i, i + 1, 1000)
+    torch.cuda.synchronize()
+    return torch.cuda.mem_get_info()[0]
+torch.zeros(1, device="cuda")
+large = plan(1_150_000)
+assert plan(1_000_000) == large, "the block was not recycled"
+print("free", large - plan(1_150_000))
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.split() == ["free", "0"], r.stdout + r.stderr
+
+
 # ------------------------------------------------------------------- masks
 
 def _bounds(z, a, f64):
