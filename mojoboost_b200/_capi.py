@@ -135,7 +135,7 @@ class _Err:
 
     def check(self, rc):
         if rc != OK:
-            msg = lib().mojotrees_error_message(self.h).decode()
+            msg = lib().mojotrees_error_message(self.h).decode(errors="replace")
             cls = UnsupportedError if rc == ERROR_UNSUPPORTED else MojoTreesError
             raise cls(rc, msg)
 

@@ -75,6 +75,14 @@ print("free", large - plan(1_150_000))
     assert r.returncode == 0 and r.stdout.split() == ["free", "0"], r.stdout + r.stderr
 
 
+# -------------------------------------------------------------- parameters
+
+def test_refused_bytes_in_a_message(mtlib):
+    """A parameter that is not UTF-8 is refused as any other wrong one."""
+    with pytest.raises(mtlib.MojoTreesError, match="integer"):
+        mtlib.train_dense(np.arange(8.0).reshape(4, 2), np.zeros(4), b"num_leaves=\xff")
+
+
 # ------------------------------------------------------------------- masks
 
 def _bounds(z, a, f64):
