@@ -15,6 +15,7 @@ is 0 or every score is -inf; an action of n_classes or more gives NaN there.
 torch is imported by the first call on device scores.
 """
 import ctypes
+import re
 import threading
 
 import numpy as np
@@ -225,17 +226,18 @@ def _scores_array(v, n):
 
 
 def _num_class(params):
-    """num_class of the parameters, 1 when they do not give it."""
-    for token in params_string(params).decode().split():
-        key, _, value = token.partition("=")
-        if key.lower() in ("num_class", "num_classes") and value.lstrip("-").isdigit():
-            return int(value)
+    """num_class of the parameters as the library reads it: 1 when they do not
+    give it, None when it is not an integer (which the library refuses)."""
+    for token in params_string(params).split():
+        key, _, value = token.partition(b"=")
+        if key.lower() in (b"num_class", b"num_classes"):
+            return int(value) if re.fullmatch(rb"[+-]?[0-9]+", value) else None
     return 1
 
 
 def _check_initial(initial, params):
     k = _num_class(params)
-    if initial is not None and (1 if initial.ndim == 1 else initial.shape[1]) != max(k, 1):
+    if initial is not None and k is not None and (1 if initial.ndim == 1 else initial.shape[1]) != max(k, 1):
         raise _invalid(f"initial_scores must have num_class = {max(k, 1)} values a row, got shape {initial.shape}")
     return initial
 

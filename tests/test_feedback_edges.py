@@ -82,6 +82,23 @@ def test_refused_bytes_in_a_message(mtlib):
     with pytest.raises(mtlib.MojoTreesError, match="integer"):
         mtlib.train_dense(np.arange(8.0).reshape(4, 2), np.zeros(4), b"num_leaves=\xff")
 
+@pytest.mark.parametrize("params,k", [
+    (None, 1), ("num_iterations=3", 1), ("num_class=3", 3), ({"num_classes": 3}, 3), (b"NUM_CLASS=3", 3), ("num_class=+3", 3),
+    ("num_class=-3", -3), ("num_class=003", 3), ("num_class=3.0", None), ("num_class=--3", None), ("num_class=", None),
+    ("num_class=\u0663", None), (b"num_class=\xff", None), ("verbosity=1\x0bnum_class=3", 3)])
+def test_num_class_is_read_as_the_library_does(mtlib, params, k):
+    from mojoboost_b200 import _feedback
+    assert _feedback._num_class(params) == k
+    X, zeros = np.arange(8.0).reshape(4, 2), np.zeros((4, 3))
+    if k == 3:  # initial scores of that width are accepted (what remains is a device)
+        if not mtlib.gpu_available():
+            with pytest.raises(mtlib.UnsupportedError, match="CUDA"):
+                mtlib.train_dense_policy(X, [0, 1, 2, 0], np.ones(4), params, initial_scores=zeros)
+    else:
+        with pytest.raises(mtlib.MojoTreesError, match="initial_scores" if k is not None else "integer") as e:
+            mtlib.train_dense_policy(X, [0, 1, 2, 0], np.ones(4), params, initial_scores=zeros)
+        assert e.value.code == -1
+
 
 # ------------------------------------------------------------------- masks
 
