@@ -1,5 +1,6 @@
 // C entry points of the losses from feedback (declared in include/mojotrees.h).
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include <algorithm>
@@ -214,6 +215,7 @@ int32_t mojotrees_b200_preference_loss(const MojoTreesPreferencePlan* plan, cons
     require(plan, "null pointer argument");
     require(score_type == mtb::SCORE_F64 || score_type == mtb::SCORE_F32, "preference scores are float64 or float32");
     require(beta > 0.0 && std::isfinite(beta), "beta must be positive");
+    require(score_type == mtb::SCORE_F64 || beta <= FLT_MAX, "beta is beyond float32 scores");
     require(label_smoothing >= 0.0 && label_smoothing <= 0.5, "label_smoothing must be in [0, 0.5]");
     require(loss_kind == mtb::PREFERENCE_LOGISTIC || loss_kind == mtb::PREFERENCE_SQUARED, "unknown preference loss");
     const mtb::PreferencePlan& p = plan->plan;

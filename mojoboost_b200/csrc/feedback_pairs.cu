@@ -84,7 +84,7 @@ __device__ __forceinline__ PairTerms<T> pair_terms(const PairMath& pm, Differenc
   const T down = x >= (T)0 ? er : r;  // sig(-x)
   const T keep = (T)(1.0 - pm.smoothing);
   t.g = -(beta * keep) * down;
-  t.h = beta * beta * er * r;
+  t.h = beta * er * (beta * r);  // beta's square may be beyond the type where this is 0
   t.loss = (T)0;
   if (want_loss) {
     const T soft = pair_log1p(e, math);

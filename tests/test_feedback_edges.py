@@ -390,3 +390,21 @@ def test_squared_loss_next_to_its_target(mtlib, beta, size):
     _close(got[0], d * d, 2 * np.abs(d) * e + e * e + d * d * 2 * fu.U32 + 2.0 ** -126, "loss")
     _close(got[1][:P], 2 * d, 2 * e + 2.0 ** -126, "grad of the winners")
     assert torch.equal(got[1][P:], -got[1][:P]) and (got[2] == 2).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,beta", [("float64", 1e160), ("float64", 1e307), ("float32", 1e20), ("float32", 1e37)])
+def test_logistic_loss_of_large_beta(mtlib, dtype, beta):
+    """A beta whose square is beyond the type: pairs that are told apart have
+    a hessian of 0 and a gradient of 0 or -beta, equal ones log 2 and -beta / 2."""
+    import torch
+    s = torch.tensor([1.0, 0.0, 0.0, 1.0, 2.0, 2.0], dtype=getattr(torch, dtype), device="cuda")
+    loss, grad, hess = mtlib.preference_loss(mtlib.PreferencePlan([0, 2, 4], [1, 3, 5], 6), s, beta=beta)
+    want = [0.0, beta, math.log(2)]
+    assert np.allclose(loss.double().cpu().numpy(), want, rtol=2.0 ** -22, atol=0)
+    big = beta if beta < 3e38 else math.inf
+    assert np.allclose(grad.double().cpu().numpy(), [0, 0, -big, big, -big / 2, big / 2], rtol=2.0 ** -22, atol=0)
+    assert hess[:4].tolist() == [0.0] * 4 and (hess[4:] > 1e38).all()
+    if dtype == "float32":
+        with pytest.raises(mtlib.MojoTreesError, match="beyond float32"):
+            mtlib.preference_loss(mtlib.PreferencePlan([0], [1], 6), s, beta=1e39)
