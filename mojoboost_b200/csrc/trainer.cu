@@ -433,10 +433,12 @@ void train_gpu(const BinnedInput& in, const TrainConfig& cfg, Model& model) {
       up(fb->weights, d_wt);
       const bool need_ref = cfg.policy_kl > 0.0 && !fb->ref_logp;
       if (!fb->old_logp || need_ref) {
-        // the policy that the fit starts from took the actions, or is the reference
+        // The policy that the fit starts from took the actions, or is the
+        // reference: its log probabilities from the loss's own arithmetic, so
+        // that the first round's ratios are 1 to the bit, inside any clip range.
         d_logp.alloc(N);
-        d_stats.alloc(2 * (size_t)N);
-        stats.kernel_launches += launch_logprobs(fb_rows, d_logp.p, d_stats.p, st);
+        const PolicyTerms t = {d_adv.p, d_adv.p, nullptr, d_wt.p, 0.0, 0.0, 0.0, nullptr, d_logp.p};
+        stats.kernel_launches += launch_policy(fb_rows, t, ScoreDerivatives{}, st);
       }
     } else {
       up(fb->reference, d_ref);

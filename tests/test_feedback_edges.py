@@ -408,3 +408,22 @@ def test_logistic_loss_of_large_beta(mtlib, dtype, beta):
     if dtype == "float32":
         with pytest.raises(mtlib.MojoTreesError, match="beyond float32"):
             mtlib.preference_loss(mtlib.PreferencePlan([0], [1], 6), s, beta=1e39)
+
+
+# -------------------------------------------------------------------- fits
+
+@gpu
+@pytest.mark.parametrize("K", [2, 5, 20])
+def test_first_round_lies_inside_any_clip_range(mtlib, K):
+    """Without old_logp the first round's ratios are 1: no row is clipped, a
+    range of no width included, and the reference is no distance away."""
+    n = 3000
+    rng = np.random.default_rng(K)
+    bins = rng.integers(0, 32, size=(5, n)).astype(np.uint8)
+    actions, adv, init = rng.integers(0, K, size=n), rng.normal(size=n), rng.normal(size=(n, K)) * 3
+    params = {"num_class": K, "num_iterations": 1, "num_leaves": 15, "min_data_in_leaf": 5, "gpu_histogram_precision": "int64"}
+    wide = mtlib.train_binned_policy(bins, 32, actions, adv, params, initial_scores=init)
+    none = mtlib.train_binned_policy(bins, 32, actions, adv, dict(params, policy_clip_low=0, policy_clip_high=0), initial_scores=init)
+    for k in range(K):
+        for name in ("feature", "threshold_bin", "count", "value"):
+            np.testing.assert_array_equal(wide.tree(k)[name], none.tree(k)[name])
