@@ -394,9 +394,12 @@ int32_t mojotrees_b200_policy_loss(const void *scores, int32_t score_type, int64
 /* The pairs of a preference loss, laid out on a device once for any number
  * of calls: item winners[p] was preferred to losers[p] (both in
  * [0, n_items), different), with weights[p] >= 0 (NULL: 1); host arrays,
- * copied.  gpu_device_id -1: the current device.  The plan is not changed by
- * calls that use it, which may overlap; free it when no graph holds one
- * (freeing waits for the device's work).  Neither may run during a capture. */
+ * copied: the plan is on the device when the call returns, for any stream.
+ * gpu_device_id -1: the current device.  The plan is not changed by calls that
+ * use it, which may overlap; free it when no graph holds one (freeing waits for
+ * the device's work).  Neither may run during a capture.  A plan takes 16
+ * bytes a pair (24 with weights) and 4 an item, in units of 2 MB; sorting the
+ * pairs on the host takes longer than tens of calls (1M pairs: 7-10 ms). */
 typedef struct MojoTreesPreferencePlan MojoTreesPreferencePlan;
 int32_t mojotrees_b200_preference_plan_create(const int64_t *winners, const int64_t *losers, const float *weights,
                                               int64_t n_pairs, int64_t n_items, int32_t gpu_device_id,
@@ -411,10 +414,11 @@ void mojotrees_b200_preference_plan_free(MojoTreesPreferencePlan *plan);
  *                                       - s log sigmoid(-beta u), s = label_smoothing
  *   MOJOTREES_B200_PREFERENCE_SQUARED   (u - 1 / (2 beta))^2, which has no use
  *                                       for label_smoothing
- * times its weight.  out_loss (scores' type [n_pairs], may be NULL) receives
- * each pair's; out_grad and out_hess (float [n_items], may both be NULL) the
- * sums over an item's pairs of the first and second derivative with respect
- * to its score, in a fixed order; 0 for an item without pairs. */
+ * times its weight; beta is positive, and within float's range for float
+ * scores.  out_loss (scores' type [n_pairs], may be NULL) receives each pair's;
+ * out_grad and out_hess (float [n_items], may both be NULL) the sums over an
+ * item's pairs of the first and second derivative with respect to its score, in
+ * a fixed order; 0 for an item without pairs. */
 #define MOJOTREES_B200_PREFERENCE_LOGISTIC 0
 #define MOJOTREES_B200_PREFERENCE_SQUARED 1
 int32_t mojotrees_b200_preference_loss(const MojoTreesPreferencePlan *plan, const void *scores, const void *reference,

@@ -8,7 +8,9 @@ scores are torch tensors on a CUDA device: the log probabilities of taken classe
 the clipped policy loss of logged decisions and the paired preference loss,
 each with its first and second derivative (include/mojotrees.h has the
 formulas).  Calls run on torch's current stream of the scores' device, do not
-wait for the device and can be captured into a CUDA graph.
+wait for the device and can be captured into a CUDA graph.  They are not
+recorded by autograd: the derivatives that a call returns are what a caller
+hands on, as in scores.backward(grad).
 
 A row takes no part, with outputs 0, when its action is negative, its weight
 is 0 or every score is -inf; an action of n_classes or more gives NaN there.
@@ -158,7 +160,8 @@ class PreferencePlan:
     """The pairs of a preference loss on a device: item winners[p] was
     preferred to losers[p], with weights[p] (default 1).  Made once from host
     arrays; any number of preference_loss calls may use it, and it has to
-    outlive them and the CUDA graphs that hold one."""
+    outlive them and the CUDA graphs that hold one.  It takes 16 bytes a pair
+    (24 with weights) and 4 an item of device memory, 2 MB at least."""
 
     def __init__(self, winners, losers, n_items, weights=None, device=None):
         w, l = _index_array("winners", winners), _index_array("losers", losers)

@@ -1,7 +1,7 @@
 // Losses that learn from feedback instead of labels: the clipped policy loss
 // of logged decisions, the paired preference loss, and the log probabilities
 // of taken classes that both start from.  Launchers shared by the C entry
-// points (feedback.cu) and the trainer.
+// points (feedback_api.cpp) and the trainer.
 #pragma once
 #include <cuda_runtime.h>
 #include <stddef.h>

@@ -15,15 +15,17 @@ namespace {
 //
 // A block (or a cluster of up to 8 of them, where a row is longer than 8192
 // vectors of 16 bytes, or rows are too few to fill the GPU) holds a row in its
-// registers: the scores are read once.  Bound are the memory system and, for
-// 16-bit scores, the exponentials, two a class (the sum's, and the gradient's
-// again: kept in float32 they would take twice the registers).  Each warp sums
-// relative to its own maximum, so one barrier joins maxima and sums; the next
-// row is fetched into L2 meanwhile.
+// registers: the scores are read once.  A class takes two exponentials (the
+// sum's, and the gradient's again: kept in float32 they would take twice the
+// registers).  Each warp sums relative to its own maximum, so one barrier joins
+// maxima and sums; the next row is fetched into L2 meanwhile.
 //
 // Measured, policy loss with gradient of 8192 x 32768 bfloat16 (1.07 GB,
-// 164 us at the copy rate): 246 us; the gradient's pass alone, which needs no
-// sum, takes 200.  Rows kept in shared memory instead, three blocks an SM,
+// 164 us at the copy rate): 233 us.  No unit is full (DRAM 55%, exponentials
+// 55%, issue slots 50%): the block waits for its row's scalars, which one warp
+// makes (a quarter of the stalls), and 64 registers a thread spill 122 bytes out
+// and 146 back in.  The gradient's pass alone, which needs no sum, takes 200, and
+// for 2047 x 50001 69 of 62 at the copy rate.  Rows kept in shared memory instead, three blocks an SM,
 // took 60% longer (more instructions a class); clusters of 2 or 4 smaller
 // blocks a row 6% and 55% longer (their barriers); 50001 classes in one block
 // of 1024 threads rather than two of 512: 129 -> 120 us.
@@ -622,6 +624,10 @@ void launch_large_t(const RowArgs<T>& A, int blocks, int per, cudaStream_t st) {
   MTB_CUDA_FB(cudaLaunchKernelEx(&lc, k_feedback_large<T, OP, HESS, THREADS, NV>, A, per));
 }
 
+// The smallest block that holds the row: as many rows as possible are under way
+// an SM.  One size up, policy loss of 200M bfloat16 scores: 200 classes 870 ->
+// 1099 us, 400 577 -> 1534, 2000 371 -> 684, 6000 270 -> 484, 12000 274 -> 366,
+// 24000 210 -> 369.
 template <typename T, int OP, bool HESS>
 void launch_large_h(const RowArgs<T>& A, int blocks, int per, cudaStream_t st) {
   if (per > 4096) launch_large_t<T, OP, HESS, 1024, 8>(A, blocks, per, st);
@@ -634,7 +640,10 @@ void launch_large_h(const RowArgs<T>& A, int blocks, int per, cudaStream_t st) {
 }
 
 // Derivatives next to each other (class_stride 1), as every caller with such
-// scores has them.
+// scores has them.  Clusters for few rows, kernel time of float16 policy rows
+// with one block a row, and with these clusters: 1 x 131072 12.2, 6.8 us; 18 x
+// 131072 12.7, 8.4; 37 x 20000 9.3, 7.3; 37 x 8000 5.3, 5.9.  From 128 vectors a
+// block on instead of 512: 37 x 2000 5.5 -> 7.2.
 template <typename T, int OP>
 void launch_large(const RowArgs<T>& A, cudaStream_t st) {
   const int vecs = A.in.K / Vec<T>::N;  // or one fewer, where a row does not start on 16 bytes

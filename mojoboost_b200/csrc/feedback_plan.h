@@ -15,7 +15,11 @@ inline int pair_lanes(long long mean) { return mean < 8 ? 1 : mean < 32 ? 4 : me
 
 // Items of more pairs than their lanes take in 24 steps have a block to
 // themselves, or from 2048 pairs a cluster of 8: a lane's steps are one after
-// the other, and a long item in a warp would be the last to end.
+// the other, and a long item in a warp would be the last to end.  Pairs of
+// popular items, 12, 24 and 48 steps: 100000 of 3000 float32 items 20.6, 21.0,
+// 30.0 us; 1M of 20000 float64 48, 46, 52; 4M of 300001 float32 122, 130, 131.
+// Clusters from 512, 2048 and 8192 pairs: 21.3, 21.0, 21.1; 58, 46, 47; 152,
+// 130, 118.
 inline int pairs_long_from(long long n_entries, long long n_items) {
   return 24 * pair_lanes(n_entries / (n_items > 1 ? n_items : 1)) + 1;
 }

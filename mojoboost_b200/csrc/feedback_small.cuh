@@ -18,9 +18,10 @@ namespace {
 // quotient, cost as much as ten classes; every lane of a row computes them.
 //
 // Measured, policy loss with gradient and hessian of 4M x 10 float64 (816 MB,
-// 125 us at the copy rate): 189 us.  Bound is the issue of instructions, 62%
-// of the slots with a quarter of the warps an SM could hold: about 1050 for 32
-// rows, a third of them float64.  A block per row took 20.2 ms; rows spread
+// 125 us at the copy rate): 190 us.  What is left is latency: 120 registers
+// leave room for a quarter of the warps an SM could hold, which fill 62% of the
+// issue slots and 47% of DRAM with about 1050 instructions for 32 rows, a third
+// of them float64.  A block per row took 20.2 ms; rows spread
 // over four lanes' registers 396 us; a branch per class 309 us, and classes
 // fixed at compile time with the next rows' copy in flight 224 us, since a
 // lane's exponentials then overlap; bulk copies and the branch-free functions
